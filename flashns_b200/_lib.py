@@ -43,6 +43,12 @@ SIGNATURES = {
     "flashns_b200_philox_points": [ctypes.c_uint64, ctypes.c_uint64, _c_int, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_ptr,
                                    _c_i64, _c_ptr],
     "flashns_b200_pack_coordinates": [_c_ptr, _c_i64, _c_i64, _c_int, _c_ptr, _c_ptr],
+    "flashns_b200_layer_norm": [_c_int] + [_c_ptr] * 5 + [_c_dbl, _c_i64, _c_i64, _c_int, _c_ptr],
+    "flashns_b200_layer_norm_vjp_scratch": [_c_int, _c_i64, _c_i64, _c_int, ctypes.POINTER(_c_size)],
+    "flashns_b200_layer_norm_vjp": [_c_int] + [_c_ptr] * 9 + [_c_size, _c_i64, _c_i64, _c_int, _c_ptr],
+    "flashns_b200_affine": [_c_int, _c_int] + [_c_ptr] * 7 + [_c_i64, _c_i64, _c_int, _c_int, _c_ptr],
+    "flashns_b200_affine_vjp_scratch": [_c_int, _c_int, _c_i64, _c_i64, _c_int, _c_int, ctypes.POINTER(_c_size)],
+    "flashns_b200_affine_vjp": [_c_int, _c_int] + [_c_ptr] * 9 + [_c_size, _c_i64, _c_i64, _c_int, _c_int, _c_ptr],
     # reference-ABI hooks (experiments/pinn_v8/native.py:26-51, experiments/cuda_jet_h100/gpu.py)
     "flashns_v8_activation": [_c_int, _c_int] + [_c_ptr] * 5 + [_c_i64, _c_i64, _c_int, _c_ptr],
     "flashns_v8_coordinate_affine": [_c_int] + [_c_ptr] * 4 + [_c_i64, _c_i64, _c_int, _c_ptr],

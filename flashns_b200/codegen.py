@@ -1,6 +1,6 @@
 """Emit the straight-line device math for jets and residual seeds.
 
-The generated headers ``csrc/jets_generated.cuh`` and
+The generated headers ``csrc/jets_generated.cuh``, ``csrc/products_generated.cuh`` and
 ``csrc/residual_generated.cuh`` are committed; ``python -m flashns_b200.codegen``
 rewrites them and ``tests/test_codegen.py`` checks that they are current.
 
@@ -153,6 +153,55 @@ def jets_header():
     return "\n\n".join(parts) + "\n"
 
 
+# ----------------------------------------------------------------- truncated products
+
+def jet_products(dim):
+    """Order-3 products the layer norm is written in: square, product, its adjoint, 1/sqrt."""
+    b = basis(dim)
+    q, pr = len(b), pairs(dim, 3)
+    low = [i for i, a in enumerate(b) if sum(a) == 1]
+
+    def function(name, arguments, what, body):
+        return "\n".join([f"// {what}, dim {dim}", f"__device__ __forceinline__ void {name}_{dim}d3({arguments}) {{",
+                          *body, "}"])
+
+    square = [f"  v[{g}] = {_sym_sum(pr[g], lambda i, j: f'd[{i}] * d[{j}]')};" for g in range(q)]
+    mul = [f"  out[{g}] = {' + '.join(f'a[{i}] * b[{j}]' for i, j in pr[g])};" for g in range(q)]
+
+    def adjoint(beta):
+        return " + ".join(f"a[{i}] * s[{alpha}]" for alpha in range(q) for i, j in pr[alpha] if j == beta)
+
+    # n = v / v_0 - 1 has no order-0 coefficient: n^2 starts at order 2, n^3 at order 3
+    rsqrt = ["  const double r0 = 1.0 / sqrt(v[0]);", "  const double w = r0 * r0;"]
+    rsqrt += [f"  const double n{g} = v[{g}] * w;" for g in range(1, q)]
+    for g, a in enumerate(b):
+        if sum(a) >= 2:
+            terms = [(i, j) for i, j in pr[g] if i and j]
+            rsqrt.append(f"  const double s{g} = {_sym_sum(terms, lambda i, j: f'n{i} * n{j}')};")
+    rsqrt.append("  r[0] = r0;")
+    for g, a in enumerate(b[1:], 1):
+        expr = f"-0.5 * n{g}"
+        if sum(a) >= 2:
+            expr += f" + 0.375 * s{g}"
+        if sum(a) == 3:
+            expr += f" - 0.3125 * ({' + '.join(f's{i} * n{j}' for i, j in pr[g] if j in low and i)})"
+        rsqrt.append(f"  r[{g}] = r0 * ({expr});")
+    return "\n\n".join([
+        function("jet_square", "const double* d, double* v", "v = d * d", square),
+        function("jet_mul", "const double* a, const double* b, double* out", "out = a * b", mul),
+        function("jet_corr", "const double* a, const double* s, double* out",
+                 "adjoint of b -> a * b at s: out_k = sum_j a_j s_(j+k)",
+                 [f"  out[{g}] = {adjoint(g)};" for g in range(q)]),
+        function("jet_corr_add", "const double* a, const double* s, double* out", "out_k += sum_j a_j s_(j+k)",
+                 [f"  out[{g}] += {adjoint(g)};" for g in range(q)]),
+        function("jet_rsqrt", "const double* v, double* r", "r = v^(-1/2), v_0 > 0", rsqrt)])
+
+
+def products_header():
+    parts = ["// GENERATED by flashns_b200/codegen.py -- do not edit.", "#pragma once", "namespace flashns_b200 {"]
+    return "\n\n".join(parts + [jet_products(dim) for dim in (2, 3)] + ["}  // namespace flashns_b200"]) + "\n"
+
+
 # ----------------------------------------------------------------- residual polynomials
 # expression: {factors(tuple of (field, alpha)): (const, nu)}
 
@@ -299,6 +348,7 @@ def residual_header():
 
 def outputs():
     return {HERE / "csrc" / "jets_generated.cuh": jets_header(),
+            HERE / "csrc" / "products_generated.cuh": products_header(),
             HERE / "csrc" / "residual_generated.cuh": residual_header()}
 
 

@@ -1,0 +1,97 @@
+// What the layer operators (norm.cu, affine.cu) share: packed units, jet products by
+// dimension, fixed-order sums over lanes, argument checks.
+#pragma once
+#include <climits>
+#include <cstddef>
+#include <cstdint>
+
+#include "common.cuh"
+#include "products_generated.cuh"
+
+namespace flashns_b200 {
+
+// A unit is Q consecutive packed rows: the jet of one full point, or up to Q value rows
+// (each a point of its own).  Both load and store alike.
+struct Packed {
+  int64_t full, value;  // points
+  template <int Q>
+  __host__ __device__ int64_t units() const { return full + (value + Q - 1) / Q; }
+  template <int Q>
+  __host__ __device__ int64_t row(int64_t u) const { return u * Q; }  // full points' rows come first
+  template <int Q>
+  __host__ __device__ int count(int64_t u) const {  // live rows of unit u
+    if (u < full) return Q;
+    const int64_t left = value - (u - full) * Q;
+    return int(left < Q ? left : Q);
+  }
+};
+
+template <int DIM>
+struct Jet {
+  static constexpr int Q = Basis<DIM>::Q;
+  static __device__ __forceinline__ void square(const double* d, double* v) {
+    if constexpr (DIM == 2) jet_square_2d3(d, v); else jet_square_3d3(d, v);
+  }
+  static __device__ __forceinline__ void mul(const double* a, const double* b, double* out) {
+    if constexpr (DIM == 2) jet_mul_2d3(a, b, out); else jet_mul_3d3(a, b, out);
+  }
+  static __device__ __forceinline__ void corr(const double* a, const double* s, double* out) {
+    if constexpr (DIM == 2) jet_corr_2d3(a, s, out); else jet_corr_3d3(a, s, out);
+  }
+  static __device__ __forceinline__ void corr_add(const double* a, const double* s, double* out) {
+    if constexpr (DIM == 2) jet_corr_add_2d3(a, s, out); else jet_corr_add_3d3(a, s, out);
+  }
+  static __device__ __forceinline__ void rsqrt(const double* v, double* r) {
+    if constexpr (DIM == 2) jet_rsqrt_2d3(v, r); else jet_rsqrt_3d3(v, r);
+  }
+};
+
+// Sums of N values over 2 * O lanes, left in every lane.  Each step halves the values a lane
+// carries (it keeps one half and gives the other away), so N values over 32 lanes take about
+// 2 N shuffles in place of 5 N; the way back hands the sums out.  Every lane gets the same
+// bits, in an order fixed by the lane numbers.
+template <int N, int O>
+__device__ __forceinline__ void lane_sums(double* v) {
+  if constexpr (O == 0) {
+    return;
+  } else if constexpr (N == 1) {
+    v[0] += __shfl_xor_sync(0xffffffffu, v[0], O);
+    lane_sums<1, O / 2>(v);
+  } else {
+    constexpr int H = (N + 1) / 2;
+    const bool up = (threadIdx.x & O) != 0;
+#pragma unroll
+    for (int i = 0; i < H; ++i) {
+      const double lo = v[i], hi = i + H < N ? v[i + H] : 0.0;
+      v[i] = (up ? hi : lo) + __shfl_xor_sync(0xffffffffu, up ? lo : hi, O);
+    }
+    lane_sums<H, O / 2>(v);
+#pragma unroll
+    for (int i = 0; i < H; ++i) {
+      const double other = __shfl_xor_sync(0xffffffffu, v[i], O), mine = v[i];
+      v[i] = up ? other : mine;
+      if (i + H < N) v[i + H] = up ? mine : other;
+    }
+  }
+}
+
+inline bool layer_sizes_ok(int dim, int64_t full, int64_t value, int widest) {
+  if ((dim != 2 && dim != 3) || full < 0 || value < 0 || widest < 1) return false;
+  const int64_t q = dim == 2 ? 10 : 20;
+  // rows <= full * q + value, padded by one unit; offsets in bytes stay in 64 bits
+  if (full > (INT64_MAX - value - q) / q) return false;
+  return full * q + value + q <= INT64_MAX / int64_t(sizeof(double)) / widest / 2;
+}
+
+inline bool ranges_overlap(const void* a, size_t na, const void* b, size_t nb) {
+  const auto pa = reinterpret_cast<uintptr_t>(a), pb = reinterpret_cast<uintptr_t>(b);
+  return a && b && na && nb && (pa <= pb ? pb - pa < na : pa - pb < nb);
+}
+
+inline cudaError_t sm_count(int* sms) {
+  int device = 0;
+  const cudaError_t e = cudaGetDevice(&device);
+  return e != cudaSuccess ? e : cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, device);
+}
+
+}  // namespace flashns_b200

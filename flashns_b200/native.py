@@ -42,6 +42,20 @@ def _check(tensors):
             raise NotImplementedError("manual parameter VJP; double backward/HVP unsupported")
 
 
+def _scratch(name, like, *sizes):
+    """Scratch of the size that entry point ``name`` gives for these sizes, on ``like``'s device."""
+    size = ctypes.c_size_t()
+    with torch.cuda.device(like.device):
+        _lib.check(getattr(_lib.library(), name)(*sizes, ctypes.byref(size)), name)
+    return like.new_empty((size.value + 7) // 8)
+
+
+def _affine_shape(hidden, weight):
+    if weight.ndim != 2 or weight.shape[0] < 1 or weight.shape[1] != hidden.shape[1]:
+        raise ValueError("expected H[rows,Cin], W[Cout,Cin]")
+    return weight.shape
+
+
 class _PackedActivation:
     def __init__(self, layout):
         self.layout = layout
@@ -176,6 +190,101 @@ class NativeCUDA:
                  loss.gradient_weight, loss.boundary_weight], (jets, pde_weights, boundary_weights, target, di, db,
                                                                partial))
         return partial.sum(), di, db
+
+
+    def layer_norm(self, layout, value, gain, bias, *, eps=1e-5):
+        """Layer norm over the channels, carried through the jets: ``(out, stats)``.
+
+        The order-0 row of a point is its ordinary layer norm; the other rows are the exact
+        Taylor coefficients of the normalized field.  ``stats[rows, 2]`` holds each row's mean
+        and reciprocal-deviation coefficients for ``layer_norm_vjp``."""
+        _check((value, gain, bias))
+        layout.check(value)
+        channels = value.shape[1]
+        if gain.shape != (channels,) or bias.shape != (channels,):
+            raise ValueError("expected gain[C], bias[C]")
+        eps = float(eps)
+        if not 0.0 < eps <= 1e300:
+            raise ValueError("positive finite eps required")
+        out, stats = torch.empty_like(value), value.new_empty((layout.rows, 2))
+        _launch("flashns_b200_layer_norm", [layout.dimension, *map(_ptr, (value, gain, bias, out, stats)), eps,
+                                            layout.full_points, layout.value_points, channels],
+                (value, gain, bias, out, stats))
+        return out, stats
+
+    def layer_norm_vjp(self, layout, value, gain, stats, seed, *, skip=None):
+        """``(d_value, d_gain, d_bias)`` of ``layer_norm`` at ``seed``; ``skip`` is added to ``d_value``
+        (the gradient that reaches ``value`` past the norm, in a residual block)."""
+        given = (value, gain, stats, seed) if skip is None else (value, gain, stats, seed, skip)
+        _check(given)
+        layout.check(value)
+        channels = value.shape[1]
+        if gain.shape != (channels,) or stats.shape != (layout.rows, 2) or seed.shape != value.shape \
+                or (skip is not None and skip.shape != value.shape):
+            raise ValueError("expected X/bar_Y[rows,C], gain[C], stats[rows,2]")
+        out, dgain, dbias = torch.empty_like(value), torch.empty_like(gain), torch.empty_like(gain)
+        scratch = _scratch("flashns_b200_layer_norm_vjp_scratch", value, layout.dimension, layout.full_points,
+                           layout.value_points, channels)
+        _launch("flashns_b200_layer_norm_vjp",
+                [layout.dimension, *map(_ptr, (value, gain, stats, seed, skip, out, dgain, dbias, scratch)),
+                 scratch.numel() * 8, layout.full_points, layout.value_points, channels],
+                (*given, out, dgain, dbias, scratch))
+        return out, dgain, dbias
+
+    def affine(self, layout, hidden, weight, bias, *, residual=None):
+        """``H W^T`` with the bias on order-0 rows, plus ``residual``."""
+        return self._affine(layout, hidden, weight, bias, residual, activation=False, keep=False)
+
+    def affine_activation(self, layout, hidden, weight, bias, *, residual=None, keep=True):
+        """The stable tanh jet of ``H W^T + b``, plus ``residual``: ``(out, activated, aux)`` with what
+        ``affine_activation_vjp`` needs, or ``out`` alone when not ``keep``.  Without a residual
+        ``activated`` is ``out``."""
+        return self._affine(layout, hidden, weight, bias, residual, activation=True, keep=keep)
+
+    def _affine(self, layout, hidden, weight, bias, residual, *, activation, keep):
+        given = (hidden, weight, bias) if residual is None else (hidden, weight, bias, residual)
+        _check(given)
+        layout.check(hidden)
+        cout, cin = _affine_shape(hidden, weight)
+        if bias.shape != (cout,) or (residual is not None and residual.shape != (layout.rows, cout)):
+            raise ValueError("expected H[rows,Cin], W[Cout,Cin], bias[Cout], residual[rows,Cout]")
+        out = hidden.new_empty((layout.rows, cout))
+        aux = hidden.new_empty((layout.points, cout)) if keep else None
+        activated = torch.empty_like(out) if keep and residual is not None else None
+        _launch("flashns_b200_affine",
+                [layout.dimension, int(activation), *map(_ptr, (hidden, weight, bias, residual, out, activated, aux)),
+                 layout.full_points, layout.value_points, cin, cout], (*given, out, activated, aux))
+        return (out, out if activated is None else activated, aux) if keep else out
+
+    def affine_vjp(self, layout, hidden, weight, seed):
+        """``(d_hidden, d_weight, d_bias)`` of ``affine`` at ``seed`` (which is the residual's gradient too)."""
+        return self._affine_vjp(layout, hidden, weight, None, None, seed)
+
+    def affine_activation_vjp(self, layout, hidden, weight, activated, aux, seed):
+        """``(d_hidden, d_weight, d_bias)`` of ``affine_activation`` at ``seed`` (which is the residual's
+        gradient too)."""
+        _check((activated, aux, seed))
+        if activated.shape != seed.shape or aux.shape != (layout.points, seed.shape[-1]):
+            raise ValueError("auxiliary/adjoint shape mismatch")
+        return self._affine_vjp(layout, hidden, weight, activated, aux, seed)
+
+    def _affine_vjp(self, layout, hidden, weight, activated, aux, seed):
+        given = (hidden, weight, seed) if activated is None else (hidden, weight, seed, activated, aux)
+        _check(given)
+        layout.check(hidden)
+        layout.check(seed)
+        cout, cin = _affine_shape(hidden, weight)
+        if seed.shape[1] != cout:
+            raise ValueError("expected H[rows,Cin], W[Cout,Cin], bar_Y[rows,Cout]")
+        activation = int(activated is not None)
+        out, dw, db = torch.empty_like(hidden), torch.empty_like(weight), weight.new_empty((cout,))
+        scratch = _scratch("flashns_b200_affine_vjp_scratch", hidden, layout.dimension, activation,
+                           layout.full_points, layout.value_points, cin, cout)
+        _launch("flashns_b200_affine_vjp",
+                [layout.dimension, activation,
+                 *map(_ptr, (hidden, weight, activated, aux, seed, out, dw, db, scratch)), scratch.numel() * 8,
+                 layout.full_points, layout.value_points, cin, cout], (*given, out, dw, db, scratch))
+        return out, dw, db
 
 
 class Native:

@@ -196,6 +196,41 @@ int flashns_stable_dgrad_vjp(int dim, bool fused, const double* d, const double*
 int flashns_b200_residuals(int head, int dim, const double* jets, double nu, double* out, int64_t n,
                            cudaStream_t stream);
 
+/* ---- layers of a pre-norm residual network on packed jets (norm.cu, affine.cu) ----
+ * No reference counterpart.  Rows are packed as in PackedLayout: full_points x Q, then
+ * value_points; FP64, contiguous, any channel counts >= 1.  An output may not overlap an
+ * input.  Sums run in a fixed order: equal inputs give equal bits.
+ *
+ * Layer norm over the channels, exact through the jets: D = X - mean, r = (mean D * D +
+ * eps)^(-1/2) with the truncated product *, out = gain (r * D) + bias (order-0 rows); a value
+ * row is normalized alone.  stats [rows][2] = (mean, r) of every row.  eps > 0. */
+int flashns_b200_layer_norm(int dim, const double* value, const double* gain, const double* bias, double* out,
+                            double* stats, double eps, int64_t full_points, int64_t value_points, int channels,
+                            cudaStream_t stream);
+/* Adjoint at seed = dL/d out: d_value (plus skip, unless NULL: the gradient that reaches
+ * `value` past the norm), d_gain, d_bias.  The scratch's size depends on the current device. */
+int flashns_b200_layer_norm_vjp_scratch(int dim, int64_t full_points, int64_t value_points, int channels,
+                                        size_t* bytes);
+int flashns_b200_layer_norm_vjp(int dim, const double* value, const double* gain, const double* stats,
+                                const double* seed, const double* skip, double* d_value, double* d_gain,
+                                double* d_bias, double* scratch, size_t scratch_bytes, int64_t full_points,
+                                int64_t value_points, int channels, cudaStream_t stream);
+/* Z = hidden weight^T (weight [cout][cin]), + bias on order-0 rows; activation = 1: A = the
+ * stable tanh jet of Z and aux = sech^2 Z_0; out = A (or Z) + residual (unless NULL).
+ * activated [rows][cout] = A and aux [points][cout] are written unless NULL (activation = 0
+ * has neither); without a residual, out is A and activated may stay NULL. */
+int flashns_b200_affine(int dim, int activation, const double* hidden, const double* weight, const double* bias,
+                        const double* residual, double* out, double* activated, double* aux, int64_t full_points,
+                        int64_t value_points, int cin, int cout, cudaStream_t stream);
+/* Adjoint at seed = dL/d out (which is the residual's gradient too): d_hidden, d_weight,
+ * d_bias; activated and aux are the forward's (activation = 0: not read). */
+int flashns_b200_affine_vjp_scratch(int dim, int activation, int64_t full_points, int64_t value_points, int cin,
+                                    int cout, size_t* bytes);
+int flashns_b200_affine_vjp(int dim, int activation, const double* hidden, const double* weight,
+                            const double* activated, const double* aux, const double* seed, double* d_hidden,
+                            double* d_weight, double* d_bias, double* scratch, size_t scratch_bytes,
+                            int64_t full_points, int64_t value_points, int cin, int cout, cudaStream_t stream);
+
 /* Vector kernels of the device-resident L-BFGS (no reference counterpart: the reference
  * uses torch.optim.LBFGS, experiments/pinn_solver/solve.py:150-167).
  *   row_dots:      out[r] = rows[r] . v for r < k (rows [k][stride]); fixed-order reductions */
