@@ -22,55 +22,229 @@ __device__ __forceinline__ void tanh_vjp(const double* h, double a1, const doubl
   if constexpr (DIM == 2) jet_vjp_2d3(h, a1, hb, zb); else jet_vjp_3d3(h, a1, hb, zb);
 }
 
-// one thread per (unit, output channel)
+// ---------------------------------------------------------------- forward
+// Z^T = W H^T on the FP64 tensor pipe (DMMA m16n8k8): MMA M = output channels, N = packed
+// rows, K = input channels.  A warp owns 16 channels of 4 units; column 2t + e of its n8 tile
+// j is row 2j + e of unit t, so a thread's accumulators hold all Q rows of one unit for two
+// channels and the tanh jet, bias and residual run from registers.  Row g of the M tile is
+// channel 2g (g < 8) or 2(g - 8) + 1, which makes a thread's two channels neighbours: the
+// residual and the outputs move as 16-byte pairs.
+//
+// A CTA keeps a block of 64 output channels' W in shared memory and runs NG groups of 4 warps
+// that share it and nothing else: each streams its own tiles (4 units x 32 input channels a
+// stage, NS stages of cp.async) and meets only its own named barrier, so one group's epilogue
+// runs under the others' MMAs and loads.  Rows are padded to 36 doubles, W's to 2 (mod 8), and
+// a 3-D unit by 8 more: every fragment load is free of bank conflicts.
+constexpr int kFwUnits = 4, kFwKC = 32, kFwLD = kFwKC + 4, kFwCB = 64, kFwGroup = 128;
+
+template <int DIM>
+constexpr int fw_unit_stride() { return Jet<DIM>::Q * kFwLD + (DIM == 3 ? 8 : 0); }
+template <int DIM, int NG, int NS, bool STREAM>
+size_t fw_smem(int cin) {
+  const size_t ld = STREAM ? kFwKC + 2 : (size_t(cin) + kFwKC - 1) / kFwKC * kFwKC + 2;
+  return sizeof(double) * (size_t(NG) * NS * kFwUnits * fw_unit_stride<DIM>() + kFwCB * ld * (STREAM ? NG * NS : 1));
+}
+
+__device__ __forceinline__ void cp_async8(void* smem, const void* gmem, bool valid) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;\n" ::"r"(smem_u32(smem)), "l"(gmem), "r"(valid ? 8 : 0));
+}
+
+// W rows c0 .. c0 + 63, columns k0 .. k0 + width - 1 into dst [64][ld], zero past the ends
+__device__ __forceinline__ void load_weight(double* dst, int ld, const double* __restrict__ w, int c0, int k0, int width,
+                                            int cin, int cout, bool vec, int tid, int threads) {
+  if (vec) {
+    const int half = width / 2;
+    for (int e = tid; e < kFwCB * half; e += threads) {
+      const int r = e / half, k = k0 + 2 * (e % half);
+      const bool ok = c0 + r < cout && k < cin;
+      cp_async16(dst + r * ld + k - k0, ok ? w + int64_t(c0 + r) * cin + k : w, ok);
+    }
+  } else {
+    for (int e = tid; e < kFwCB * width; e += threads) {
+      const int r = e / width, k = k0 + e % width;
+      const bool ok = c0 + r < cout && k < cin;
+      cp_async8(dst + r * ld + k - k0, ok ? w + int64_t(c0 + r) * cin + k : w, ok);
+    }
+  }
+}
+
+// the accumulators of unit u, channels c and c + 1, through bias, tanh jet and residual
 template <int DIM, bool ACT>
-__global__ void __launch_bounds__(kAffThreads)
-    affine_forward(const double* __restrict__ hidden, const double* __restrict__ weight, const double* __restrict__ bias,
-                   const double* __restrict__ residual, double* __restrict__ out, double* __restrict__ activated,
-                   double* __restrict__ aux, Packed rows, int cin, int cout) {
+__device__ __forceinline__ void forward_epilogue(const double (&acc)[Jet<DIM>::Q / 2][4], double b0, double b1, int64_t u,
+                                                 int c, const Packed& rows, int cout,
+                                                 const double* __restrict__ residual, double* __restrict__ out,
+                                                 double* __restrict__ activated, double* __restrict__ aux, bool vec) {
   constexpr int Q = Jet<DIM>::Q;
-  const int64_t total = rows.units<Q>() * cout;
-  for (int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += int64_t(gridDim.x) * blockDim.x) {
-    const int64_t u = i / cout;
-    const int c = int(i % cout), n = rows.count<Q>(u);
-    const bool full = u < rows.full;
-    const int64_t row = rows.row<Q>(u);
-    double z[Q], h[Q];
+  const bool full = u < rows.full, two = c + 1 < cout;
+  const int n = rows.count<Q>(u);
+  const int64_t at = rows.row<Q>(u) * cout + c;
+  double h0[Q], h1[Q], a0, a1;
 #pragma unroll
-    for (int s = 0; s < Q; ++s) z[s] = 0.0;
-    for (int k = 0; k < cin; ++k) {
-      const double w = weight[int64_t(c) * cin + k];
+  for (int s = 0; s < Q; ++s) {
+    h0[s] = acc[s >> 1][s & 1] + (s == 0 || !full ? b0 : 0.0);
+    h1[s] = acc[s >> 1][2 + (s & 1)] + (s == 0 || !full ? b1 : 0.0);
+  }
+  if constexpr (ACT) {
+    if (full) {
+      tanh_forward<DIM>(h0, h0, a0);
+      tanh_forward<DIM>(h1, h1, a1);
+      if (aux) {
+        aux[u * cout + c] = a0;
+        if (two) aux[u * cout + c + 1] = a1;
+      }
+    } else {
+      double* ax = aux ? aux + (rows.full + (u - rows.full) * Q) * cout + c : nullptr;
 #pragma unroll
-      for (int s = 0; s < Q; ++s)
-        if (s < n) z[s] += w * hidden[(row + s) * cin + k];
-    }
-    const double b = bias[c];
-#pragma unroll
-    for (int s = 0; s < Q; ++s) {
-      if (s == 0 || !full) z[s] += b;
-      h[s] = z[s];
-    }
-    if constexpr (ACT) {
-      if (full) {
-        double a1;
-        tanh_forward<DIM>(z, h, a1);
-        if (aux) aux[u * cout + c] = a1;
-      } else {
-#pragma unroll
-        for (int s = 0; s < Q; ++s) {
-          double a1;
-          jet_fwd_2d0(z + s, h + s, a1);
-          if (aux && s < n) aux[(rows.full + (u - rows.full) * Q + s) * cout + c] = a1;
+      for (int s = 0; s < Q; ++s) {
+        jet_fwd_2d0(h0 + s, h0 + s, a0);
+        jet_fwd_2d0(h1 + s, h1 + s, a1);
+        if (ax && s < n) {
+          ax[int64_t(s) * cout] = a0;
+          if (two) ax[int64_t(s) * cout + 1] = a1;
         }
       }
     }
+  }
 #pragma unroll
-    for (int s = 0; s < Q; ++s) {
-      if (s >= n) continue;
-      const int64_t at = (row + s) * cout + c;
-      if (activated) activated[at] = h[s];
-      out[at] = residual ? h[s] + residual[at] : h[s];
+  for (int s = 0; s < Q; ++s) {
+    if (s >= n) continue;
+    const int64_t i = at + int64_t(s) * cout;
+    if (vec) {
+      if (activated) *reinterpret_cast<double2*>(activated + i) = make_double2(h0[s], h1[s]);
+      if (residual) {
+        const double2 r = *reinterpret_cast<const double2*>(residual + i);
+        h0[s] += r.x, h1[s] += r.y;
+      }
+      *reinterpret_cast<double2*>(out + i) = make_double2(h0[s], h1[s]);
+    } else {
+      if (activated) activated[i] = h0[s];
+      out[i] = residual ? h0[s] + residual[i] : h0[s];
+      if (two) {
+        if (activated) activated[i + 1] = h1[s];
+        out[i + 1] = residual ? h1[s] + residual[i + 1] : h1[s];
+      }
     }
+  }
+}
+
+template <int DIM, bool ACT, int NG, int NS, bool STREAM>
+__global__ void __launch_bounds__(NG* kFwGroup, 1)
+    affine_forward(const double* __restrict__ hidden, const double* __restrict__ weight, const double* __restrict__ bias,
+                   const double* __restrict__ residual, double* __restrict__ out, double* __restrict__ activated,
+                   double* __restrict__ aux, Packed rows, int cin, int cout, bool vec_in, bool vec_out) {
+  constexpr int Q = Jet<DIM>::Q, NT = Q / 2, US = fw_unit_stride<DIM>(), RT = kFwUnits * Q, KC = kFwKC;
+  extern __shared__ __align__(16) double smem[];
+  const int tid = threadIdx.x, group = tid / kFwGroup, gt = tid % kFwGroup, warp = gt >> 5;
+  const int lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int blocks = (cout + kFwCB - 1) / kFwCB, cb = blockIdx.x % blocks, c0 = cb * kFwCB;
+  const int64_t per = gridDim.x / blocks, units = rows.units<Q>(), total = rows.full * Q + rows.value;
+  const int64_t tiles = (units + kFwUnits - 1) / kFwUnits, first = blockIdx.x / blocks + group * per;
+  const int64_t mine = first < tiles ? (tiles - 1 - first) / (per * NG) + 1 : 0;
+  const int nk = (cin + KC - 1) / KC, ldw = STREAM ? KC + 2 : nk * KC + 2;
+  double* ring = smem + group * NS * kFwUnits * US;
+  double* sw = smem + NG * NS * kFwUnits * US + (STREAM ? group * NS * kFwCB * ldw : 0);
+  const int64_t steps = mine * nk;
+
+  auto load = [&](int64_t step) {
+    const int64_t r0 = (first + step / nk * per * NG) * RT;
+    const int k0 = int(step % nk) * KC, stage = int(step % NS);
+    double* dst = ring + stage * kFwUnits * US;
+    if (vec_in) {
+#pragma unroll
+      for (int e = gt; e < RT * (KC / 2); e += kFwGroup) {
+        const int r = e / (KC / 2), k = 2 * (e % (KC / 2));
+        const bool ok = r0 + r < total && k0 + k < cin;  // cin even: covers k + 1
+        cp_async16(dst + r / Q * US + r % Q * kFwLD + k, ok ? hidden + (r0 + r) * cin + k0 + k : hidden, ok);
+      }
+    } else {
+      for (int e = gt; e < RT * KC; e += kFwGroup) {
+        const int r = e / KC, k = e % KC;
+        const bool ok = r0 + r < total && k0 + k < cin;
+        cp_async8(dst + r / Q * US + r % Q * kFwLD + k, ok ? hidden + (r0 + r) * cin + k0 + k : hidden, ok);
+      }
+    }
+    if constexpr (STREAM)
+      load_weight(sw + stage * kFwCB * ldw, ldw, weight, c0, k0, KC, cin, cout, vec_in, gt, kFwGroup);
+  };
+
+  if constexpr (!STREAM) load_weight(sw, ldw, weight, c0, 0, nk * KC, cin, cout, vec_in, tid, NG * kFwGroup);
+  cp_async_commit();
+#pragma unroll
+  for (int s = 0; s < NS - 1; ++s) {
+    if (s < steps) load(s);
+    cp_async_commit();
+  }
+  cp_async_wait<NS - 1>();
+  __syncthreads();  // W is there for every group
+
+  const int ch = warp * 16 + 2 * g, c = c0 + ch;  // this thread's channels c, c + 1
+  const double b0 = c < cout ? bias[c] : 0.0, b1 = c + 1 < cout ? bias[c + 1] : 0.0;
+  double acc[NT][4];
+  for (int64_t step = 0; step < steps; ++step) {
+    const int kc = int(step % nk), stage = int(step % NS);
+    cp_async_wait<NS - 2>();
+    named_sync(1 + group, kFwGroup);  // the step's tile is there, the stage loaded next is read out
+    if (step + NS - 1 < steps) load(step + NS - 1);
+    cp_async_commit();
+    if (kc == 0) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[j][e] = 0.0;
+    }
+    const double* bp = ring + stage * kFwUnits * US + (g >> 1) * US + (g & 1) * kFwLD + t;
+    const double* ap = sw + (STREAM ? stage * kFwCB * ldw : kc * KC) + ch * ldw + t;
+    const int left = cin - kc * KC, ks = left < KC ? (left + 7) / 8 : KC / 8;
+#pragma unroll 2
+    for (int k = 0; k < ks; ++k) {
+      const double a[4] = {ap[8 * k], ap[8 * k + ldw], ap[8 * k + 4], ap[8 * k + ldw + 4]};
+#pragma unroll
+      for (int j = 0; j < NT; ++j) mma_m16n8k8(acc[j], a, bp[2 * j * kFwLD + 8 * k], bp[2 * j * kFwLD + 8 * k + 4]);
+    }
+    if (kc + 1 == nk) {
+      const int64_t u = (first + step / nk * per * NG) * kFwUnits + t;
+      if (u < units && c < cout)
+        forward_epilogue<DIM, ACT>(acc, b0, b1, u, c, rows, cout, residual, out, activated, aux, vec_out);
+      __syncwarp();
+    }
+  }
+  cp_async_wait<0>();
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+template <int DIM, bool ACT, int NG, int NS, bool STREAM>
+cudaError_t launch_forward(const double* hidden, const double* weight, const double* bias, const double* residual,
+                           double* out, double* activated, double* aux, Packed rows, int cin, int cout,
+                           cudaStream_t stream) {
+  const auto kernel = affine_forward<DIM, ACT, NG, NS, STREAM>;
+  const size_t smem = fw_smem<DIM, NG, NS, STREAM>(cin);
+  int sms = 0;
+  cudaError_t e = sm_count(&sms);
+  // a per-device attribute: set on every call, so that each device gets it
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+  if (e != cudaSuccess) return e;
+  const int64_t blocks = (int64_t(cout) + kFwCB - 1) / kFwCB;
+  const int64_t tiles = (rows.units<Jet<DIM>::Q>() + kFwUnits - 1) / kFwUnits;
+  const int64_t most = sms / blocks > 0 ? sms / blocks : 1, per = tiles < most ? tiles : most;
+  const bool vec_in = cin % 2 == 0 && aligned16(hidden) && aligned16(weight);
+  const bool vec_out = cout % 2 == 0 && aligned16(out) && aligned16(residual) && aligned16(activated);
+  kernel<<<unsigned(per * blocks), NG * kFwGroup, smem, stream>>>(hidden, weight, bias, residual, out, activated, aux,
+                                                                 rows, cin, cout, vec_in, vec_out);
+  return cudaGetLastError();
+}
+
+// W's block beside as many groups and stages as 227 KB hold
+template <int DIM, bool ACT, typename... Args>
+cudaError_t forward(int cin, Args... args) {
+  if constexpr (DIM == 2) {
+    if (cin <= 160) return launch_forward<2, ACT, 4, 3, false>(args...);
+    if (cin <= 256) return launch_forward<2, ACT, 4, 2, false>(args...);
+    return launch_forward<2, ACT, 4, 2, true>(args...);
+  } else {
+    if (cin <= 160) return launch_forward<3, ACT, 3, 2, false>(args...);
+    if (cin <= 256) return launch_forward<3, ACT, 2, 2, false>(args...);
+    return launch_forward<3, ACT, 2, 2, true>(args...);
   }
 }
 
@@ -181,12 +355,9 @@ int flashns_b200_affine(int dim, int activation, const double* hidden, const dou
       ranges_overlap(activated, bytes, hidden, in) || ranges_overlap(activated, bytes, residual, bytes) ||
       ranges_overlap(out, bytes, activated, bytes))
     return int(cudaErrorInvalidValue);
-  const unsigned grid = grid_for((dim == 2 ? rows.units<10>() : rows.units<20>()) * cout);
-  if (dim == 2 && activation) affine_forward<2, true><<<grid, kAffThreads, 0, stream>>>(hidden, weight, bias, residual, out, activated, aux, rows, cin, cout);
-  else if (dim == 2) affine_forward<2, false><<<grid, kAffThreads, 0, stream>>>(hidden, weight, bias, residual, out, activated, aux, rows, cin, cout);
-  else if (activation) affine_forward<3, true><<<grid, kAffThreads, 0, stream>>>(hidden, weight, bias, residual, out, activated, aux, rows, cin, cout);
-  else affine_forward<3, false><<<grid, kAffThreads, 0, stream>>>(hidden, weight, bias, residual, out, activated, aux, rows, cin, cout);
-  return int(cudaGetLastError());
+  const auto run = [&](auto launch) { return int(launch(cin, hidden, weight, bias, residual, out, activated, aux, rows, cin, cout, stream)); };
+  if (dim == 2) return activation ? run([](auto... a) { return forward<2, true>(a...); }) : run([](auto... a) { return forward<2, false>(a...); });
+  return activation ? run([](auto... a) { return forward<3, true>(a...); }) : run([](auto... a) { return forward<3, false>(a...); });
 }
 
 int flashns_b200_affine_vjp_scratch(int dim, int activation, int64_t full_points, int64_t value_points, int cin,
