@@ -15,6 +15,11 @@ from flashns_b200.jet_spec import JetSpec
 from flashns_b200.jet_stable import stable_a1  # noqa: F401  (the reference exports it here too)
 
 
+@lru_cache(None)
+def _q(dimension):
+    return JetSpec(dimension).q
+
+
 @dataclass(frozen=True)
 class PackedLayout:
     full_points: int
@@ -28,7 +33,7 @@ class PackedLayout:
 
     @property
     def q(self):
-        return JetSpec(self.dimension).q
+        return _q(self.dimension)
 
     @property
     def points(self):

@@ -7,10 +7,16 @@ boundary rows.
 """
 
 from dataclasses import dataclass
+from functools import lru_cache
 from itertools import product
 from math import factorial, prod
 
 _OPERATIONS = {"affine", "tanh", "pointwise_fixed_loss", "first_parameter_vjp", "dgrad_jet_vjp"}
+
+
+@lru_cache(None)
+def _coefficient_order(d):
+    return tuple(sorted((a for a in product(range(4), repeat=d) if sum(a) <= 3), key=lambda a: (sum(a), a)))
 
 
 @dataclass(frozen=True)
@@ -31,8 +37,7 @@ class JetSpec:
 
     @property
     def coefficient_order(self):
-        d = self.coordinate_dimension
-        return tuple(sorted((a for a in product(range(4), repeat=d) if sum(a) <= 3), key=lambda a: (sum(a), a)))
+        return _coefficient_order(self.coordinate_dimension)
 
     @property
     def q(self):

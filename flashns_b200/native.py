@@ -8,6 +8,7 @@ Launches are asynchronous on the current stream; shape/dtype errors raise
 """
 
 import ctypes
+from functools import lru_cache
 
 import torch
 
@@ -16,14 +17,17 @@ from flashns_b200.jet_spec import JetSpec
 
 
 def _ptr(t):
-    return ctypes.c_void_p(t.data_ptr()) if t is not None and t.numel() else None
+    return t.data_ptr() if t is not None and t.numel() else None
 
 
 def _launch(name, args, tensors):
+    """One call on the current stream of ``tensors[0]``'s device.  ``tensors``: what must outlive the
+    launch where it came from another stream (tensors allocated for this call need not be named)."""
     lib = _lib.library()
-    with torch.cuda.device(tensors[0].device):
-        stream = torch.cuda.current_stream()
-        status = getattr(lib, name)(*args, ctypes.c_void_p(stream.cuda_stream))
+    index = tensors[0].get_device()
+    with torch.cuda.device(index):
+        stream = torch.cuda.current_stream(index)
+        status = getattr(lib, name)(*args, stream.cuda_stream)
         for t in tensors:
             if t is not None and t.numel():
                 t.record_stream(stream)
@@ -42,12 +46,17 @@ def _check(tensors):
             raise NotImplementedError("manual parameter VJP; double backward/HVP unsupported")
 
 
-def _scratch(name, like, *sizes):
-    """Scratch of the size that entry point ``name`` gives for these sizes, on ``like``'s device."""
+@lru_cache(256)
+def _scratch_doubles(name, index, *sizes):
     size = ctypes.c_size_t()
-    with torch.cuda.device(like.device):
+    with torch.cuda.device(index):
         _lib.check(getattr(_lib.library(), name)(*sizes, ctypes.byref(size)), name)
-    return like.new_empty((size.value + 7) // 8)
+    return (size.value + 7) // 8
+
+
+def _scratch(name, like, *sizes):
+    """Scratch of the size that entry point ``name`` gives for these sizes on ``like``'s device."""
+    return like.new_empty((_scratch_doubles(name, like.get_device(), *sizes),))
 
 
 def _affine_shape(hidden, weight):
@@ -209,7 +218,7 @@ class NativeCUDA:
         out, stats = torch.empty_like(value), value.new_empty((layout.rows, 2))
         _launch("flashns_b200_layer_norm", [layout.dimension, *map(_ptr, (value, gain, bias, out, stats)), eps,
                                             layout.full_points, layout.value_points, channels],
-                (value, gain, bias, out, stats))
+                (value, gain, bias))
         return out, stats
 
     def layer_norm_vjp(self, layout, value, gain, stats, seed, *, skip=None):
@@ -227,8 +236,7 @@ class NativeCUDA:
                            layout.value_points, channels)
         _launch("flashns_b200_layer_norm_vjp",
                 [layout.dimension, *map(_ptr, (value, gain, stats, seed, skip, out, dgain, dbias, scratch)),
-                 scratch.numel() * 8, layout.full_points, layout.value_points, channels],
-                (*given, out, dgain, dbias, scratch))
+                 scratch.numel() * 8, layout.full_points, layout.value_points, channels], given)
         return out, dgain, dbias
 
     def affine(self, layout, hidden, weight, bias, *, residual=None):
@@ -253,7 +261,7 @@ class NativeCUDA:
         activated = torch.empty_like(out) if keep and residual is not None else None
         _launch("flashns_b200_affine",
                 [layout.dimension, int(activation), *map(_ptr, (hidden, weight, bias, residual, out, activated, aux)),
-                 layout.full_points, layout.value_points, cin, cout], (*given, out, activated, aux))
+                 layout.full_points, layout.value_points, cin, cout], given)
         return (out, out if activated is None else activated, aux) if keep else out
 
     def affine_vjp(self, layout, hidden, weight, seed):
@@ -283,7 +291,7 @@ class NativeCUDA:
         _launch("flashns_b200_affine_vjp",
                 [layout.dimension, activation,
                  *map(_ptr, (hidden, weight, activated, aux, seed, out, dw, db, scratch)), scratch.numel() * 8,
-                 layout.full_points, layout.value_points, cin, cout], (*given, out, dw, db, scratch))
+                 layout.full_points, layout.value_points, cin, cout], given)
         return out, dw, db
 
 
