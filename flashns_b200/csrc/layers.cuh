@@ -75,6 +75,24 @@ __device__ __forceinline__ void lane_sums(double* v) {
   }
 }
 
+// The first half of lane_sums: every lane ends with its own few of the N sums, v[0 ..] being
+// the sums first, first + 1, ... below limit (call with first = 0, limit = N).
+template <int N, int O>
+__device__ __forceinline__ void lane_shares(double* v, int& first, int& limit) {
+  if constexpr (O > 0) {
+    constexpr int H = (N + 1) / 2;
+    const bool up = (threadIdx.x & O) != 0;
+#pragma unroll
+    for (int i = 0; i < H; ++i) {
+      const double lo = v[i], hi = i + H < N ? v[i + H] : 0.0;
+      v[i] = (up ? hi : lo) + __shfl_xor_sync(0xffffffffu, up ? lo : hi, O);
+    }
+    if (up) first += H;
+    else limit = limit < first + H ? limit : first + H;
+    lane_shares<H, O / 2>(v, first, limit);
+  }
+}
+
 inline bool layer_sizes_ok(int dim, int64_t full, int64_t value, int widest) {
   if ((dim != 2 && dim != 3) || full < 0 || value < 0 || widest < 1) return false;
   const int64_t q = dim == 2 ? 10 : 20;

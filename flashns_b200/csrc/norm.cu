@@ -8,6 +8,9 @@
 //   dX_c = corr(r, gain_c G_c - M) + corr(D_c, w) [+ skip_c],
 //   dgain_c = sum over points of <r, corr(D_c, G_c)>,  dbias_c = sum over points of G_(0,c).
 // (sum_c D_c = 0, so the mean's share of dX passes through the first term alone.)
+#include <algorithm>
+#include <type_traits>
+
 #include "flashns_b200.h"
 #include "layers.cuh"
 
@@ -200,22 +203,335 @@ __global__ void __launch_bounds__(kNormThreads)
   }
 }
 
-// dgain, dbias [channels] each from partials [parts][2][channels], summed in block order
-__global__ void __launch_bounds__(kNormThreads)
+// ---------------------------------------------------------------- a unit in registers
+// T lanes of a warp, or W whole warps (a block), hold one unit: lane l has channels
+// l, l + L, ... (L = T W lanes, K of them), all Q rows each, so every row is read once in
+// 8-byte runs of L channels.  The sums over channels are K-term sums in the lane and a halving
+// exchange over the lanes (lane_sums), joined over the warps through shared memory.
+template <int N, int T, int W>
+__device__ __forceinline__ void unit_sums(double (&v)[N], double* shared, int& turn) {
+  if constexpr (W == 1) {
+    lane_sums<N, T / 2>(v);
+  } else {
+    // two buffers in turn: one barrier separates a buffer's readers from its next writers
+    double* sums = shared + (turn ^= 1) * W * N;
+    const int warp = threadIdx.x >> 5;
+    int first = 0, limit = N;
+    lane_shares<N, 16>(v, first, limit);
+#pragma unroll
+    for (int i = 0; i < (N + 31) / 32; ++i)
+      if (first + i < limit) sums[warp * N + first + i] = v[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      double s = sums[i];
+#pragma unroll
+      for (int w = 1; w < W; ++w) s += sums[w * N + i];
+      v[i] = s;
+    }
+  }
+}
+
+template <int T, int W>
+constexpr int unit_threads() { return W == 1 ? kNormThreads : 32 * W; }
+template <int T, int W>
+constexpr int unit_groups() { return W == 1 ? kNormThreads / T : 1; }
+
+template <int DIM, int T, int K, int W>
+__global__ void __launch_bounds__(unit_threads<T, W>())
+    norm_forward_unit(const double* __restrict__ x, const double* __restrict__ gain, const double* __restrict__ bias,
+                      double* __restrict__ out, double* __restrict__ stats, double eps, Packed rows, int channels) {
+  constexpr int Q = Jet<DIM>::Q, L = T * W;
+  __shared__ double shared[W > 1 ? 2 * W * Q : 1];
+  int turn = 0;
+  const int lane = W > 1 ? threadIdx.x : threadIdx.x % T;
+  const int64_t u = int64_t(blockIdx.x) * unit_groups<T, W>() + (W > 1 ? 0 : threadIdx.x / T);
+  const int n = u < rows.units<Q>() ? rows.count<Q>(u) : 0;  // no rows: the lanes only take part in the sums
+  const bool full = u < rows.full;
+  const int64_t row = rows.row<Q>(u);
+  double d[K][Q], sums[Q], r[Q];
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int s = 0; s < Q; ++s) {
+      const int c = lane + k * L;
+      d[k][s] = s < n && c < channels ? x[(row + s) * channels + c] : 0.0;
+    }
+  const double inv = 1.0 / channels;
+#pragma unroll
+  for (int s = 0; s < Q; ++s) {
+    sums[s] = d[0][s];
+#pragma unroll
+    for (int k = 1; k < K; ++k) sums[s] += d[k][s];
+  }
+  unit_sums<Q, T, W>(sums, shared, turn);
+  double mean[Q];
+#pragma unroll
+  for (int s = 0; s < Q; ++s) {
+    mean[s] = sums[s] * inv;
+    sums[s] = 0.0;
+  }
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    if (lane + k * L < channels) {
+      double p[Q];
+#pragma unroll
+      for (int s = 0; s < Q; ++s) d[k][s] -= mean[s];
+      if (full) {
+        Jet<DIM>::square(d[k], p);
+      } else {
+#pragma unroll
+        for (int s = 0; s < Q; ++s) p[s] = d[k][s] * d[k][s];
+      }
+#pragma unroll
+      for (int s = 0; s < Q; ++s) sums[s] += p[s];
+    }
+  }
+  unit_sums<Q, T, W>(sums, shared, turn);
+#pragma unroll
+  for (int s = 0; s < Q; ++s) sums[s] *= inv;
+  if (full) {
+    sums[0] += eps;
+    Jet<DIM>::rsqrt(sums, r);
+  } else {
+#pragma unroll
+    for (int s = 0; s < Q; ++s) r[s] = 1.0 / sqrt(sums[s] + eps);
+  }
+#pragma unroll
+  for (int s = 0; s < Q; ++s)
+    if (lane == s % L && s < n) {
+      stats[2 * (row + s)] = mean[s];
+      stats[2 * (row + s) + 1] = r[s];
+    }
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int c = lane + k * L;
+    if (c < channels && n > 0) {
+      const double gc = gain[c], bc = bias[c];
+      double y[Q];
+      if (full) {
+        Jet<DIM>::mul(r, d[k], y);
+      } else {
+#pragma unroll
+        for (int s = 0; s < Q; ++s) y[s] = r[s] * d[k][s];
+      }
+#pragma unroll
+      for (int s = 0; s < Q; ++s)
+        if (s < n) out[(row + s) * channels + c] = gc * y[s] + (s == 0 || !full ? bc : 0.0);
+    }
+  }
+}
+
+template <int DIM, int T, int K, int W>
+__global__ void __launch_bounds__(unit_threads<T, W>())
+    norm_backward_unit(const double* __restrict__ x, const double* __restrict__ gain, const double* __restrict__ stats,
+                       const double* __restrict__ seed, const double* __restrict__ skip, double* __restrict__ dx,
+                       double* __restrict__ partials, Packed rows, int channels) {
+  constexpr int Q = Jet<DIM>::Q, L = T * W, G = unit_groups<T, W>();
+  __shared__ double shared[W > 1 ? 4 * W * Q : 2 * K * kNormThreads];
+  int turn = 0;
+  const int lane = W > 1 ? threadIdx.x : threadIdx.x % T, group = W > 1 ? 0 : threadIdx.x / T;
+  const int64_t units = rows.units<Q>();
+  const double inv = 1.0 / channels;
+  double gk[K], dgain[K], dbias[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    gk[k] = lane + k * L < channels ? gain[lane + k * L] : 0.0;
+    dgain[k] = dbias[k] = 0.0;
+  }
+  // the block's groups step together, so that a group without a unit still takes part in the shuffles
+  for (int64_t u0 = int64_t(blockIdx.x) * G; u0 < units; u0 += int64_t(gridDim.x) * G) {
+    const int64_t u = u0 + group;
+    const int n = u < units ? rows.count<Q>(u) : 0;
+    const bool full = u < rows.full;
+    const int64_t row = rows.row<Q>(u);
+    double d[K][Q], g[K][Q], r[Q], sums[2 * Q], w[Q];
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int s = 0; s < Q; ++s) {
+        const int c = lane + k * L;
+        const bool ok = s < n && c < channels;
+        d[k][s] = ok ? x[(row + s) * channels + c] : 0.0;
+        g[k][s] = ok ? seed[(row + s) * channels + c] : 0.0;
+      }
+#pragma unroll
+    for (int s = 0; s < Q; ++s) {
+      const double mean = s < n ? stats[2 * (row + s)] : 0.0;
+      r[s] = s < n ? stats[2 * (row + s) + 1] : 0.0;
+      sums[s] = sums[Q + s] = 0.0;
+#pragma unroll
+      for (int k = 0; k < K; ++k) d[k][s] = lane + k * L < channels ? d[k][s] - mean : 0.0;
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      double p[Q];
+      if (full) {
+        Jet<DIM>::corr(d[k], g[k], p);
+        dbias[k] += g[k][0];
+      } else {
+#pragma unroll
+        for (int s = 0; s < Q; ++s) {
+          p[s] = d[k][s] * g[k][s];
+          dbias[k] += g[k][s];
+        }
+      }
+#pragma unroll
+      for (int s = 0; s < Q; ++s) {
+        dgain[k] += r[s] * p[s];
+        sums[s] += gk[k] * p[s];
+        g[k][s] *= gk[k];
+        sums[Q + s] += g[k][s];
+      }
+    }
+    unit_sums<2 * Q, T, W>(sums, shared, turn);
+    if (full) {
+      double r2[Q], r3[Q];
+      Jet<DIM>::mul(r, r, r2);
+      Jet<DIM>::mul(r2, r, r3);
+      Jet<DIM>::corr(r3, sums, w);
+    } else {
+#pragma unroll
+      for (int s = 0; s < Q; ++s) w[s] = r[s] * r[s] * r[s] * sums[s];
+    }
+#pragma unroll
+    for (int s = 0; s < Q; ++s) {
+      w[s] *= -inv;
+      sums[Q + s] *= inv;
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = lane + k * L;
+      if (c >= channels) continue;
+      double y[Q];
+#pragma unroll
+      for (int s = 0; s < Q; ++s) g[k][s] -= sums[Q + s];
+      if (full) {
+        Jet<DIM>::corr(r, g[k], y);
+        Jet<DIM>::corr_add(d[k], w, y);
+      } else {
+#pragma unroll
+        for (int s = 0; s < Q; ++s) y[s] = r[s] * g[k][s] + d[k][s] * w[s];
+      }
+#pragma unroll
+      for (int s = 0; s < Q; ++s) {
+        if (s >= n) continue;
+        const int64_t at = (row + s) * channels + c;
+        dx[at] = skip ? y[s] + skip[at] : y[s];
+      }
+    }
+    __syncwarp();
+  }
+  double* mine = partials + int64_t(blockIdx.x) * 2 * channels;
+  if constexpr (W > 1) {
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+      if (lane + k * L < channels) {
+        mine[lane + k * L] = dgain[k];
+        mine[channels + lane + k * L] = dbias[k];
+      }
+  } else {  // the block's groups, in order
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      shared[(group * K + k) * T + lane] = dgain[k];
+      shared[K * kNormThreads + (group * K + k) * T + lane] = dbias[k];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 2 * K * T; i += kNormThreads) {
+      const int which = i / (K * T), c = i % (K * T);
+      double s = 0.0;
+      for (int q = 0; q < G; ++q) s += shared[which * K * kNormThreads + q * K * T + c];
+      if (c < channels) mine[which * channels + c] = s;
+    }
+  }
+}
+
+// dgain, dbias [channels] each from partials [parts][2][channels]: 8 strands of parts a value,
+// each in order, then the strands in order
+constexpr int kFinishStrands = 8, kFinishLanes = 32;
+__global__ void __launch_bounds__(kFinishStrands* kFinishLanes)
     norm_finish(const double* __restrict__ partials, int parts, double* __restrict__ dgain, double* __restrict__ dbias,
                 int channels) {
-  for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < 2 * channels; i += gridDim.x * blockDim.x) {
-    double s = 0.0;
-    for (int k = 0; k < parts; ++k) s += partials[int64_t(k) * 2 * channels + i];
+  __shared__ double shared[kFinishStrands][kFinishLanes];
+  const int lane = threadIdx.x % kFinishLanes, strand = threadIdx.x / kFinishLanes;
+  const int64_t i = int64_t(blockIdx.x) * kFinishLanes + lane, n = 2 * int64_t(channels);
+  double s = 0.0;
+  if (i < n) {
+#pragma unroll 8
+    for (int k = strand; k < parts; k += kFinishStrands) s += partials[k * n + i];
+  }
+  shared[strand][lane] = s;
+  __syncthreads();
+  if (strand == 0 && i < n) {
+    for (int k = 1; k < kFinishStrands; ++k) s += shared[k][lane];
     if (i < channels) dgain[i] = s;
     else dbias[i - channels] = s;
   }
 }
 
-// blocks of the backward kernel: each keeps one [2][channels] partial
+// How a unit is held at a width: calls f(T, K, W) (as integral constants), or says that no
+// register form has it.
+template <int V>
+using Int = std::integral_constant<int, V>;
+template <int DIM, bool BACKWARD, typename F>
+bool with_unit(int channels, const F& f) {
+  if (channels <= 16) return f(Int<8>{}, Int<2>{}, Int<1>{}), true;
+  if (channels <= 32) return f(Int<16>{}, Int<2>{}, Int<1>{}), true;
+  if constexpr (DIM == 2) {
+    if (channels <= 64) return f(Int<32>{}, Int<2>{}, Int<1>{}), true;
+    if (channels <= 128) return f(Int<32>{}, Int<2>{}, Int<2>{}), true;
+    if (channels <= 256) return f(Int<32>{}, Int<2>{}, Int<4>{}), true;
+  } else {
+    if (channels <= 64) return f(Int<32>{}, Int<1>{}, Int<2>{}), true;
+    if (channels <= 128) return f(Int<32>{}, Int<1>{}, Int<4>{}), true;
+    if (channels <= 256) return f(Int<32>{}, Int<1>{}, Int<8>{}), true;
+  }
+  return false;
+}
+
+// blocks of the backward kernel, each of which keeps one [2][channels] partial: all that are
+// resident at once (at most 16 a multiprocessor), or one for each of its units
 int64_t norm_parts(int dim, Packed rows, int sms) {
   const int64_t units = dim == 2 ? rows.units<10>() : rows.units<20>(), most = int64_t(sms) * 8;
   return units < most ? units : most;
+}
+
+template <int DIM>
+cudaError_t launch_norm(const double* x, const double* gain, const double* bias, double* out, double* stats, double eps,
+                        Packed rows, int channels, int sms, cudaStream_t stream) {
+  const int64_t units = rows.units<Jet<DIM>::Q>();
+  const bool done = with_unit<DIM, false>(channels, [&](auto t, auto k, auto w) {
+    constexpr int T = t, K = k, W = w, G = unit_groups<T, W>();
+    norm_forward_unit<DIM, T, K, W><<<unsigned((units + G - 1) / G), unit_threads<T, W>(), 0, stream>>>(
+        x, gain, bias, out, stats, eps, rows, channels);
+  });
+  if (!done)
+    norm_forward<DIM><<<unsigned(norm_parts(DIM, rows, sms)), kNormThreads, 0, stream>>>(x, gain, bias, out, stats, eps,
+                                                                                       rows, channels);
+  return cudaGetLastError();
+}
+
+template <int DIM>
+cudaError_t launch_norm_vjp(const double* x, const double* gain, const double* stats, const double* seed,
+                            const double* skip, double* dx, double* dgain, double* dbias, double* partials, Packed rows,
+                            int channels, int sms, cudaStream_t stream) {
+  int64_t parts = norm_parts(DIM, rows, sms);
+  const bool done = with_unit<DIM, true>(channels, [&](auto t, auto k, auto w) {
+    constexpr int T = t, K = k, W = w, G = unit_groups<T, W>();
+    const auto kernel = norm_backward_unit<DIM, T, K, W>;
+    const int64_t blocks = (rows.units<Jet<DIM>::Q>() + G - 1) / G;
+    int per_sm = 0;
+    cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, unit_threads<T, W>(), 0);
+    parts = std::min(std::min(parts, blocks), int64_t(sms) * (per_sm > 0 ? per_sm : 1));
+    kernel<<<unsigned(parts), unit_threads<T, W>(), 0, stream>>>(x, gain, stats, seed, skip, dx, partials, rows, channels);
+  });
+  if (!done)
+    norm_backward<DIM><<<unsigned(parts), kNormThreads, 0, stream>>>(x, gain, stats, seed, skip, dx, partials, rows, channels);
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  norm_finish<<<unsigned((2 * int64_t(channels) + kFinishLanes - 1) / kFinishLanes), kFinishStrands * kFinishLanes, 0,
+                stream>>>(partials, int(parts), dgain, dbias, channels);
+  return cudaGetLastError();
 }
 
 }  // namespace
@@ -243,10 +559,8 @@ int flashns_b200_layer_norm(int dim, const double* value, const double* gain, co
   int sms = 0;
   cudaError_t e = sm_count(&sms);
   if (e != cudaSuccess) return int(e);
-  const unsigned grid = unsigned(norm_parts(dim, rows, sms));
-  if (dim == 2) norm_forward<2><<<grid, kNormThreads, 0, stream>>>(value, gain, bias, out, stats, eps, rows, channels);
-  else norm_forward<3><<<grid, kNormThreads, 0, stream>>>(value, gain, bias, out, stats, eps, rows, channels);
-  return int(cudaGetLastError());
+  return int(dim == 2 ? launch_norm<2>(value, gain, bias, out, stats, eps, rows, channels, sms, stream)
+                      : launch_norm<3>(value, gain, bias, out, stats, eps, rows, channels, sms, stream));
 }
 
 int flashns_b200_layer_norm_vjp_scratch(int dim, int64_t full_points, int64_t value_points, int channels,
@@ -284,14 +598,9 @@ int flashns_b200_layer_norm_vjp(int dim, const double* value, const double* gain
   int sms = 0;
   cudaError_t e = sm_count(&sms);
   if (e != cudaSuccess) return int(e);
-  const int parts = int(norm_parts(dim, rows, sms));
-  if (scratch_bytes < size_t(parts) * 2 * small) return int(cudaErrorInvalidValue);
-  if (dim == 2) norm_backward<2><<<parts, kNormThreads, 0, stream>>>(value, gain, stats, seed, skip, d_value, scratch, rows, channels);
-  else norm_backward<3><<<parts, kNormThreads, 0, stream>>>(value, gain, stats, seed, skip, d_value, scratch, rows, channels);
-  e = cudaGetLastError();
-  if (e != cudaSuccess) return int(e);
-  norm_finish<<<(2 * channels + kNormThreads - 1) / kNormThreads, kNormThreads, 0, stream>>>(scratch, parts, d_gain, d_bias, channels);
-  return int(cudaGetLastError());
+  if (scratch_bytes < size_t(norm_parts(dim, rows, sms)) * 2 * small) return int(cudaErrorInvalidValue);
+  const auto launch = dim == 2 ? launch_norm_vjp<2> : launch_norm_vjp<3>;
+  return int(launch(value, gain, stats, seed, skip, d_value, d_gain, d_bias, scratch, rows, channels, sms, stream));
 }
 
 }  // extern "C"
