@@ -203,191 +203,303 @@ __global__ void __launch_bounds__(kNormThreads)
   }
 }
 
-// ---------------------------------------------------------------- a unit in registers
-// T lanes of a warp, or W whole warps (a block), hold one unit: lane l has channels
-// l, l + L, ... (L = T W lanes, K of them), all Q rows each, so every row is read once in
-// 8-byte runs of L channels.  The sums over channels are K-term sums in the lane and a halving
-// exchange over the lanes (lane_sums), joined over the warps through shared memory.
-template <int N, int T, int W>
-__device__ __forceinline__ void unit_sums(double (&v)[N], double* shared, int& turn) {
-  if constexpr (W == 1) {
-    lane_sums<N, T / 2>(v);
-  } else {
-    // two buffers in turn: one barrier separates a buffer's readers from its next writers
-    double* sums = shared + (turn ^= 1) * W * N;
-    const int warp = threadIdx.x >> 5;
-    int first = 0, limit = N;
-    lane_shares<N, 16>(v, first, limit);
-#pragma unroll
-    for (int i = 0; i < (N + 31) / 32; ++i)
-      if (first + i < limit) sums[warp * N + first + i] = v[i];
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      double s = sums[i];
-#pragma unroll
-      for (int w = 1; w < W; ++w) s += sums[w * N + i];
-      v[i] = s;
-    }
-  }
+// ---------------------------------------------------------------- streamed units
+// A group of W warps takes one unit at a time (T < 32 lanes of a warp: one each of several
+// units, so that narrow layers fill their warps); lane l has channels l and l + T W (K of
+// them).  HBM bounds the sizes that matter, but only while a unit costs few instructions: a
+// value is 16 to 32 bytes and some 50 multiply-adds.  So
+//   - a lane copies its own values of the group's next unit into its own column of shared
+//     memory (cp.async, 8 bytes each: any width and alignment, whole lines a warp) while it
+//     works on this one.  No other lane reads them, so no barrier waits for them, and the
+//     fixed column layout leaves no address arithmetic in the passes;
+//   - rows past a short unit are copied as zeros, so no pass tests for them;
+//   - sums over channels are a halving exchange over the lanes (each ends with its own few),
+//     then one shared-memory read that joins the warps and hands all sums to all lanes.
+// Blocks are persistent, one a multiprocessor; each has as many groups as its shared memory
+// and registers hold.
+constexpr int kUnitMostLanes = 256;  // lanes of the widest group
+constexpr size_t kUnitSmem = 226 * 1024;
+template <int DIM, bool BACKWARD>
+constexpr int unit_k() { return DIM == 3 && BACKWARD ? 1 : 2; }  // channels a lane
+template <int DIM, bool BACKWARD>
+constexpr int unit_warps() { return BACKWARD ? 8 : DIM == 2 ? 16 : 10; }  // most warps of a block
+template <bool BACKWARD>
+constexpr int unit_slots() { return BACKWARD ? 5 : 2; }  // X (and G) twice; skip
+
+__device__ __forceinline__ void copy8(double* smem, const double* gmem, bool valid) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;\n" ::"r"(smem_u32(smem)), "l"(gmem), "r"(valid ? 8 : 0));
 }
 
-template <int T, int W>
-constexpr int unit_threads() { return W == 1 ? kNormThreads : 32 * W; }
-template <int T, int W>
-constexpr int unit_groups() { return W == 1 ? kNormThreads / T : 1; }
+template <int DIM, bool BACKWARD, int T, int W>
+struct Place {
+  static constexpr int Q = Jet<DIM>::Q, K = unit_k<DIM, BACKWARD>(), L = T * W, N = BACKWARD ? 2 * Q : Q;
+  static constexpr int kUnits = W > 1 ? 1 : 32 / T;         // units of a set, the group's step
+  static constexpr int kThreads = 32 * W;                   // of a group
+  static constexpr int kSlot = Q * K * kThreads;            // doubles of one set's values
+  static constexpr int kSums = (W > 1 ? W : kUnits) * N;    // one buffer of sums
+  static constexpr int kStats = BACKWARD ? kUnits * 2 * Q : 0;
+  static constexpr int kDoubles = unit_slots<BACKWARD>() * kSlot + 2 * kSums + 2 * kStats;
+  static constexpr int kGroups = int(kUnitSmem / sizeof(double) / kDoubles) < unit_warps<DIM, BACKWARD>() / W
+                                     ? int(kUnitSmem / sizeof(double) / kDoubles)
+                                     : unit_warps<DIM, BACKWARD>() / W;
+  static constexpr int kBlock = kGroups * kThreads;
+  int group, sub, lane, in_group;
+  __device__ Place()
+      : group(threadIdx.x / kThreads), sub(W > 1 ? 0 : threadIdx.x % 32 / T), lane(threadIdx.x % L),
+        in_group(threadIdx.x % kThreads) {}
+  __device__ __forceinline__ void sync() const {
+    if constexpr (W == 1) __syncwarp(); else named_sync(1 + group, kThreads);
+  }
+  // this lane's values of rows row .. row + n - 1 into its column of `slot`, zeros up to Q rows
+  __device__ __forceinline__ void copy(double* slot, const double* __restrict__ from, int64_t row, int n, int channels) const {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      if (lane + k * L >= channels) continue;
+      const double* src = from + row * channels + lane + k * L;
+      const unsigned to = smem_u32(slot + k * Q * kThreads);
+      // rolled up: unrolled, the Q addresses of every array are kept in registers
+#pragma unroll 1
+      for (int s = 0; s < Q; s += 2, src += 2 * int64_t(channels)) {
+        const bool a = s < n, b = s + 1 < n;
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;\n" ::"r"(to + 8u * s * kThreads),
+                     "l"(a ? src : from), "r"(a ? 8 : 0));
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;\n" ::"r"(to + 8u * (s + 1) * kThreads),
+                     "l"(b ? src + channels : from), "r"(b ? 8 : 0));
+      }
+    }
+  }
+  // v: this lane's part of N sums; all of them in every lane of the unit
+  __device__ __forceinline__ void sum(double (&v)[N], double* sums) const {
+    int first = 0, limit = N;
+    lane_shares<N, T / 2>(v, first, limit);
+    double* mine = sums + (W > 1 ? in_group / 32 : sub) * N;
+#pragma unroll
+    for (int i = 0; i < (N + T - 1) / T + 1; ++i)
+      if (first + i < limit) mine[first + i] = v[i];
+    sync();
+    const double2* all = reinterpret_cast<const double2*>(W > 1 ? sums : mine);
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      double2 s = all[i];
+#pragma unroll
+      for (int w = 1; w < W; ++w) {
+        const double2 o = all[w * (N / 2) + i];
+        s.x += o.x, s.y += o.y;
+      }
+      v[2 * i] = s.x, v[2 * i + 1] = s.y;
+    }
+  }
+  // rows row .. row + n - 1 of channel c
+  __device__ __forceinline__ static void store(double* __restrict__ out, const double (&y)[Q], int64_t row, int n, int c,
+                                               int channels) {
+    double* to = out + row * channels + c;
+    if (n == Q) {
+#pragma unroll
+      for (int s = 0; s < Q; ++s) to[int64_t(s) * channels] = y[s];
+    } else {
+#pragma unroll
+      for (int s = 0; s < Q; ++s)
+        if (s < n) to[int64_t(s) * channels] = y[s];
+    }
+  }
+};
 
-template <int DIM, int T, int K, int W>
-__global__ void __launch_bounds__(unit_threads<T, W>())
+template <int DIM, int T, int W>
+__global__ void __launch_bounds__(Place<DIM, false, T, W>::kBlock, 1)
     norm_forward_unit(const double* __restrict__ x, const double* __restrict__ gain, const double* __restrict__ bias,
                       double* __restrict__ out, double* __restrict__ stats, double eps, Packed rows, int channels) {
-  constexpr int Q = Jet<DIM>::Q, L = T * W;
-  __shared__ double shared[W > 1 ? 2 * W * Q : 1];
-  int turn = 0;
-  const int lane = W > 1 ? threadIdx.x : threadIdx.x % T;
-  const int64_t u = int64_t(blockIdx.x) * unit_groups<T, W>() + (W > 1 ? 0 : threadIdx.x / T);
-  const int n = u < rows.units<Q>() ? rows.count<Q>(u) : 0;  // no rows: the lanes only take part in the sums
-  const bool full = u < rows.full;
-  const int64_t row = rows.row<Q>(u);
-  double d[K][Q], sums[Q], r[Q];
-#pragma unroll
-  for (int k = 0; k < K; ++k)
-#pragma unroll
-    for (int s = 0; s < Q; ++s) {
-      const int c = lane + k * L;
-      d[k][s] = s < n && c < channels ? x[(row + s) * channels + c] : 0.0;
-    }
+  using At = Place<DIM, false, T, W>;
+  constexpr int Q = At::Q, K = At::K, L = At::L, TH = At::kThreads;
+  extern __shared__ __align__(16) double smem[];
+  const At at;
+  double* buffers = smem + at.group * At::kDoubles;
+  double *mine = buffers + at.in_group, *sums_at = buffers + 2 * At::kSlot;
+  const int64_t units = rows.units<Q>(), sets = (units + At::kUnits - 1) / At::kUnits;
+  const int64_t stride = int64_t(gridDim.x) * At::kGroups;
   const double inv = 1.0 / channels;
-#pragma unroll
-  for (int s = 0; s < Q; ++s) {
-    sums[s] = d[0][s];
-#pragma unroll
-    for (int k = 1; k < K; ++k) sums[s] += d[k][s];
-  }
-  unit_sums<Q, T, W>(sums, shared, turn);
-  double mean[Q];
-#pragma unroll
-  for (int s = 0; s < Q; ++s) {
-    mean[s] = sums[s] * inv;
-    sums[s] = 0.0;
-  }
+  double gk[K], bk[K];
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    if (lane + k * L < channels) {
-      double p[Q];
+    const int c = at.lane + k * L;
+    gk[k] = c < channels ? gain[c] : 0.0;
+    bk[k] = c < channels ? bias[c] : 0.0;
+  }
+  auto load = [&](int64_t set, int stage) {
+    const int64_t u = set * At::kUnits + at.sub;
+    if (set < sets) at.copy(mine + stage * At::kSlot, x, rows.row<Q>(u), u < units ? rows.count<Q>(u) : 0, channels);
+    cp_async_commit();
+  };
+  int stage = 0;
+  const int64_t first = blockIdx.x + int64_t(at.group) * gridDim.x;  // few units: one a block
+  load(first, 0);
+  for (int64_t set = first; set < sets; set += stride, stage ^= 1) {
+    load(set + stride, stage ^ 1);
+    const int64_t u = set * At::kUnits + at.sub;
+    const int n = u < units ? rows.count<Q>(u) : 0;  // no rows: the lanes only take part in the sums
+    const bool full = u < rows.full;
+    const int64_t row = rows.row<Q>(u);
+    const double* xs = mine + stage * At::kSlot;
+    double sums[Q], mean[Q], r[Q];
 #pragma unroll
-      for (int s = 0; s < Q; ++s) d[k][s] -= mean[s];
+    for (int s = 0; s < Q; ++s) sums[s] = 0.0;
+    cp_async_wait<1>();
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      if (at.lane + k * L >= channels) continue;
+#pragma unroll
+      for (int s = 0; s < Q; ++s) sums[s] += xs[(k * Q + s) * TH];
+    }
+    __syncwarp();
+    at.sum(sums, sums_at);
+#pragma unroll
+    for (int s = 0; s < Q; ++s) {
+      mean[s] = sums[s] * inv;
+      sums[s] = 0.0;
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      if (at.lane + k * L >= channels) continue;
+      double d[Q], p[Q];
+#pragma unroll
+      for (int s = 0; s < Q; ++s) d[s] = xs[(k * Q + s) * TH] - mean[s];
       if (full) {
-        Jet<DIM>::square(d[k], p);
+        Jet<DIM>::square(d, p);
       } else {
 #pragma unroll
-        for (int s = 0; s < Q; ++s) p[s] = d[k][s] * d[k][s];
+        for (int s = 0; s < Q; ++s) p[s] = d[s] * d[s];
       }
 #pragma unroll
       for (int s = 0; s < Q; ++s) sums[s] += p[s];
     }
-  }
-  unit_sums<Q, T, W>(sums, shared, turn);
+    __syncwarp();
+    at.sum(sums, sums_at + At::kSums);
 #pragma unroll
-  for (int s = 0; s < Q; ++s) sums[s] *= inv;
-  if (full) {
-    sums[0] += eps;
-    Jet<DIM>::rsqrt(sums, r);
-  } else {
+    for (int s = 0; s < Q; ++s) sums[s] *= inv;
+    if (full) {
+      sums[0] += eps;
+      Jet<DIM>::rsqrt(sums, r);
+    } else {
 #pragma unroll
-    for (int s = 0; s < Q; ++s) r[s] = 1.0 / sqrt(sums[s] + eps);
-  }
-#pragma unroll
-  for (int s = 0; s < Q; ++s)
-    if (lane == s % L && s < n) {
-      stats[2 * (row + s)] = mean[s];
-      stats[2 * (row + s) + 1] = r[s];
+      for (int s = 0; s < Q; ++s) r[s] = 1.0 / sqrt(sums[s] + eps);
     }
+    double* st = stats + 2 * row;
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int c = lane + k * L;
-    if (c < channels && n > 0) {
-      const double gc = gain[c], bc = bias[c];
-      double y[Q];
-      if (full) {
-        Jet<DIM>::mul(r, d[k], y);
-      } else {
-#pragma unroll
-        for (int s = 0; s < Q; ++s) y[s] = r[s] * d[k][s];
+    for (int s = 0; s < Q; ++s)
+      if (at.lane == s % T && s < n) {
+        st[2 * s] = mean[s];
+        st[2 * s + 1] = r[s];
       }
 #pragma unroll
-      for (int s = 0; s < Q; ++s)
-        if (s < n) out[(row + s) * channels + c] = gc * y[s] + (s == 0 || !full ? bc : 0.0);
+    for (int k = 0; k < K; ++k) {
+      const int c = at.lane + k * L;
+      if (c >= channels) continue;
+      double d[Q], y[Q];
+#pragma unroll
+      for (int s = 0; s < Q; ++s) d[s] = xs[(k * Q + s) * TH] - mean[s];
+      if (full) {
+        Jet<DIM>::mul(r, d, y);
+#pragma unroll
+        for (int s = 0; s < Q; ++s) y[s] = s == 0 ? gk[k] * y[s] + bk[k] : gk[k] * y[s];
+      } else {
+#pragma unroll
+        for (int s = 0; s < Q; ++s) y[s] = gk[k] * (r[s] * d[s]) + bk[k];
+      }
+      At::store(out, y, row, n, c, channels);
     }
+    __syncwarp();
   }
+  cp_async_wait<0>();
 }
 
-template <int DIM, int T, int K, int W>
-__global__ void __launch_bounds__(unit_threads<T, W>())
+template <int DIM, int T, int W>
+__global__ void __launch_bounds__(Place<DIM, true, T, W>::kBlock, 1)
     norm_backward_unit(const double* __restrict__ x, const double* __restrict__ gain, const double* __restrict__ stats,
                        const double* __restrict__ seed, const double* __restrict__ skip, double* __restrict__ dx,
                        double* __restrict__ partials, Packed rows, int channels) {
-  constexpr int Q = Jet<DIM>::Q, L = T * W, G = unit_groups<T, W>();
-  __shared__ double shared[W > 1 ? 4 * W * Q : 2 * K * kNormThreads];
-  int turn = 0;
-  const int lane = W > 1 ? threadIdx.x : threadIdx.x % T, group = W > 1 ? 0 : threadIdx.x / T;
-  const int64_t units = rows.units<Q>();
+  using At = Place<DIM, true, T, W>;
+  constexpr int Q = At::Q, K = At::K, L = At::L, TH = At::kThreads;
+  extern __shared__ __align__(16) double smem[];
+  const At at;
+  double* buffers = smem + at.group * At::kDoubles;  // [2][X, G], skip
+  double *mine = buffers + at.in_group, *sums_at = buffers + 5 * At::kSlot;
+  double* stats_at = sums_at + 2 * At::kSums;  // [2][unit][Q] of (mean, r)
+  const int64_t units = rows.units<Q>(), sets = (units + At::kUnits - 1) / At::kUnits;
+  const int64_t stride = int64_t(gridDim.x) * At::kGroups, all_rows = rows.full * Q + rows.value;
   const double inv = 1.0 / channels;
   double gk[K], dgain[K], dbias[K];
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    gk[k] = lane + k * L < channels ? gain[lane + k * L] : 0.0;
+    gk[k] = at.lane + k * L < channels ? gain[at.lane + k * L] : 0.0;
     dgain[k] = dbias[k] = 0.0;
   }
-  // the block's groups step together, so that a group without a unit still takes part in the shuffles
-  for (int64_t u0 = int64_t(blockIdx.x) * G; u0 < units; u0 += int64_t(gridDim.x) * G) {
-    const int64_t u = u0 + group;
+  auto load = [&](int64_t set, int stage) {
+    const int64_t u = set * At::kUnits + at.sub;
+    if (set < sets) {
+      const int n = u < units ? rows.count<Q>(u) : 0;
+      double* slot = mine + 2 * stage * At::kSlot;
+      at.copy(slot, x, rows.row<Q>(u), n, channels);
+      at.copy(slot + At::kSlot, seed, rows.row<Q>(u), n, channels);
+#pragma unroll
+      for (int i = 0; i < (At::kStats + TH - 1) / TH; ++i) {
+        const int e = at.in_group + i * TH;
+        const int64_t j = set * At::kStats + e;
+        if (e < At::kStats) copy8(stats_at + stage * At::kStats + e, j < 2 * all_rows ? stats + j : stats, j < 2 * all_rows);
+      }
+    }
+    cp_async_commit();
+  };
+  int stage = 0;
+  const int64_t first = blockIdx.x + int64_t(at.group) * gridDim.x;
+  load(first, 0);
+  for (int64_t set = first; set < sets; set += stride, stage ^= 1) {
+    const int64_t u = set * At::kUnits + at.sub;
     const int n = u < units ? rows.count<Q>(u) : 0;
     const bool full = u < rows.full;
     const int64_t row = rows.row<Q>(u);
-    double d[K][Q], g[K][Q], r[Q], sums[2 * Q], w[Q];
+    const double *xs = mine + 2 * stage * At::kSlot, *gs = xs + At::kSlot;
+    double* es = mine + 4 * At::kSlot;
+    const double2* st = reinterpret_cast<const double2*>(stats_at + stage * At::kStats + at.sub * 2 * Q);
+    double r[Q], sums[2 * Q], w[Q];
+    if (skip) at.copy(es, skip, row, n, channels);
+    cp_async_commit();
+    cp_async_wait<1>();  // X, G and stats of this unit
+    at.sync();           // the other lanes' stats; and the next stage's stats have been read
+    load(set + stride, stage ^ 1);
 #pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-      for (int s = 0; s < Q; ++s) {
-        const int c = lane + k * L;
-        const bool ok = s < n && c < channels;
-        d[k][s] = ok ? x[(row + s) * channels + c] : 0.0;
-        g[k][s] = ok ? seed[(row + s) * channels + c] : 0.0;
-      }
-#pragma unroll
-    for (int s = 0; s < Q; ++s) {
-      const double mean = s < n ? stats[2 * (row + s)] : 0.0;
-      r[s] = s < n ? stats[2 * (row + s) + 1] : 0.0;
-      sums[s] = sums[Q + s] = 0.0;
-#pragma unroll
-      for (int k = 0; k < K; ++k) d[k][s] = lane + k * L < channels ? d[k][s] - mean : 0.0;
-    }
+    for (int s = 0; s < 2 * Q; ++s) sums[s] = 0.0;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      double p[Q];
+      if (at.lane + k * L >= channels) continue;
+      double d[Q], g[Q], p[Q];
+#pragma unroll
+      for (int s = 0; s < Q; ++s) {
+        d[s] = xs[(k * Q + s) * TH] - st[s].x;
+        g[s] = gs[(k * Q + s) * TH];
+      }
       if (full) {
-        Jet<DIM>::corr(d[k], g[k], p);
-        dbias[k] += g[k][0];
+        Jet<DIM>::corr(d, g, p);
+        dbias[k] += g[0];
       } else {
 #pragma unroll
         for (int s = 0; s < Q; ++s) {
-          p[s] = d[k][s] * g[k][s];
-          dbias[k] += g[k][s];
+          p[s] = d[s] * g[s];
+          dbias[k] += g[s];
         }
       }
 #pragma unroll
       for (int s = 0; s < Q; ++s) {
-        dgain[k] += r[s] * p[s];
+        dgain[k] += st[s].y * p[s];
         sums[s] += gk[k] * p[s];
-        g[k][s] *= gk[k];
-        sums[Q + s] += g[k][s];
+        sums[Q + s] += gk[k] * g[s];
       }
     }
-    unit_sums<2 * Q, T, W>(sums, shared, turn);
+    __syncwarp();
+    at.sum(sums, sums_at + stage * At::kSums);
+#pragma unroll
+    for (int s = 0; s < Q; ++s) r[s] = st[s].y;
     if (full) {
       double r2[Q], r3[Q];
-      Jet<DIM>::mul(r, r, r2);
+      Jet<DIM>::square(r, r2);
       Jet<DIM>::mul(r2, r, r3);
       Jet<DIM>::corr(r3, sums, w);
     } else {
@@ -399,50 +511,47 @@ __global__ void __launch_bounds__(unit_threads<T, W>())
       w[s] *= -inv;
       sums[Q + s] *= inv;
     }
+    cp_async_wait<1>();  // skip
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int c = lane + k * L;
+      const int c = at.lane + k * L;
       if (c >= channels) continue;
-      double y[Q];
-#pragma unroll
-      for (int s = 0; s < Q; ++s) g[k][s] -= sums[Q + s];
-      if (full) {
-        Jet<DIM>::corr(r, g[k], y);
-        Jet<DIM>::corr_add(d[k], w, y);
-      } else {
-#pragma unroll
-        for (int s = 0; s < Q; ++s) y[s] = r[s] * g[k][s] + d[k][s] * w[s];
-      }
+      double d[Q], g[Q], y[Q];
 #pragma unroll
       for (int s = 0; s < Q; ++s) {
-        if (s >= n) continue;
-        const int64_t at = (row + s) * channels + c;
-        dx[at] = skip ? y[s] + skip[at] : y[s];
+        d[s] = xs[(k * Q + s) * TH] - st[s].x;
+        g[s] = gk[k] * gs[(k * Q + s) * TH] - sums[Q + s];
       }
+      if (full) {
+        Jet<DIM>::corr(r, g, y);
+        Jet<DIM>::corr_add(d, w, y);
+      } else {
+#pragma unroll
+        for (int s = 0; s < Q; ++s) y[s] = r[s] * g[s] + d[s] * w[s];
+      }
+      if (skip) {
+#pragma unroll
+        for (int s = 0; s < Q; ++s) y[s] += es[(k * Q + s) * TH];
+      }
+      At::store(dx, y, row, n, c, channels);
     }
     __syncwarp();
   }
-  double* mine = partials + int64_t(blockIdx.x) * 2 * channels;
-  if constexpr (W > 1) {
+  cp_async_wait<0>();
+  // the block's lanes that share a channel, in order
+  __syncthreads();
 #pragma unroll
-    for (int k = 0; k < K; ++k)
-      if (lane + k * L < channels) {
-        mine[lane + k * L] = dgain[k];
-        mine[channels + lane + k * L] = dbias[k];
-      }
-  } else {  // the block's groups, in order
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      shared[(group * K + k) * T + lane] = dgain[k];
-      shared[K * kNormThreads + (group * K + k) * T + lane] = dbias[k];
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < 2 * K * T; i += kNormThreads) {
-      const int which = i / (K * T), c = i % (K * T);
-      double s = 0.0;
-      for (int q = 0; q < G; ++q) s += shared[which * K * kNormThreads + q * K * T + c];
-      if (c < channels) mine[which * channels + c] = s;
-    }
+  for (int k = 0; k < K; ++k) {
+    const int i = (threadIdx.x / L * K + k) * L + threadIdx.x % L;
+    smem[i] = dgain[k];
+    smem[K * At::kBlock + i] = dbias[k];
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 2 * K * L; i += At::kBlock) {
+    const int which = i / (K * L), c = i % (K * L);
+    double s = 0.0;
+    for (int q = 0; q < At::kBlock / L; ++q) s += smem[which * K * At::kBlock + q * K * L + c];
+    if (c < channels) partials[(int64_t(blockIdx.x) * 2 + which) * channels + c] = s;
   }
 }
 
@@ -469,68 +578,76 @@ __global__ void __launch_bounds__(kFinishStrands* kFinishLanes)
   }
 }
 
-// How a unit is held at a width: calls f(T, K, W) (as integral constants), or says that no
-// register form has it.
 template <int V>
 using Int = std::integral_constant<int, V>;
+// How many lanes share a unit of `channels`: calls f(T, W) (integral constants) with the
+// fewest whose K channels each cover them; false where none do.
 template <int DIM, bool BACKWARD, typename F>
-bool with_unit(int channels, const F& f) {
-  if (channels <= 16) return f(Int<8>{}, Int<2>{}, Int<1>{}), true;
-  if (channels <= 32) return f(Int<16>{}, Int<2>{}, Int<1>{}), true;
-  if constexpr (DIM == 2) {
-    if (channels <= 64) return f(Int<32>{}, Int<2>{}, Int<1>{}), true;
-    if (channels <= 128) return f(Int<32>{}, Int<2>{}, Int<2>{}), true;
-    if (channels <= 256) return f(Int<32>{}, Int<2>{}, Int<4>{}), true;
-  } else {
-    if (channels <= 64) return f(Int<32>{}, Int<1>{}, Int<2>{}), true;
-    if (channels <= 128) return f(Int<32>{}, Int<1>{}, Int<4>{}), true;
-    if (channels <= 256) return f(Int<32>{}, Int<1>{}, Int<8>{}), true;
-  }
-  return false;
+bool with_lanes(int channels, const F& f) {
+  constexpr int K = unit_k<DIM, BACKWARD>();
+  const int lanes = (channels + K - 1) / K;
+  if (lanes <= 8) f(Int<8>{}, Int<1>{});
+  else if (lanes <= 16) f(Int<16>{}, Int<1>{});
+  else if (lanes <= 32) f(Int<32>{}, Int<1>{});
+  else if (lanes <= 64) f(Int<32>{}, Int<2>{});
+  else if (lanes <= 128) f(Int<32>{}, Int<4>{});
+  else if (lanes <= kUnitMostLanes) f(Int<32>{}, Int<8>{});
+  else return false;
+  return true;
 }
 
-// blocks of the backward kernel, each of which keeps one [2][channels] partial: all that are
-// resident at once (at most 16 a multiprocessor), or one for each of its units
-int64_t norm_parts(int dim, Packed rows, int sms) {
-  const int64_t units = dim == 2 ? rows.units<10>() : rows.units<20>(), most = int64_t(sms) * 8;
-  return units < most ? units : most;
+// blocks of the adjoint, each of which keeps one [2][channels] partial: one a multiprocessor
+// where units are streamed, eight of the small ones elsewhere; at most one a unit
+template <int DIM>
+int64_t norm_parts(Packed rows, int channels, int sms) {
+  const bool streamed = with_lanes<DIM, true>(channels, [](auto, auto) {});
+  return std::min(rows.units<Jet<DIM>::Q>(), int64_t(sms) * (streamed ? 1 : 8));
+}
+int64_t norm_parts(int dim, Packed rows, int channels, int sms) {
+  return dim == 2 ? norm_parts<2>(rows, channels, sms) : norm_parts<3>(rows, channels, sms);
 }
 
 template <int DIM>
 cudaError_t launch_norm(const double* x, const double* gain, const double* bias, double* out, double* stats, double eps,
                         Packed rows, int channels, int sms, cudaStream_t stream) {
   const int64_t units = rows.units<Jet<DIM>::Q>();
-  const bool done = with_unit<DIM, false>(channels, [&](auto t, auto k, auto w) {
-    constexpr int T = t, K = k, W = w, G = unit_groups<T, W>();
-    norm_forward_unit<DIM, T, K, W><<<unsigned((units + G - 1) / G), unit_threads<T, W>(), 0, stream>>>(
-        x, gain, bias, out, stats, eps, rows, channels);
+  cudaError_t e = cudaSuccess;
+  const bool done = with_lanes<DIM, false>(channels, [&](auto t, auto w) {
+    using At = Place<DIM, false, t, w>;
+    const auto kernel = norm_forward_unit<DIM, t, w>;
+    const int smem = int(sizeof(double)) * At::kGroups * At::kDoubles;
+    // a per-device attribute: set on every call, so that each device gets it
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess)
+      kernel<<<unsigned(std::min<int64_t>(units, sms)), At::kBlock, smem, stream>>>(x, gain, bias, out, stats, eps, rows,
+                                                                                   channels);
   });
   if (!done)
-    norm_forward<DIM><<<unsigned(norm_parts(DIM, rows, sms)), kNormThreads, 0, stream>>>(x, gain, bias, out, stats, eps,
-                                                                                       rows, channels);
-  return cudaGetLastError();
+    norm_forward<DIM><<<unsigned(std::min(units, int64_t(sms) * 8)), kNormThreads, 0, stream>>>(x, gain, bias, out, stats,
+                                                                                              eps, rows, channels);
+  return e != cudaSuccess ? e : cudaGetLastError();
 }
 
 template <int DIM>
 cudaError_t launch_norm_vjp(const double* x, const double* gain, const double* stats, const double* seed,
                             const double* skip, double* dx, double* dgain, double* dbias, double* partials, Packed rows,
                             int channels, int sms, cudaStream_t stream) {
-  int64_t parts = norm_parts(DIM, rows, sms);
-  const bool done = with_unit<DIM, true>(channels, [&](auto t, auto k, auto w) {
-    constexpr int T = t, K = k, W = w, G = unit_groups<T, W>();
-    const auto kernel = norm_backward_unit<DIM, T, K, W>;
-    const int64_t blocks = (rows.units<Jet<DIM>::Q>() + G - 1) / G;
-    int per_sm = 0;
-    cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, unit_threads<T, W>(), 0);
-    parts = std::min(std::min(parts, blocks), int64_t(sms) * (per_sm > 0 ? per_sm : 1));
-    kernel<<<unsigned(parts), unit_threads<T, W>(), 0, stream>>>(x, gain, stats, seed, skip, dx, partials, rows, channels);
+  const int parts = int(norm_parts<DIM>(rows, channels, sms));
+  cudaError_t e = cudaSuccess;
+  const bool done = with_lanes<DIM, true>(channels, [&](auto t, auto w) {
+    using At = Place<DIM, true, t, w>;
+    const auto kernel = norm_backward_unit<DIM, t, w>;
+    const int smem = int(sizeof(double)) * At::kGroups * At::kDoubles;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess)
+      kernel<<<parts, At::kBlock, smem, stream>>>(x, gain, stats, seed, skip, dx, partials, rows, channels);
   });
   if (!done)
-    norm_backward<DIM><<<unsigned(parts), kNormThreads, 0, stream>>>(x, gain, stats, seed, skip, dx, partials, rows, channels);
-  const cudaError_t e = cudaGetLastError();
+    norm_backward<DIM><<<parts, kNormThreads, 0, stream>>>(x, gain, stats, seed, skip, dx, partials, rows, channels);
+  if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   norm_finish<<<unsigned((2 * int64_t(channels) + kFinishLanes - 1) / kFinishLanes), kFinishStrands * kFinishLanes, 0,
-                stream>>>(partials, int(parts), dgain, dbias, channels);
+                stream>>>(partials, parts, dgain, dbias, channels);
   return cudaGetLastError();
 }
 
@@ -571,7 +688,7 @@ int flashns_b200_layer_norm_vjp_scratch(int dim, int64_t full_points, int64_t va
   int sms = 0;
   cudaError_t e = sm_count(&sms);
   if (e != cudaSuccess) return int(e);
-  *bytes = size_t(norm_parts(dim, Packed{full_points, value_points}, sms)) * 2 * channels * sizeof(double);
+  *bytes = size_t(norm_parts(dim, Packed{full_points, value_points}, channels, sms)) * 2 * channels * sizeof(double);
   return int(cudaSuccess);
 }
 
@@ -598,7 +715,7 @@ int flashns_b200_layer_norm_vjp(int dim, const double* value, const double* gain
   int sms = 0;
   cudaError_t e = sm_count(&sms);
   if (e != cudaSuccess) return int(e);
-  if (scratch_bytes < size_t(norm_parts(dim, rows, sms)) * 2 * small) return int(cudaErrorInvalidValue);
+  if (scratch_bytes < size_t(norm_parts(dim, rows, channels, sms)) * 2 * small) return int(cudaErrorInvalidValue);
   const auto launch = dim == 2 ? launch_norm_vjp<2> : launch_norm_vjp<3>;
   return int(launch(value, gain, stats, seed, skip, d_value, d_gain, d_bias, scratch, rows, channels, sms, stream));
 }
