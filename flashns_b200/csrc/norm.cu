@@ -230,12 +230,15 @@ __device__ __forceinline__ void copy8(double* smem, const double* gmem, bool val
   asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;\n" ::"r"(smem_u32(smem)), "l"(gmem), "r"(valid ? 8 : 0));
 }
 
-template <int DIM, bool BACKWARD, int T, int W>
+template <int DIM, bool BACKWARD, int T, int W, bool EXACT>
 struct Place {
+  static constexpr int kDim = DIM;
+  static constexpr bool kExact = EXACT;
   static constexpr int Q = Jet<DIM>::Q, K = unit_k<DIM, BACKWARD>(), L = T * W, N = BACKWARD ? 2 * Q : Q;
   static constexpr int kUnits = W > 1 ? 1 : 32 / T;         // units of a set, the group's step
   static constexpr int kThreads = 32 * W;                   // of a group
   static constexpr int kSlot = Q * K * kThreads;            // doubles of one set's values
+  static constexpr int kRow = EXACT ? K * L : kThreads, kChannel = EXACT ? L : Q * kThreads;  // strides in a slot
   static constexpr int kSums = (W > 1 ? W : kUnits) * N;    // one buffer of sums
   static constexpr int kStats = BACKWARD ? kUnits * 2 * Q : 0;
   static constexpr int kDoubles = unit_slots<BACKWARD>() * kSlot + 2 * kSums + 2 * kStats;
@@ -250,11 +253,29 @@ struct Place {
   __device__ __forceinline__ void sync() const {
     if constexpr (W == 1) __syncwarp(); else named_sync(1 + group, kThreads);
   }
-  // this lane's values of rows row .. row + n - 1 into its column of `slot`, zeros up to Q rows
-  __device__ __forceinline__ void copy(double* slot, const double* __restrict__ from, int64_t row, int n, int channels) const {
+  __device__ __forceinline__ int column() const { return EXACT ? sub * Q * K * L + lane : in_group; }
+  __device__ __forceinline__ bool has(int k, int channels) const { return EXACT || lane + k * L < channels; }
+  // the set's rows (row .. row + n - 1 are this unit's) into `slot`, zeros up to Q rows
+  __device__ __forceinline__ void copy(double* slot, const double* __restrict__ from, int64_t set, int64_t total,
+                                       int64_t row, int n, int channels) const {
+    if constexpr (EXACT) {
+      const int64_t left = total * (K * L) - set * kSlot;
+      const double* src = from + set * kSlot + 2 * in_group;
+      const unsigned to = smem_u32(slot + 2 * in_group);
+      if (left >= kSlot) {
+#pragma unroll
+        for (int i = 0; i < kSlot; i += 2 * kThreads)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(to + 8u * i), "l"(src + i));
+      } else {
+        for (int i = 0; i < kSlot; i += 2 * kThreads)
+          cp_async16(slot + 2 * in_group + i, 2 * in_group + i < left ? src + i : from, 2 * in_group + i < left);
+      }
+      return;
+    }
+    slot += in_group;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      if (lane + k * L >= channels) continue;
+      if (!has(k, channels)) continue;
       const double* src = from + row * channels + lane + k * L;
       const unsigned to = smem_u32(slot + k * Q * kThreads);
       // rolled up: unrolled, the Q addresses of every array are kept in registers
@@ -292,6 +313,7 @@ struct Place {
   // rows row .. row + n - 1 of channel c
   __device__ __forceinline__ static void store(double* __restrict__ out, const double (&y)[Q], int64_t row, int n, int c,
                                                int channels) {
+    if constexpr (EXACT) channels = K * L;
     double* to = out + row * channels + c;
     if (n == Q) {
 #pragma unroll
@@ -304,17 +326,16 @@ struct Place {
   }
 };
 
-template <int DIM, int T, int W>
-__global__ void __launch_bounds__(Place<DIM, false, T, W>::kBlock, 1)
+template <typename At>
+__global__ void __launch_bounds__(At::kBlock, 1)
     norm_forward_unit(const double* __restrict__ x, const double* __restrict__ gain, const double* __restrict__ bias,
                       double* __restrict__ out, double* __restrict__ stats, double eps, Packed rows, int channels) {
-  using At = Place<DIM, false, T, W>;
-  constexpr int Q = At::Q, K = At::K, L = At::L, TH = At::kThreads;
+  constexpr int DIM = At::kDim, Q = At::Q, K = At::K, L = At::L;
   extern __shared__ __align__(16) double smem[];
   const At at;
   double* buffers = smem + at.group * At::kDoubles;
-  double *mine = buffers + at.in_group, *sums_at = buffers + 2 * At::kSlot;
-  const int64_t units = rows.units<Q>(), sets = (units + At::kUnits - 1) / At::kUnits;
+  double* sums_at = buffers + 2 * At::kSlot;
+  const int64_t total = rows.full * Q + rows.value, units = rows.units<Q>(), sets = (units + At::kUnits - 1) / At::kUnits;
   const int64_t stride = int64_t(gridDim.x) * At::kGroups;
   const double inv = 1.0 / channels;
   double gk[K], bk[K];
@@ -326,28 +347,30 @@ __global__ void __launch_bounds__(Place<DIM, false, T, W>::kBlock, 1)
   }
   auto load = [&](int64_t set, int stage) {
     const int64_t u = set * At::kUnits + at.sub;
-    if (set < sets) at.copy(mine + stage * At::kSlot, x, rows.row<Q>(u), u < units ? rows.count<Q>(u) : 0, channels);
+    if (set < sets)
+      at.copy(buffers + stage * At::kSlot, x, set, total, rows.row<Q>(u), u < units ? rows.count<Q>(u) : 0, channels);
     cp_async_commit();
   };
   int stage = 0;
   const int64_t first = blockIdx.x + int64_t(at.group) * gridDim.x;  // few units: one a block
   load(first, 0);
   for (int64_t set = first; set < sets; set += stride, stage ^= 1) {
-    load(set + stride, stage ^ 1);
     const int64_t u = set * At::kUnits + at.sub;
     const int n = u < units ? rows.count<Q>(u) : 0;  // no rows: the lanes only take part in the sums
     const bool full = u < rows.full;
     const int64_t row = rows.row<Q>(u);
-    const double* xs = mine + stage * At::kSlot;
+    const double* xs = buffers + stage * At::kSlot + at.column();
     double sums[Q], mean[Q], r[Q];
 #pragma unroll
     for (int s = 0; s < Q; ++s) sums[s] = 0.0;
-    cp_async_wait<1>();
+    cp_async_wait<0>();
+    if constexpr (At::kExact) at.sync();  // the other lanes' copies; and the other stage has been read out
+    load(set + stride, stage ^ 1);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      if (at.lane + k * L >= channels) continue;
+      if (!at.has(k, channels)) continue;
 #pragma unroll
-      for (int s = 0; s < Q; ++s) sums[s] += xs[(k * Q + s) * TH];
+      for (int s = 0; s < Q; ++s) sums[s] += xs[k * At::kChannel + s * At::kRow];
     }
     __syncwarp();
     at.sum(sums, sums_at);
@@ -358,10 +381,10 @@ __global__ void __launch_bounds__(Place<DIM, false, T, W>::kBlock, 1)
     }
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      if (at.lane + k * L >= channels) continue;
+      if (!at.has(k, channels)) continue;
       double d[Q], p[Q];
 #pragma unroll
-      for (int s = 0; s < Q; ++s) d[s] = xs[(k * Q + s) * TH] - mean[s];
+      for (int s = 0; s < Q; ++s) d[s] = xs[k * At::kChannel + s * At::kRow] - mean[s];
       if (full) {
         Jet<DIM>::square(d, p);
       } else {
@@ -382,20 +405,22 @@ __global__ void __launch_bounds__(Place<DIM, false, T, W>::kBlock, 1)
 #pragma unroll
       for (int s = 0; s < Q; ++s) r[s] = 1.0 / sqrt(sums[s] + eps);
     }
-    double* st = stats + 2 * row;
+    if (at.lane == 0) {
+      double* st = stats + 2 * row;
 #pragma unroll
-    for (int s = 0; s < Q; ++s)
-      if (at.lane == s % T && s < n) {
-        st[2 * s] = mean[s];
-        st[2 * s + 1] = r[s];
-      }
+      for (int s = 0; s < Q; ++s)
+        if (s < n) {
+          st[2 * s] = mean[s];
+          st[2 * s + 1] = r[s];
+        }
+    }
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int c = at.lane + k * L;
-      if (c >= channels) continue;
+      if (!at.has(k, channels)) continue;
       double d[Q], y[Q];
 #pragma unroll
-      for (int s = 0; s < Q; ++s) d[s] = xs[(k * Q + s) * TH] - mean[s];
+      for (int s = 0; s < Q; ++s) d[s] = xs[k * At::kChannel + s * At::kRow] - mean[s];
       if (full) {
         Jet<DIM>::mul(r, d, y);
 #pragma unroll
@@ -411,17 +436,16 @@ __global__ void __launch_bounds__(Place<DIM, false, T, W>::kBlock, 1)
   cp_async_wait<0>();
 }
 
-template <int DIM, int T, int W>
-__global__ void __launch_bounds__(Place<DIM, true, T, W>::kBlock, 1)
+template <typename At>
+__global__ void __launch_bounds__(At::kBlock, 1)
     norm_backward_unit(const double* __restrict__ x, const double* __restrict__ gain, const double* __restrict__ stats,
                        const double* __restrict__ seed, const double* __restrict__ skip, double* __restrict__ dx,
                        double* __restrict__ partials, Packed rows, int channels) {
-  using At = Place<DIM, true, T, W>;
-  constexpr int Q = At::Q, K = At::K, L = At::L, TH = At::kThreads;
+  constexpr int DIM = At::kDim, Q = At::Q, K = At::K, L = At::L, TH = At::kThreads;
   extern __shared__ __align__(16) double smem[];
   const At at;
   double* buffers = smem + at.group * At::kDoubles;  // [2][X, G], skip
-  double *mine = buffers + at.in_group, *sums_at = buffers + 5 * At::kSlot;
+  double* sums_at = buffers + 5 * At::kSlot;
   double* stats_at = sums_at + 2 * At::kSums;  // [2][unit][Q] of (mean, r)
   const int64_t units = rows.units<Q>(), sets = (units + At::kUnits - 1) / At::kUnits;
   const int64_t stride = int64_t(gridDim.x) * At::kGroups, all_rows = rows.full * Q + rows.value;
@@ -436,9 +460,9 @@ __global__ void __launch_bounds__(Place<DIM, true, T, W>::kBlock, 1)
     const int64_t u = set * At::kUnits + at.sub;
     if (set < sets) {
       const int n = u < units ? rows.count<Q>(u) : 0;
-      double* slot = mine + 2 * stage * At::kSlot;
-      at.copy(slot, x, rows.row<Q>(u), n, channels);
-      at.copy(slot + At::kSlot, seed, rows.row<Q>(u), n, channels);
+      double* slot = buffers + 2 * stage * At::kSlot;
+      at.copy(slot, x, set, all_rows, rows.row<Q>(u), n, channels);
+      at.copy(slot + At::kSlot, seed, set, all_rows, rows.row<Q>(u), n, channels);
 #pragma unroll
       for (int i = 0; i < (At::kStats + TH - 1) / TH; ++i) {
         const int e = at.in_group + i * TH;
@@ -456,25 +480,25 @@ __global__ void __launch_bounds__(Place<DIM, true, T, W>::kBlock, 1)
     const int n = u < units ? rows.count<Q>(u) : 0;
     const bool full = u < rows.full;
     const int64_t row = rows.row<Q>(u);
-    const double *xs = mine + 2 * stage * At::kSlot, *gs = xs + At::kSlot;
-    double* es = mine + 4 * At::kSlot;
+    const double* xs = buffers + 2 * stage * At::kSlot + at.column();
+    const double *gs = xs + At::kSlot, *es = buffers + 4 * At::kSlot + at.column();
     const double2* st = reinterpret_cast<const double2*>(stats_at + stage * At::kStats + at.sub * 2 * Q);
     double r[Q], sums[2 * Q], w[Q];
-    if (skip) at.copy(es, skip, row, n, channels);
+    cp_async_wait<0>();  // X, G and stats of this unit
+    at.sync();           // the other lanes' copies; and the slots loaded next have been read out
+    if (skip) at.copy(buffers + 4 * At::kSlot, skip, set, all_rows, row, n, channels);
     cp_async_commit();
-    cp_async_wait<1>();  // X, G and stats of this unit
-    at.sync();           // the other lanes' stats; and the next stage's stats have been read
     load(set + stride, stage ^ 1);
 #pragma unroll
     for (int s = 0; s < 2 * Q; ++s) sums[s] = 0.0;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      if (at.lane + k * L >= channels) continue;
+      if (!at.has(k, channels)) continue;
       double d[Q], g[Q], p[Q];
 #pragma unroll
       for (int s = 0; s < Q; ++s) {
-        d[s] = xs[(k * Q + s) * TH] - st[s].x;
-        g[s] = gs[(k * Q + s) * TH];
+        d[s] = xs[k * At::kChannel + s * At::kRow] - st[s].x;
+        g[s] = gs[k * At::kChannel + s * At::kRow];
       }
       if (full) {
         Jet<DIM>::corr(d, g, p);
@@ -494,6 +518,7 @@ __global__ void __launch_bounds__(Place<DIM, true, T, W>::kBlock, 1)
       }
     }
     __syncwarp();
+    cp_async_wait<1>();  // skip, which the sums' barrier shows to the other lanes
     at.sum(sums, sums_at + stage * At::kSums);
 #pragma unroll
     for (int s = 0; s < Q; ++s) r[s] = st[s].y;
@@ -511,16 +536,15 @@ __global__ void __launch_bounds__(Place<DIM, true, T, W>::kBlock, 1)
       w[s] *= -inv;
       sums[Q + s] *= inv;
     }
-    cp_async_wait<1>();  // skip
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int c = at.lane + k * L;
-      if (c >= channels) continue;
+      if (!at.has(k, channels)) continue;
       double d[Q], g[Q], y[Q];
 #pragma unroll
       for (int s = 0; s < Q; ++s) {
-        d[s] = xs[(k * Q + s) * TH] - st[s].x;
-        g[s] = gk[k] * gs[(k * Q + s) * TH] - sums[Q + s];
+        d[s] = xs[k * At::kChannel + s * At::kRow] - st[s].x;
+        g[s] = gk[k] * gs[k * At::kChannel + s * At::kRow] - sums[Q + s];
       }
       if (full) {
         Jet<DIM>::corr(r, g, y);
@@ -531,7 +555,7 @@ __global__ void __launch_bounds__(Place<DIM, true, T, W>::kBlock, 1)
       }
       if (skip) {
 #pragma unroll
-        for (int s = 0; s < Q; ++s) y[s] += es[(k * Q + s) * TH];
+        for (int s = 0; s < Q; ++s) y[s] += es[k * At::kChannel + s * At::kRow];
       }
       At::store(dx, y, row, n, c, channels);
     }
@@ -580,27 +604,34 @@ __global__ void __launch_bounds__(kFinishStrands* kFinishLanes)
 
 template <int V>
 using Int = std::integral_constant<int, V>;
-// How many lanes share a unit of `channels`: calls f(T, W) (integral constants) with the
-// fewest whose K channels each cover them; false where none do.
+template <typename A>
+struct Type { using type = A; };
+// How many lanes share a unit of `channels`: calls f(Type<Place<...>>) with the fewest whose K
+// channels each cover them; false where none do.  Exact: they cover no more, and the tensors
+// are aligned.
 template <int DIM, bool BACKWARD, typename F>
-bool with_lanes(int channels, const F& f) {
+bool with_lanes(int channels, bool aligned, const F& f) {
   constexpr int K = unit_k<DIM, BACKWARD>();
   const int lanes = (channels + K - 1) / K;
-  if (lanes <= 8) f(Int<8>{}, Int<1>{});
-  else if (lanes <= 16) f(Int<16>{}, Int<1>{});
-  else if (lanes <= 32) f(Int<32>{}, Int<1>{});
-  else if (lanes <= 64) f(Int<32>{}, Int<2>{});
-  else if (lanes <= 128) f(Int<32>{}, Int<4>{});
-  else if (lanes <= kUnitMostLanes) f(Int<32>{}, Int<8>{});
-  else return false;
-  return true;
+  const auto call = [&](auto t, auto w) {
+    if (aligned && channels == K * t * w) f(Type<Place<DIM, BACKWARD, t, w, true>>{});
+    else f(Type<Place<DIM, BACKWARD, t, w, false>>{});
+    return true;
+  };
+  if (lanes <= 8) return call(Int<8>{}, Int<1>{});
+  if (lanes <= 16) return call(Int<16>{}, Int<1>{});
+  if (lanes <= 32) return call(Int<32>{}, Int<1>{});
+  if (lanes <= 64) return call(Int<32>{}, Int<2>{});
+  if (lanes <= 128) return call(Int<32>{}, Int<4>{});
+  return lanes <= kUnitMostLanes && call(Int<32>{}, Int<8>{});
 }
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // blocks of the adjoint, each of which keeps one [2][channels] partial: one a multiprocessor
 // where units are streamed, eight of the small ones elsewhere; at most one a unit
 template <int DIM>
 int64_t norm_parts(Packed rows, int channels, int sms) {
-  const bool streamed = with_lanes<DIM, true>(channels, [](auto, auto) {});
+  const bool streamed = with_lanes<DIM, true>(channels, false, [](auto) {});
   return std::min(rows.units<Jet<DIM>::Q>(), int64_t(sms) * (streamed ? 1 : 8));
 }
 int64_t norm_parts(int dim, Packed rows, int channels, int sms) {
@@ -612,9 +643,9 @@ cudaError_t launch_norm(const double* x, const double* gain, const double* bias,
                         Packed rows, int channels, int sms, cudaStream_t stream) {
   const int64_t units = rows.units<Jet<DIM>::Q>();
   cudaError_t e = cudaSuccess;
-  const bool done = with_lanes<DIM, false>(channels, [&](auto t, auto w) {
-    using At = Place<DIM, false, t, w>;
-    const auto kernel = norm_forward_unit<DIM, t, w>;
+  const bool done = with_lanes<DIM, false>(channels, aligned16(x), [&](auto place) {
+    using At = typename decltype(place)::type;
+    const auto kernel = norm_forward_unit<At>;
     const int smem = int(sizeof(double)) * At::kGroups * At::kDoubles;
     // a per-device attribute: set on every call, so that each device gets it
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
@@ -634,9 +665,10 @@ cudaError_t launch_norm_vjp(const double* x, const double* gain, const double* s
                             int channels, int sms, cudaStream_t stream) {
   const int parts = int(norm_parts<DIM>(rows, channels, sms));
   cudaError_t e = cudaSuccess;
-  const bool done = with_lanes<DIM, true>(channels, [&](auto t, auto w) {
-    using At = Place<DIM, true, t, w>;
-    const auto kernel = norm_backward_unit<DIM, t, w>;
+  const bool aligned = aligned16(x) && aligned16(seed) && aligned16(skip);
+  const bool done = with_lanes<DIM, true>(channels, aligned, [&](auto place) {
+    using At = typename decltype(place)::type;
+    const auto kernel = norm_backward_unit<At>;
     const int smem = int(sizeof(double)) * At::kGroups * At::kDoubles;
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e == cudaSuccess)
