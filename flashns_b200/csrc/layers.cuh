@@ -112,4 +112,22 @@ inline cudaError_t sm_count(int* sms) {
   return e != cudaSuccess ? e : cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, device);
 }
 
+// Launch that may start while the stream's previous kernel drains; the kernel waits
+// (pdl_wait) before it reads what that one wrote.
+template <typename... P, typename... A>
+cudaError_t launch_dependent(void (*kernel)(P...), unsigned grid, unsigned threads, size_t smem, cudaStream_t stream,
+                             A... args) {
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(grid);
+  config.blockDim = dim3(threads);
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  cudaLaunchAttribute attribute;
+  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &attribute;
+  config.numAttrs = 1;
+  return cudaLaunchKernelEx(&config, kernel, static_cast<P>(args)...);
+}
+
 }  // namespace flashns_b200

@@ -208,13 +208,13 @@ __global__ void __launch_bounds__(kNormThreads)
 // units, so that narrow layers fill their warps); lane l has channels l and l + T W (K of
 // them).  HBM bounds the sizes that matter, but only while a unit costs few instructions: a
 // value is 16 to 32 bytes and some 50 multiply-adds.  So
-//   - a lane copies its own values of the group's next unit into its own column of shared
-//     memory (cp.async, 8 bytes each: any width and alignment, whole lines a warp) while it
-//     works on this one.  No other lane reads them, so no barrier waits for them, and the
-//     fixed column layout leaves no address arithmetic in the passes;
-//   - rows past a short unit are copied as zeros, so no pass tests for them;
+//   - a group copies its next unit, one contiguous run, into shared memory (cp.async, 16 bytes
+//     where the width is even and the tensors aligned) while it works on this one; rows past
+//     the last are copied as zeros, so no pass tests for them;
+//   - a width that the lanes cover exactly is a constant, which leaves no address arithmetic in
+//     the copies and passes (16,384 + 4,096 points, 64 wide: the adjoint 63 us against 86);
 //   - sums over channels are a halving exchange over the lanes (each ends with its own few),
-//     then one shared-memory read that joins the warps and hands all sums to all lanes.
+//     then shared memory joins the warps and hands all sums to all lanes.
 // Blocks are persistent, one a multiprocessor; each has as many groups as its shared memory
 // and registers hold.
 constexpr int kUnitMostLanes = 256;  // lanes of the widest group
@@ -237,9 +237,8 @@ struct Place {
   static constexpr int Q = Jet<DIM>::Q, K = unit_k<DIM, BACKWARD>(), L = T * W, N = BACKWARD ? 2 * Q : Q;
   static constexpr int kUnits = W > 1 ? 1 : 32 / T;         // units of a set, the group's step
   static constexpr int kThreads = 32 * W;                   // of a group
-  static constexpr int kSlot = Q * K * kThreads;            // doubles of one set's values
-  static constexpr int kRow = EXACT ? K * L : kThreads, kChannel = EXACT ? L : Q * kThreads;  // strides in a slot
-  static constexpr int kSums = (W > 1 ? W : kUnits) * N;    // one buffer of sums
+  static constexpr int kSlot = Q * K * kThreads;            // doubles of one set's values, at most
+  static constexpr int kSums = (W > 1 ? 2 * W : kUnits) * N;  // one buffer of sums
   static constexpr int kStats = BACKWARD ? kUnits * 2 * Q : 0;
   static constexpr int kDoubles = unit_slots<BACKWARD>() * kSlot + 2 * kSums + 2 * kStats;
   static constexpr int kGroups = int(kUnitSmem / sizeof(double) / kDoubles) < unit_warps<DIM, BACKWARD>() / W
@@ -253,40 +252,25 @@ struct Place {
   __device__ __forceinline__ void sync() const {
     if constexpr (W == 1) __syncwarp(); else named_sync(1 + group, kThreads);
   }
-  __device__ __forceinline__ int column() const { return EXACT ? sub * Q * K * L + lane : in_group; }
   __device__ __forceinline__ bool has(int k, int channels) const { return EXACT || lane + k * L < channels; }
-  // the set's rows (row .. row + n - 1 are this unit's) into `slot`, zeros up to Q rows
+  // the set's values (a contiguous run; rows past the last as zeros) into `slot`
   __device__ __forceinline__ void copy(double* slot, const double* __restrict__ from, int64_t set, int64_t total,
-                                       int64_t row, int n, int channels) const {
-    if constexpr (EXACT) {
-      const int64_t left = total * (K * L) - set * kSlot;
-      const double* src = from + set * kSlot + 2 * in_group;
+                                       int channels, bool vec) const {
+    const int width = EXACT ? K * L : channels, values = kUnits * Q * width;
+    const int64_t left = total * width - set * values;
+    const double* src = from + set * values;
+    if (EXACT && left >= values) {
       const unsigned to = smem_u32(slot + 2 * in_group);
-      if (left >= kSlot) {
 #pragma unroll
-        for (int i = 0; i < kSlot; i += 2 * kThreads)
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(to + 8u * i), "l"(src + i));
-      } else {
-        for (int i = 0; i < kSlot; i += 2 * kThreads)
-          cp_async16(slot + 2 * in_group + i, 2 * in_group + i < left ? src + i : from, 2 * in_group + i < left);
-      }
-      return;
-    }
-    slot += in_group;
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      if (!has(k, channels)) continue;
-      const double* src = from + row * channels + lane + k * L;
-      const unsigned to = smem_u32(slot + k * Q * kThreads);
-      // rolled up: unrolled, the Q addresses of every array are kept in registers
-#pragma unroll 1
-      for (int s = 0; s < Q; s += 2, src += 2 * int64_t(channels)) {
-        const bool a = s < n, b = s + 1 < n;
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;\n" ::"r"(to + 8u * s * kThreads),
-                     "l"(a ? src : from), "r"(a ? 8 : 0));
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;\n" ::"r"(to + 8u * (s + 1) * kThreads),
-                     "l"(b ? src + channels : from), "r"(b ? 8 : 0));
-      }
+      for (int i = 0; i < kSlot; i += 2 * kThreads)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(to + 8u * i), "l"(src + 2 * in_group + i));
+    } else if ((EXACT || vec) && (left >= values || left % 2 == 0)) {
+      // rolled up: unrolled, every copy's address is kept in registers
+#pragma unroll 2
+      for (int i = 2 * in_group; i < values; i += 2 * kThreads) cp_async16(slot + i, i < left ? src + i : from, i < left);
+    } else {
+#pragma unroll 2
+      for (int i = in_group; i < values; i += kThreads) copy8(slot + i, i < left ? src + i : from, i < left);
     }
   }
   // v: this lane's part of N sums; all of them in every lane of the unit
@@ -298,17 +282,22 @@ struct Place {
     for (int i = 0; i < (N + T - 1) / T + 1; ++i)
       if (first + i < limit) mine[first + i] = v[i];
     sync();
-    const double2* all = reinterpret_cast<const double2*>(W > 1 ? sums : mine);
+    if constexpr (W > 1) {  // every warp joins the warps' sums, a few a lane, into its own copy
+      double* own = sums + W * N + in_group / 32 * N;
 #pragma unroll
-    for (int i = 0; i < N / 2; ++i) {
-      double2 s = all[i];
+      for (int i = threadIdx.x % 32; i < N; i += 32) {
+        double s = sums[i];
 #pragma unroll
-      for (int w = 1; w < W; ++w) {
-        const double2 o = all[w * (N / 2) + i];
-        s.x += o.x, s.y += o.y;
+        for (int w = 1; w < W; ++w) s += sums[w * N + i];
+        own[i] = s;
       }
-      v[2 * i] = s.x, v[2 * i + 1] = s.y;
+      __syncwarp();
+      mine = own;
     }
+    const double2* all = reinterpret_cast<const double2*>(mine);
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) v[2 * i] = all[i].x, v[2 * i + 1] = all[i].y;
+    if constexpr (W > 1) __syncwarp();  // read before the next sums' copy
   }
   // rows row .. row + n - 1 of channel c
   __device__ __forceinline__ static void store(double* __restrict__ out, const double (&y)[Q], int64_t row, int n, int c,
@@ -329,12 +318,13 @@ struct Place {
 template <typename At>
 __global__ void __launch_bounds__(At::kBlock, 1)
     norm_forward_unit(const double* __restrict__ x, const double* __restrict__ gain, const double* __restrict__ bias,
-                      double* __restrict__ out, double* __restrict__ stats, double eps, Packed rows, int channels) {
+                      double* __restrict__ out, double* __restrict__ stats, double eps, Packed rows, int channels, bool vec) {
   constexpr int DIM = At::kDim, Q = At::Q, K = At::K, L = At::L;
   extern __shared__ __align__(16) double smem[];
   const At at;
   double* buffers = smem + at.group * At::kDoubles;
   double* sums_at = buffers + 2 * At::kSlot;
+  const int width = At::kExact ? K * L : channels;
   const int64_t total = rows.full * Q + rows.value, units = rows.units<Q>(), sets = (units + At::kUnits - 1) / At::kUnits;
   const int64_t stride = int64_t(gridDim.x) * At::kGroups;
   const double inv = 1.0 / channels;
@@ -346,9 +336,7 @@ __global__ void __launch_bounds__(At::kBlock, 1)
     bk[k] = c < channels ? bias[c] : 0.0;
   }
   auto load = [&](int64_t set, int stage) {
-    const int64_t u = set * At::kUnits + at.sub;
-    if (set < sets)
-      at.copy(buffers + stage * At::kSlot, x, set, total, rows.row<Q>(u), u < units ? rows.count<Q>(u) : 0, channels);
+    if (set < sets) at.copy(buffers + stage * At::kSlot, x, set, total, channels, vec);
     cp_async_commit();
   };
   int stage = 0;
@@ -359,18 +347,18 @@ __global__ void __launch_bounds__(At::kBlock, 1)
     const int n = u < units ? rows.count<Q>(u) : 0;  // no rows: the lanes only take part in the sums
     const bool full = u < rows.full;
     const int64_t row = rows.row<Q>(u);
-    const double* xs = buffers + stage * At::kSlot + at.column();
+    const double* xs = buffers + stage * At::kSlot + at.sub * Q * width + at.lane;
     double sums[Q], mean[Q], r[Q];
 #pragma unroll
     for (int s = 0; s < Q; ++s) sums[s] = 0.0;
     cp_async_wait<0>();
-    if constexpr (At::kExact) at.sync();  // the other lanes' copies; and the other stage has been read out
+    at.sync();  // the other lanes' copies; and the other stage has been read out
     load(set + stride, stage ^ 1);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       if (!at.has(k, channels)) continue;
 #pragma unroll
-      for (int s = 0; s < Q; ++s) sums[s] += xs[k * At::kChannel + s * At::kRow];
+      for (int s = 0; s < Q; ++s) sums[s] += xs[k * L + s * width];
     }
     __syncwarp();
     at.sum(sums, sums_at);
@@ -384,7 +372,7 @@ __global__ void __launch_bounds__(At::kBlock, 1)
       if (!at.has(k, channels)) continue;
       double d[Q], p[Q];
 #pragma unroll
-      for (int s = 0; s < Q; ++s) d[s] = xs[k * At::kChannel + s * At::kRow] - mean[s];
+      for (int s = 0; s < Q; ++s) d[s] = xs[k * L + s * width] - mean[s];
       if (full) {
         Jet<DIM>::square(d, p);
       } else {
@@ -420,7 +408,7 @@ __global__ void __launch_bounds__(At::kBlock, 1)
       if (!at.has(k, channels)) continue;
       double d[Q], y[Q];
 #pragma unroll
-      for (int s = 0; s < Q; ++s) d[s] = xs[k * At::kChannel + s * At::kRow] - mean[s];
+      for (int s = 0; s < Q; ++s) d[s] = xs[k * L + s * width] - mean[s];
       if (full) {
         Jet<DIM>::mul(r, d, y);
 #pragma unroll
@@ -440,12 +428,13 @@ template <typename At>
 __global__ void __launch_bounds__(At::kBlock, 1)
     norm_backward_unit(const double* __restrict__ x, const double* __restrict__ gain, const double* __restrict__ stats,
                        const double* __restrict__ seed, const double* __restrict__ skip, double* __restrict__ dx,
-                       double* __restrict__ partials, Packed rows, int channels) {
+                       double* __restrict__ partials, Packed rows, int channels, bool vec) {
   constexpr int DIM = At::kDim, Q = At::Q, K = At::K, L = At::L, TH = At::kThreads;
   extern __shared__ __align__(16) double smem[];
   const At at;
   double* buffers = smem + at.group * At::kDoubles;  // [2][X, G], skip
   double* sums_at = buffers + 5 * At::kSlot;
+  const int width = At::kExact ? K * L : channels;
   double* stats_at = sums_at + 2 * At::kSums;  // [2][unit][Q] of (mean, r)
   const int64_t units = rows.units<Q>(), sets = (units + At::kUnits - 1) / At::kUnits;
   const int64_t stride = int64_t(gridDim.x) * At::kGroups, all_rows = rows.full * Q + rows.value;
@@ -457,12 +446,10 @@ __global__ void __launch_bounds__(At::kBlock, 1)
     dgain[k] = dbias[k] = 0.0;
   }
   auto load = [&](int64_t set, int stage) {
-    const int64_t u = set * At::kUnits + at.sub;
     if (set < sets) {
-      const int n = u < units ? rows.count<Q>(u) : 0;
       double* slot = buffers + 2 * stage * At::kSlot;
-      at.copy(slot, x, set, all_rows, rows.row<Q>(u), n, channels);
-      at.copy(slot + At::kSlot, seed, set, all_rows, rows.row<Q>(u), n, channels);
+      at.copy(slot, x, set, all_rows, channels, vec);
+      at.copy(slot + At::kSlot, seed, set, all_rows, channels, vec);
 #pragma unroll
       for (int i = 0; i < (At::kStats + TH - 1) / TH; ++i) {
         const int e = at.in_group + i * TH;
@@ -480,13 +467,13 @@ __global__ void __launch_bounds__(At::kBlock, 1)
     const int n = u < units ? rows.count<Q>(u) : 0;
     const bool full = u < rows.full;
     const int64_t row = rows.row<Q>(u);
-    const double* xs = buffers + 2 * stage * At::kSlot + at.column();
-    const double *gs = xs + At::kSlot, *es = buffers + 4 * At::kSlot + at.column();
+    const double* xs = buffers + 2 * stage * At::kSlot + at.sub * Q * width + at.lane;
+    const double *gs = xs + At::kSlot, *es = buffers + 4 * At::kSlot + at.sub * Q * width + at.lane;
     const double2* st = reinterpret_cast<const double2*>(stats_at + stage * At::kStats + at.sub * 2 * Q);
     double r[Q], sums[2 * Q], w[Q];
     cp_async_wait<0>();  // X, G and stats of this unit
     at.sync();           // the other lanes' copies; and the slots loaded next have been read out
-    if (skip) at.copy(buffers + 4 * At::kSlot, skip, set, all_rows, row, n, channels);
+    if (skip) at.copy(buffers + 4 * At::kSlot, skip, set, all_rows, channels, vec);
     cp_async_commit();
     load(set + stride, stage ^ 1);
 #pragma unroll
@@ -497,8 +484,8 @@ __global__ void __launch_bounds__(At::kBlock, 1)
       double d[Q], g[Q], p[Q];
 #pragma unroll
       for (int s = 0; s < Q; ++s) {
-        d[s] = xs[k * At::kChannel + s * At::kRow] - st[s].x;
-        g[s] = gs[k * At::kChannel + s * At::kRow];
+        d[s] = xs[k * L + s * width] - st[s].x;
+        g[s] = gs[k * L + s * width];
       }
       if (full) {
         Jet<DIM>::corr(d, g, p);
@@ -543,8 +530,8 @@ __global__ void __launch_bounds__(At::kBlock, 1)
       double d[Q], g[Q], y[Q];
 #pragma unroll
       for (int s = 0; s < Q; ++s) {
-        d[s] = xs[k * At::kChannel + s * At::kRow] - st[s].x;
-        g[s] = gk[k] * gs[k * At::kChannel + s * At::kRow] - sums[Q + s];
+        d[s] = xs[k * L + s * width] - st[s].x;
+        g[s] = gk[k] * gs[k * L + s * width] - sums[Q + s];
       }
       if (full) {
         Jet<DIM>::corr(r, g, y);
@@ -555,13 +542,14 @@ __global__ void __launch_bounds__(At::kBlock, 1)
       }
       if (skip) {
 #pragma unroll
-        for (int s = 0; s < Q; ++s) y[s] += es[k * At::kChannel + s * At::kRow];
+        for (int s = 0; s < Q; ++s) y[s] += es[k * L + s * width];
       }
       At::store(dx, y, row, n, c, channels);
     }
     __syncwarp();
   }
   cp_async_wait<0>();
+  pdl_trigger();
   // the block's lanes that share a channel, in order
   __syncthreads();
 #pragma unroll
@@ -579,9 +567,9 @@ __global__ void __launch_bounds__(At::kBlock, 1)
   }
 }
 
-// dgain, dbias [channels] each from partials [parts][2][channels]: 8 strands of parts a value,
+// dgain, dbias [channels] each from partials [parts][2][channels]: 32 strands of parts a value,
 // each in order, then the strands in order
-constexpr int kFinishStrands = 8, kFinishLanes = 32;
+constexpr int kFinishStrands = 32, kFinishLanes = 32;
 __global__ void __launch_bounds__(kFinishStrands* kFinishLanes)
     norm_finish(const double* __restrict__ partials, int parts, double* __restrict__ dgain, double* __restrict__ dbias,
                 int channels) {
@@ -589,6 +577,7 @@ __global__ void __launch_bounds__(kFinishStrands* kFinishLanes)
   const int lane = threadIdx.x % kFinishLanes, strand = threadIdx.x / kFinishLanes;
   const int64_t i = int64_t(blockIdx.x) * kFinishLanes + lane, n = 2 * int64_t(channels);
   double s = 0.0;
+  pdl_wait();
   if (i < n) {
 #pragma unroll 8
     for (int k = strand; k < parts; k += kFinishStrands) s += partials[k * n + i];
@@ -651,7 +640,7 @@ cudaError_t launch_norm(const double* x, const double* gain, const double* bias,
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e == cudaSuccess)
       kernel<<<unsigned(std::min<int64_t>(units, sms)), At::kBlock, smem, stream>>>(x, gain, bias, out, stats, eps, rows,
-                                                                                   channels);
+                                                                                   channels, aligned16(x) && channels % 2 == 0);
   });
   if (!done)
     norm_forward<DIM><<<unsigned(std::min(units, int64_t(sms) * 8)), kNormThreads, 0, stream>>>(x, gain, bias, out, stats,
@@ -672,15 +661,16 @@ cudaError_t launch_norm_vjp(const double* x, const double* gain, const double* s
     const int smem = int(sizeof(double)) * At::kGroups * At::kDoubles;
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e == cudaSuccess)
-      kernel<<<parts, At::kBlock, smem, stream>>>(x, gain, stats, seed, skip, dx, partials, rows, channels);
+      kernel<<<parts, At::kBlock, smem, stream>>>(x, gain, stats, seed, skip, dx, partials, rows, channels,
+                                                  aligned && channels % 2 == 0);
   });
   if (!done)
     norm_backward<DIM><<<parts, kNormThreads, 0, stream>>>(x, gain, stats, seed, skip, dx, partials, rows, channels);
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  norm_finish<<<unsigned((2 * int64_t(channels) + kFinishLanes - 1) / kFinishLanes), kFinishStrands * kFinishLanes, 0,
-                stream>>>(partials, parts, dgain, dbias, channels);
-  return cudaGetLastError();
+  const unsigned blocks = unsigned((2 * int64_t(channels) + kFinishLanes - 1) / kFinishLanes);
+  return launch_dependent(norm_finish, blocks, kFinishStrands * kFinishLanes, 0, stream, partials, parts, dgain, dbias,
+                          channels);
 }
 
 }  // namespace
