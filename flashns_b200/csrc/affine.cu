@@ -45,6 +45,13 @@ size_t fw_smem(int cin) {
   return sizeof(double) * (size_t(NG) * NS * kFwUnits * fw_unit_stride<DIM>() + kFwCB * ld * (STREAM ? NG * NS : 1));
 }
 
+// hides a loop-invariant stride, so that its multiples are formed where they are used and not
+// kept in registers through the MMAs
+__device__ __forceinline__ int64_t opaque(int64_t v) {
+  asm volatile("mov.b64 %0, %0;" : "+l"(v));
+  return v;
+}
+__device__ __forceinline__ void prefetch_line(const void* gmem) { asm volatile("prefetch.global.L2 [%0];\n" ::"l"(gmem)); }
 __device__ __forceinline__ void cp_async8(void* smem, const void* gmem, bool valid) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;\n" ::"r"(smem_u32(smem)), "l"(gmem), "r"(valid ? 8 : 0));
 }
@@ -78,6 +85,7 @@ __device__ __forceinline__ void forward_epilogue(const double (&acc)[Jet<DIM>::Q
   const bool full = u < rows.full, two = c + 1 < cout;
   const int n = rows.count<Q>(u);
   const int64_t at = rows.row<Q>(u) * cout + c;
+  const bool whole = vec && n == Q;
   double h0[Q], h1[Q], a0, a1;
 #pragma unroll
   for (int s = 0; s < Q; ++s) {
@@ -105,24 +113,38 @@ __device__ __forceinline__ void forward_epilogue(const double (&acc)[Jet<DIM>::Q
       }
     }
   }
+  if (whole) {
+    const int64_t step = opaque(cout);
+    if (activated) {
+      double* to = activated + at;
+#pragma unroll
+      for (int s = 0; s < Q; ++s, to += step) *reinterpret_cast<double2*>(to) = make_double2(h0[s], h1[s]);
+    }
+    if (residual) {
+      const double* from = residual + at;
+#pragma unroll
+      for (int half = 0; half < Q; half += 10) {  // ten rows requested at once
+        double2 r[10];
+#pragma unroll
+        for (int s = 0; s < 10; ++s, from += step) r[s] = *reinterpret_cast<const double2*>(from);
+#pragma unroll
+        for (int s = 0; s < 10; ++s) h0[half + s] += r[s].x, h1[half + s] += r[s].y;
+      }
+    }
+    double* to = out + at;
+#pragma unroll
+    for (int s = 0; s < Q; ++s, to += step) *reinterpret_cast<double2*>(to) = make_double2(h0[s], h1[s]);
+    return;
+  }
 #pragma unroll
   for (int s = 0; s < Q; ++s) {
     if (s >= n) continue;
     const int64_t i = at + int64_t(s) * cout;
-    if (vec) {
-      if (activated) *reinterpret_cast<double2*>(activated + i) = make_double2(h0[s], h1[s]);
-      if (residual) {
-        const double2 r = *reinterpret_cast<const double2*>(residual + i);
-        h0[s] += r.x, h1[s] += r.y;
-      }
-      *reinterpret_cast<double2*>(out + i) = make_double2(h0[s], h1[s]);
-    } else {
-      if (activated) activated[i] = h0[s];
-      out[i] = residual ? h0[s] + residual[i] : h0[s];
-      if (two) {
-        if (activated) activated[i + 1] = h1[s];
-        out[i + 1] = residual ? h1[s] + residual[i + 1] : h1[s];
-      }
+    if (activated) activated[i] = h0[s];
+    out[i] = residual ? h0[s] + residual[i] : h0[s];
+    if (two) {
+      if (activated) activated[i + 1] = h1[s];
+      out[i + 1] = residual ? h1[s] + residual[i + 1] : h1[s];
     }
   }
 }
@@ -149,12 +171,19 @@ __global__ void __launch_bounds__(NG* kFwGroup, 1)
     const int64_t r0 = (first + step / nk * per * NG) * RT;
     const int k0 = int(step % nk) * KC, stage = int(step % NS);
     double* dst = ring + stage * kFwUnits * US;
-    if (vec_in) {
+    if (vec_in) {  // 16 lanes a row, rows sub, sub + 2, ... of each unit
+      const int unit = (gt >> 4) & 3, sub = gt >> 6, k = 2 * (gt & 15);
+      const int64_t r = r0 + unit * Q + sub, step = opaque(2 * int64_t(cin));
+      const double* src = hidden + r * cin + k0 + k;
+      double* to = dst + unit * US + sub * kFwLD + k;
+      if (r0 + RT <= total && k0 + k < cin) {  // cin even: covers k + 1
 #pragma unroll
-      for (int e = gt; e < RT * (KC / 2); e += kFwGroup) {
-        const int r = e / (KC / 2), k = 2 * (e % (KC / 2));
-        const bool ok = r0 + r < total && k0 + k < cin;  // cin even: covers k + 1
-        cp_async16(dst + r / Q * US + r % Q * kFwLD + k, ok ? hidden + (r0 + r) * cin + k0 + k : hidden, ok);
+        for (int i = 0; i < Q / 2; ++i, src += step) cp_async16(to + 2 * i * kFwLD, src, true);
+      } else {
+        for (int i = 0; i < Q / 2; ++i, src += step) {
+          const bool ok = r + 2 * i < total && k0 + k < cin;
+          cp_async16(to + 2 * i * kFwLD, ok ? src : hidden, ok);
+        }
       }
     } else {
       for (int e = gt; e < RT * KC; e += kFwGroup) {
@@ -191,6 +220,15 @@ __global__ void __launch_bounds__(NG* kFwGroup, 1)
       for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[j][e] = 0.0;
+      if (residual) {  // the tile's residual towards L2, for the epilogue
+        const int64_t r0 = (first + step / nk * per * NG) * RT;
+        const int width = cout - c0 < kFwCB ? cout - c0 : kFwCB;
+        for (int e = gt; e < RT * (kFwCB / 16); e += kFwGroup) {
+          const int64_t r = r0 + e / (kFwCB / 16);
+          const int k = e % (kFwCB / 16) * 16;
+          if (r < total && k < width) prefetch_line(residual + r * cout + c0 + k);
+        }
+      }
     }
     const double* bp = ring + stage * kFwUnits * US + (g >> 1) * US + (g & 1) * kFwLD + t;
     const double* ap = sw + (STREAM ? stage * kFwCB * ldw : kc * KC) + ch * ldw + t;
