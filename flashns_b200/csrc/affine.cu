@@ -149,27 +149,53 @@ __device__ __forceinline__ void forward_epilogue(const double (&acc)[Jet<DIM>::Q
   }
 }
 
+// eight input channels of a tile: A rows ap and ap + ldw, B columns of n8 tile j at row 2 j
+template <int NT>
+__device__ __forceinline__ void forward_step(double (&acc)[NT][4], const double* ap, int ldw, const double* bp) {
+  const double a[4] = {ap[0], ap[ldw], ap[4], ap[ldw + 4]};
+#pragma unroll
+  for (int j = 0; j < NT; ++j) mma_m16n8k8(acc[j], a, bp[2 * j * kFwLD], bp[2 * j * kFwLD + 4]);
+}
+
+// Two groups' turns on the tensor pipe, g and g + NG / 2: a group runs a tile's MMAs between
+// take and pass, so its epilogue runs under the partner's MMAs.  A turn barrier counts its
+// group syncing and the partner arriving; the later group opens with one arrival, and the
+// closing sync takes up the one arrival that is left over (the first group's tiles are as many
+// as the second's, or one more).
+template <int NG, bool TURNS>
+struct PairTurns {
+  int mine, other;
+  bool second;
+  __device__ PairTurns(int g) : mine(1 + NG + g), other(1 + NG + (g + NG / 2) % NG), second(g >= NG / 2) {
+    if (TURNS && second) named_arrive(other, 2 * kFwGroup);
+  }
+  __device__ void take() const { if (TURNS) named_sync(mine, 2 * kFwGroup); }
+  __device__ void pass() const { if (TURNS) named_arrive(other, 2 * kFwGroup); }
+  __device__ void close(int64_t tiles, int64_t partner) const {
+    if (TURNS && (second ? partner > tiles : partner + 1 > tiles)) named_sync(mine, 2 * kFwGroup);
+  }
+};
+
 template <int DIM, bool ACT, int NG, int NS, bool STREAM>
 __global__ void __launch_bounds__(NG* kFwGroup, 1)
     affine_forward(const double* __restrict__ hidden, const double* __restrict__ weight, const double* __restrict__ bias,
                    const double* __restrict__ residual, double* __restrict__ out, double* __restrict__ activated,
                    double* __restrict__ aux, Packed rows, int cin, int cout, bool vec_in, bool vec_out) {
   constexpr int Q = Jet<DIM>::Q, NT = Q / 2, US = fw_unit_stride<DIM>(), RT = kFwUnits * Q, KC = kFwKC;
+  constexpr bool TURNS = NG % 2 == 0;
   extern __shared__ __align__(16) double smem[];
   const int tid = threadIdx.x, group = tid / kFwGroup, gt = tid % kFwGroup, warp = gt >> 5;
   const int lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int blocks = (cout + kFwCB - 1) / kFwCB, cb = blockIdx.x % blocks, c0 = cb * kFwCB;
   const int64_t per = gridDim.x / blocks, units = rows.units<Q>(), total = rows.full * Q + rows.value;
   const int64_t tiles = (units + kFwUnits - 1) / kFwUnits, first = blockIdx.x / blocks + group * per;
-  const int64_t mine = first < tiles ? (tiles - 1 - first) / (per * NG) + 1 : 0;
+  const auto count = [&](int64_t from) { return from < tiles ? (tiles - 1 - from) / (per * NG) + 1 : 0; };
+  const int64_t mine = count(first);
   const int nk = (cin + KC - 1) / KC, ldw = STREAM ? KC + 2 : nk * KC + 2;
   double* ring = smem + group * NS * kFwUnits * US;
   double* sw = smem + NG * NS * kFwUnits * US + (STREAM ? group * NS * kFwCB * ldw : 0);
-  const int64_t steps = mine * nk;
-
-  auto load = [&](int64_t step) {
-    const int64_t r0 = (first + step / nk * per * NG) * RT;
-    const int k0 = int(step % nk) * KC, stage = int(step % NS);
+  const int64_t tile_step = per * NG;
+  auto load_chunk = [&](int64_t r0, int k0, int stage) {
     double* dst = ring + stage * kFwUnits * US;
     if (vec_in) {  // 16 lanes a row, rows sub, sub + 2, ... of each unit
       const int unit = (gt >> 4) & 3, sub = gt >> 6, k = 2 * (gt & 15);
@@ -195,57 +221,66 @@ __global__ void __launch_bounds__(NG* kFwGroup, 1)
     if constexpr (STREAM)
       load_weight(sw + stage * kFwCB * ldw, ldw, weight, c0, k0, KC, cin, cout, vec_in, gt, kFwGroup);
   };
+  // the next chunk to load: its tile, K chunk and stage
+  int64_t load_tile = first;
+  int load_kc = 0, load_stage = 0;
+
+  auto load = [&] {
+    if (load_tile < tiles) load_chunk(load_tile * RT, load_kc * KC, load_stage);
+    cp_async_commit();
+    load_stage = load_stage + 1 == NS ? 0 : load_stage + 1;
+    if (++load_kc == nk) load_kc = 0, load_tile += tile_step;
+  };
 
   if constexpr (!STREAM) load_weight(sw, ldw, weight, c0, 0, nk * KC, cin, cout, vec_in, tid, NG * kFwGroup);
   cp_async_commit();
 #pragma unroll
-  for (int s = 0; s < NS - 1; ++s) {
-    if (s < steps) load(s);
-    cp_async_commit();
-  }
+  for (int s = 0; s < NS - 1; ++s) load();
   cp_async_wait<NS - 1>();
   __syncthreads();  // W is there for every group
 
   const int ch = warp * 16 + 2 * g, c = c0 + ch;  // this thread's channels c, c + 1
   const double b0 = c < cout ? bias[c] : 0.0, b1 = c + 1 < cout ? bias[c + 1] : 0.0;
   double acc[NT][4];
-  for (int64_t step = 0; step < steps; ++step) {
-    const int kc = int(step % nk), stage = int(step % NS);
-    cp_async_wait<NS - 2>();
-    named_sync(1 + group, kFwGroup);  // the step's tile is there, the stage loaded next is read out
-    if (step + NS - 1 < steps) load(step + NS - 1);
-    cp_async_commit();
-    if (kc == 0) {
+  const PairTurns<NG, TURNS> turns(group);
+  int stage = 0;
+  for (int64_t tile = first; tile < tiles; tile += tile_step) {
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
+    for (int j = 0; j < NT; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[j][e] = 0.0;
-      if (residual) {  // the tile's residual towards L2, for the epilogue
-        const int64_t r0 = (first + step / nk * per * NG) * RT;
-        const int width = cout - c0 < kFwCB ? cout - c0 : kFwCB;
-        for (int e = gt; e < RT * (kFwCB / 16); e += kFwGroup) {
-          const int64_t r = r0 + e / (kFwCB / 16);
-          const int k = e % (kFwCB / 16) * 16;
-          if (r < total && k < width) prefetch_line(residual + r * cout + c0 + k);
-        }
+      for (int e = 0; e < 4; ++e) acc[j][e] = 0.0;
+    if (residual) {  // the tile's residual towards L2, for the epilogue
+      const int width = cout - c0 < kFwCB ? cout - c0 : kFwCB;
+      for (int e = gt; e < RT * (kFwCB / 16); e += kFwGroup) {
+        const int64_t r = tile * RT + e / (kFwCB / 16);
+        const int k = e % (kFwCB / 16) * 16;
+        if (r < total && k < width) prefetch_line(residual + r * cout + c0 + k);
       }
     }
-    const double* bp = ring + stage * kFwUnits * US + (g >> 1) * US + (g & 1) * kFwLD + t;
-    const double* ap = sw + (STREAM ? stage * kFwCB * ldw : kc * KC) + ch * ldw + t;
-    const int left = cin - kc * KC, ks = left < KC ? (left + 7) / 8 : KC / 8;
-#pragma unroll 2
-    for (int k = 0; k < ks; ++k) {
-      const double a[4] = {ap[8 * k], ap[8 * k + ldw], ap[8 * k + 4], ap[8 * k + ldw + 4]};
+    for (int kc = 0; kc < nk; ++kc) {
+      cp_async_wait<NS - 2>();
+      named_sync(1 + group, kFwGroup);  // the chunk is there, the stage loaded next is read out
+      load();
+      if (kc == 0) turns.take();
+      const double* bp = ring + stage * kFwUnits * US + (g >> 1) * US + (g & 1) * kFwLD + t;
+      const double* ap = sw + (STREAM ? stage * kFwCB * ldw : kc * KC) + ch * ldw + t;
+      const int left = cin - kc * KC;
+      if (left >= KC) {
 #pragma unroll
-      for (int j = 0; j < NT; ++j) mma_m16n8k8(acc[j], a, bp[2 * j * kFwLD + 8 * k], bp[2 * j * kFwLD + 8 * k + 4]);
+        for (int k = 0; k < KC / 8; ++k) forward_step<NT>(acc, ap + 8 * k, ldw, bp + 8 * k);
+      } else {
+#pragma unroll 1
+        for (int k = 0; k < (left + 7) / 8; ++k) forward_step<NT>(acc, ap + 8 * k, ldw, bp + 8 * k);
+      }
+      stage = stage + 1 == NS ? 0 : stage + 1;
     }
-    if (kc + 1 == nk) {
-      const int64_t u = (first + step / nk * per * NG) * kFwUnits + t;
-      if (u < units && c < cout)
-        forward_epilogue<DIM, ACT>(acc, b0, b1, u, c, rows, cout, residual, out, activated, aux, vec_out);
-      __syncwarp();
-    }
+    turns.pass();
+    const int64_t u = tile * kFwUnits + t;
+    if (u < units && c < cout)
+      forward_epilogue<DIM, ACT>(acc, b0, b1, u, c, rows, cout, residual, out, activated, aux, vec_out);
+    __syncwarp();
   }
+  turns.close(mine, count(blockIdx.x / blocks + (group + NG / 2) % NG * per));
   cp_async_wait<0>();
 }
 
