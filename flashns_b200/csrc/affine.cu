@@ -35,14 +35,14 @@ __device__ __forceinline__ void tanh_vjp(const double* h, double a1, const doubl
 // stage, NS stages of cp.async) and meets only its own named barrier, so one group's epilogue
 // runs under the others' MMAs and loads.  Rows are padded to 36 doubles, W's to 2 (mod 8), and
 // a 3-D unit by 8 more: every fragment load is free of bank conflicts.
-constexpr int kFwUnits = 4, kFwKC = 32, kFwLD = kFwKC + 4, kFwCB = 64, kFwGroup = 128;
+constexpr int kFwKC = 32, kFwLD = kFwKC + 4, kFwCB = 64;
 
 template <int DIM>
 constexpr int fw_unit_stride() { return Jet<DIM>::Q * kFwLD + (DIM == 3 ? 8 : 0); }
-template <int DIM, int NG, int NS, bool STREAM>
+template <int DIM, int NG, int GW, int NS, bool STREAM>
 size_t fw_smem(int cin) {
   const size_t ld = STREAM ? kFwKC + 2 : (size_t(cin) + kFwKC - 1) / kFwKC * kFwKC + 2;
-  return sizeof(double) * (size_t(NG) * NS * kFwUnits * fw_unit_stride<DIM>() + kFwCB * ld * (STREAM ? NG * NS : 1));
+  return sizeof(double) * (size_t(NG) * NS * GW * fw_unit_stride<DIM>() + kFwCB * ld * (STREAM ? NG * NS : 1));
 }
 
 // hides a loop-invariant stride, so that its multiples are formed where they are used and not
@@ -75,24 +75,21 @@ __device__ __forceinline__ void load_weight(double* dst, int ld, const double* _
   }
 }
 
-// the accumulators of unit u, channels c and c + 1, through bias, tanh jet and residual
+// Bias and tanh jet of unit u, channels c and c + 1: the accumulators' rows into h0, h1; a1 is
+// stored here.
 template <int DIM, bool ACT>
-__device__ __forceinline__ void forward_epilogue(const double (&acc)[Jet<DIM>::Q / 2][4], double b0, double b1, int64_t u,
-                                                 int c, const Packed& rows, int cout,
-                                                 const double* __restrict__ residual, double* __restrict__ out,
-                                                 double* __restrict__ activated, double* __restrict__ aux, bool vec) {
+__device__ __forceinline__ void forward_jets(const double (&acc)[Jet<DIM>::Q / 2][4], double b0, double b1, int64_t u,
+                                             int c, const Packed& rows, int cout, double* __restrict__ aux, bool two,
+                                             double (&h0)[Jet<DIM>::Q], double (&h1)[Jet<DIM>::Q]) {
   constexpr int Q = Jet<DIM>::Q;
-  const bool full = u < rows.full, two = c + 1 < cout;
-  const int n = rows.count<Q>(u);
-  const int64_t at = rows.row<Q>(u) * cout + c;
-  const bool whole = vec && n == Q;
-  double h0[Q], h1[Q], a0, a1;
+  const bool full = u < rows.full;
 #pragma unroll
   for (int s = 0; s < Q; ++s) {
     h0[s] = acc[s >> 1][s & 1] + (s == 0 || !full ? b0 : 0.0);
     h1[s] = acc[s >> 1][2 + (s & 1)] + (s == 0 || !full ? b1 : 0.0);
   }
   if constexpr (ACT) {
+    double a0, a1;
     if (full) {
       tanh_forward<DIM>(h0, h0, a0);
       tanh_forward<DIM>(h1, h1, a1);
@@ -101,6 +98,7 @@ __device__ __forceinline__ void forward_epilogue(const double (&acc)[Jet<DIM>::Q
         if (two) aux[u * cout + c + 1] = a1;
       }
     } else {
+      const int n = rows.count<Q>(u);
       double* ax = aux ? aux + (rows.full + (u - rows.full) * Q) * cout + c : nullptr;
 #pragma unroll
       for (int s = 0; s < Q; ++s) {
@@ -113,6 +111,17 @@ __device__ __forceinline__ void forward_epilogue(const double (&acc)[Jet<DIM>::Q
       }
     }
   }
+}
+
+// h0, h1 of unit u to `activated`, and with the residual to `out`
+template <int DIM>
+__device__ __forceinline__ void forward_store(double (&h0)[Jet<DIM>::Q], double (&h1)[Jet<DIM>::Q], int64_t u, int c,
+                                              const Packed& rows, int cout, const double* __restrict__ residual,
+                                              double* __restrict__ out, double* __restrict__ activated, bool vec, bool two) {
+  constexpr int Q = Jet<DIM>::Q;
+  const int n = rows.count<Q>(u);
+  const int64_t at = rows.row<Q>(u) * cout + c;
+  const bool whole = vec && n == Q;
   if (whole) {
     const int64_t step = opaque(cout);
     if (activated) {
@@ -157,48 +166,48 @@ __device__ __forceinline__ void forward_step(double (&acc)[NT][4], const double*
   for (int j = 0; j < NT; ++j) mma_m16n8k8(acc[j], a, bp[2 * j * kFwLD], bp[2 * j * kFwLD + 4]);
 }
 
-// Two groups' turns on the tensor pipe, g and g + NG / 2: a group runs a tile's MMAs between
-// take and pass, so its epilogue runs under the partner's MMAs.  A turn barrier counts its
-// group syncing and the partner arriving; the later group opens with one arrival, and the
-// closing sync takes up the one arrival that is left over (the first group's tiles are as many
-// as the second's, or one more).
-template <int NG, bool TURNS>
-struct PairTurns {
-  int mine, other;
-  bool second;
-  __device__ PairTurns(int g) : mine(1 + NG + g), other(1 + NG + (g + NG / 2) % NG), second(g >= NG / 2) {
-    if (TURNS && second) named_arrive(other, 2 * kFwGroup);
+// The groups' turns on the tensor pipe: group g runs a tile's MMAs between take and pass, after
+// group g - 1 (group 0 after the last).  Turn barrier g counts group g syncing and its
+// predecessor arriving; the last group opens the ring with one arrival, and a group whose
+// predecessor arrived once more than it synced closes with one more sync (tiles are dealt in
+// turn, so the groups' counts differ by at most one).
+template <int NG, int THREADS>
+struct Turns {
+  int g;
+  __device__ explicit Turns(int group) : g(group) {
+    if (g == NG - 1) named_arrive(1 + NG, 2 * THREADS);
   }
-  __device__ void take() const { if (TURNS) named_sync(mine, 2 * kFwGroup); }
-  __device__ void pass() const { if (TURNS) named_arrive(other, 2 * kFwGroup); }
-  __device__ void close(int64_t tiles, int64_t partner) const {
-    if (TURNS && (second ? partner > tiles : partner + 1 > tiles)) named_sync(mine, 2 * kFwGroup);
+  __device__ void take() const { named_sync(1 + NG + g, 2 * THREADS); }
+  __device__ void pass() const { named_arrive(1 + NG + (g + 1) % NG, 2 * THREADS); }
+  // tiles of this group and of its predecessor
+  __device__ void close(int64_t mine, int64_t before) const {
+    if (before + (g == 0) > mine) named_sync(1 + NG + g, 2 * THREADS);
   }
 };
 
-template <int DIM, bool ACT, int NG, int NS, bool STREAM>
-__global__ void __launch_bounds__(NG* kFwGroup, 1)
+template <int DIM, bool ACT, int NG, int GW, int NS, bool STREAM>
+__global__ void __launch_bounds__(NG* GW * 32, 1)
     affine_forward(const double* __restrict__ hidden, const double* __restrict__ weight, const double* __restrict__ bias,
                    const double* __restrict__ residual, double* __restrict__ out, double* __restrict__ activated,
                    double* __restrict__ aux, Packed rows, int cin, int cout, bool vec_in, bool vec_out) {
-  constexpr int Q = Jet<DIM>::Q, NT = Q / 2, US = fw_unit_stride<DIM>(), RT = kFwUnits * Q, KC = kFwKC;
-  constexpr bool TURNS = NG % 2 == 0;
+  constexpr int Q = Jet<DIM>::Q, NT = Q / 2, US = fw_unit_stride<DIM>(), KC = kFwKC;
+  constexpr int GT = 32 * GW, UT = GW, RT = UT * Q;  // a group's threads; units and rows of its tile
   extern __shared__ __align__(16) double smem[];
-  const int tid = threadIdx.x, group = tid / kFwGroup, gt = tid % kFwGroup, warp = gt >> 5;
+  const int tid = threadIdx.x, group = tid / GT, gt = tid % GT, wc = (gt >> 5) & 3, wr = gt >> 7;
   const int lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int blocks = (cout + kFwCB - 1) / kFwCB, cb = blockIdx.x % blocks, c0 = cb * kFwCB;
   const int64_t per = gridDim.x / blocks, units = rows.units<Q>(), total = rows.full * Q + rows.value;
-  const int64_t tiles = (units + kFwUnits - 1) / kFwUnits, first = blockIdx.x / blocks + group * per;
+  const int64_t tiles = (units + UT - 1) / UT, first = blockIdx.x / blocks + group * per;
   const auto count = [&](int64_t from) { return from < tiles ? (tiles - 1 - from) / (per * NG) + 1 : 0; };
   const int64_t mine = count(first);
   const int nk = (cin + KC - 1) / KC, ldw = STREAM ? KC + 2 : nk * KC + 2;
-  double* ring = smem + group * NS * kFwUnits * US;
-  double* sw = smem + NG * NS * kFwUnits * US + (STREAM ? group * NS * kFwCB * ldw : 0);
+  double* ring = smem + group * NS * UT * US;
+  double* sw = smem + NG * NS * UT * US + (STREAM ? group * NS * kFwCB * ldw : 0);
   const int64_t tile_step = per * NG;
   auto load_chunk = [&](int64_t r0, int k0, int stage) {
-    double* dst = ring + stage * kFwUnits * US;
+    double* dst = ring + stage * UT * US;
     if (vec_in) {  // 16 lanes a row, rows sub, sub + 2, ... of each unit
-      const int unit = (gt >> 4) & 3, sub = gt >> 6, k = 2 * (gt & 15);
+      const int unit = (gt >> 4) % UT, sub = (gt >> 4) / UT, k = 2 * (gt & 15);
       const int64_t r = r0 + unit * Q + sub, step = opaque(2 * int64_t(cin));
       const double* src = hidden + r * cin + k0 + k;
       double* to = dst + unit * US + sub * kFwLD + k;
@@ -212,14 +221,14 @@ __global__ void __launch_bounds__(NG* kFwGroup, 1)
         }
       }
     } else {
-      for (int e = gt; e < RT * KC; e += kFwGroup) {
+      for (int e = gt; e < RT * KC; e += GT) {
         const int r = e / KC, k = e % KC;
         const bool ok = r0 + r < total && k0 + k < cin;
         cp_async8(dst + r / Q * US + r % Q * kFwLD + k, ok ? hidden + (r0 + r) * cin + k0 + k : hidden, ok);
       }
     }
     if constexpr (STREAM)
-      load_weight(sw + stage * kFwCB * ldw, ldw, weight, c0, k0, KC, cin, cout, vec_in, gt, kFwGroup);
+      load_weight(sw + stage * kFwCB * ldw, ldw, weight, c0, k0, KC, cin, cout, vec_in, gt, GT);
   };
   // the next chunk to load: its tile, K chunk and stage
   int64_t load_tile = first;
@@ -232,17 +241,17 @@ __global__ void __launch_bounds__(NG* kFwGroup, 1)
     if (++load_kc == nk) load_kc = 0, load_tile += tile_step;
   };
 
-  if constexpr (!STREAM) load_weight(sw, ldw, weight, c0, 0, nk * KC, cin, cout, vec_in, tid, NG * kFwGroup);
+  if constexpr (!STREAM) load_weight(sw, ldw, weight, c0, 0, nk * KC, cin, cout, vec_in, tid, NG * GT);
   cp_async_commit();
 #pragma unroll
   for (int s = 0; s < NS - 1; ++s) load();
   cp_async_wait<NS - 1>();
   __syncthreads();  // W is there for every group
 
-  const int ch = warp * 16 + 2 * g, c = c0 + ch;  // this thread's channels c, c + 1
+  const int ch = wc * 16 + 2 * g, c = c0 + ch;  // this thread's channels c, c + 1
   const double b0 = c < cout ? bias[c] : 0.0, b1 = c + 1 < cout ? bias[c + 1] : 0.0;
   double acc[NT][4];
-  const PairTurns<NG, TURNS> turns(group);
+  const Turns<NG, GT> turns(group);
   int stage = 0;
   for (int64_t tile = first; tile < tiles; tile += tile_step) {
 #pragma unroll
@@ -251,7 +260,7 @@ __global__ void __launch_bounds__(NG* kFwGroup, 1)
       for (int e = 0; e < 4; ++e) acc[j][e] = 0.0;
     if (residual) {  // the tile's residual towards L2, for the epilogue
       const int width = cout - c0 < kFwCB ? cout - c0 : kFwCB;
-      for (int e = gt; e < RT * (kFwCB / 16); e += kFwGroup) {
+      for (int e = gt; e < RT * (kFwCB / 16); e += GT) {
         const int64_t r = tile * RT + e / (kFwCB / 16);
         const int k = e % (kFwCB / 16) * 16;
         if (r < total && k < width) prefetch_line(residual + r * cout + c0 + k);
@@ -259,10 +268,10 @@ __global__ void __launch_bounds__(NG* kFwGroup, 1)
     }
     for (int kc = 0; kc < nk; ++kc) {
       cp_async_wait<NS - 2>();
-      named_sync(1 + group, kFwGroup);  // the chunk is there, the stage loaded next is read out
+      named_sync(1 + group, GT);  // the chunk is there, the stage loaded next is read out
       load();
       if (kc == 0) turns.take();
-      const double* bp = ring + stage * kFwUnits * US + (g >> 1) * US + (g & 1) * kFwLD + t;
+      const double* bp = ring + stage * UT * US + (wr * 4 + (g >> 1)) * US + (g & 1) * kFwLD + t;
       const double* ap = sw + (STREAM ? stage * kFwCB * ldw : kc * KC) + ch * ldw + t;
       const int left = cin - kc * KC;
       if (left >= KC) {
@@ -275,49 +284,176 @@ __global__ void __launch_bounds__(NG* kFwGroup, 1)
       stage = stage + 1 == NS ? 0 : stage + 1;
     }
     turns.pass();
-    const int64_t u = tile * kFwUnits + t;
-    if (u < units && c < cout)
-      forward_epilogue<DIM, ACT>(acc, b0, b1, u, c, rows, cout, residual, out, activated, aux, vec_out);
+    const int64_t u = tile * UT + wr * 4 + t;
+    const bool live = u < units && c < cout;
+    double h0[Q], h1[Q];
+    if (live) forward_jets<DIM, ACT>(acc, b0, b1, u, c, rows, cout, aux, c + 1 < cout, h0, h1);
+    if (live) forward_store<DIM>(h0, h1, u, c, rows, cout, residual, out, activated, vec_out, c + 1 < cout);
     __syncwarp();
   }
-  turns.close(mine, count(blockIdx.x / blocks + (group + NG / 2) % NG * per));
+  turns.close(mine, count(blockIdx.x / blocks + (group + NG - 1) % NG * per));
+  cp_async_wait<0>();
+}
+
+// ---------------------------------------------------------------- forward, resident tiles
+// The same product where W's block and two whole tiles fit in shared memory (cin <= 132): two
+// groups of 8 warps, WC of them across channels (16 each) and 8 / WC across rows (40 each, as
+// four blocks of 10; a 3-D unit is two blocks).  A group waits for its whole tile before it
+// takes its turn, runs MMAs and tanh jets in one stretch, hands the turn on, and only then
+// loads its next tile and stores: between take and pass there is no barrier and no memory
+// access, and the partner's turn covers the group's.  The jets stay inside the turn because DMMA
+// and DFMA share one datapath with DMMA first: outside it they crawl behind the partner's MMAs.
+constexpr int kTileGroup = 256, kTileSmem = 227 * 1024;
+constexpr int tile_rows(int wc) { return 320 / wc; }
+__host__ __device__ constexpr int tile_ld(int cin) { return (cin + 7) / 8 * 8 + 4; }   // 4 or 12 (mod 16)
+__host__ __device__ constexpr int tile_ldw(int cin) { return (cin + 7) / 8 * 8 + 2; }  // 2 (mod 8)
+constexpr size_t tile_smem(int wc, int cin) {
+  return sizeof(double) * (2 * size_t(tile_rows(wc)) * tile_ld(cin) + size_t(16 * wc) * tile_ldw(cin));
+}
+
+// rows r0 .. r0 + count - 1 (< total) and columns 0 .. cin8 - 1 (zeros past cin) of src into
+// dst [count][ld]: one row a warp
+__device__ __forceinline__ void load_rows(double* dst, int ld, const double* __restrict__ src, int64_t r0, int count,
+                                          int64_t total, int cin, bool vec, int warp, int warps, int lane) {
+  const int cin8 = (cin + 7) / 8 * 8;
+  const double* row = src + (r0 + warp) * cin;
+  double* to = dst + warp * ld;
+  const int64_t step = opaque(int64_t(warps) * cin);
+  for (int r = warp; r < count; r += warps, row += step, to += warps * ld) {
+    const bool live = r0 + r < total;
+    if (vec) {
+      for (int k = 2 * lane; k < cin8; k += 64) cp_async16(to + k, live && k < cin ? row + k : src, live && k < cin);
+    } else {
+      for (int k = lane; k < cin8; k += 32) cp_async8(to + k, live && k < cin ? row + k : src, live && k < cin);
+    }
+  }
+}
+
+template <int DIM, bool ACT, int WC>
+__global__ void __launch_bounds__(2 * kTileGroup, 1)
+    affine_forward_tile(const double* __restrict__ hidden, const double* __restrict__ weight,
+                        const double* __restrict__ bias, const double* __restrict__ residual, double* __restrict__ out,
+                        double* __restrict__ activated, double* __restrict__ aux, Packed rows, int cin, int cout,
+                        bool vec_in, bool vec_out) {
+  constexpr int Q = Jet<DIM>::Q, NT = 5, RT = tile_rows(WC), CB = 16 * WC, UB = Q / 10;  // blocks of 10 rows a unit
+  extern __shared__ __align__(16) double smem[];
+  const int tid = threadIdx.x, group = tid / kTileGroup, gt = tid % kTileGroup, warp = gt >> 5, wc = warp % WC, wr = warp / WC;
+  const int lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int blocks = (cout + CB - 1) / CB, c0 = blockIdx.x % blocks * CB;
+  const int64_t per = gridDim.x / blocks, total = rows.full * Q + rows.value;
+  const int64_t tiles = (total + RT - 1) / RT, first = blockIdx.x / blocks + group * per;
+  const auto count = [&](int64_t from) { return from < tiles ? (tiles - 1 - from) / (2 * per) + 1 : 0; };
+  const int ld = tile_ld(cin), ldw = tile_ldw(cin), ks = (cin + 7) / 8;
+  double *tile_at = smem + group * RT * ld, *sw = smem + 2 * RT * ld;
+
+  load_rows(sw, ldw, weight, c0, CB, cout, cin, vec_in, tid >> 5, 16, lane);
+  if (first < tiles) load_rows(tile_at, ld, hidden, first * RT, RT, total, cin, vec_in, warp, 8, lane);
+  cp_async_commit();
+  cp_async_wait<0>();
+  __syncthreads();
+
+  const int ch = wc * 16 + 2 * g, c = c0 + ch;  // this thread's channels c, c + 1
+  const double b0 = c < cout ? bias[c] : 0.0, b1 = c + 1 < cout ? bias[c + 1] : 0.0;
+  const double* ap = sw + ch * ldw + t;
+  const double* bp = tile_at + (wr * 40 + (g >> 1) * 10 + (g & 1)) * ld + t;
+  const Turns<2, kTileGroup> turns(group);
+  for (int64_t tile = first; tile < tiles; tile += 2 * per) {
+    double acc[NT][4];
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[j][e] = 0.0;
+    if (residual) {  // towards L2, for this tile's stores
+      const int width = cout - c0 < CB ? cout - c0 : CB;
+      for (int e = gt; e < RT * WC; e += kTileGroup) {
+        const int64_t r = tile * RT + e / WC;
+        if (r < total && e % WC * 16 < width) prefetch_line(residual + r * cout + c0 + e % WC * 16);
+      }
+    }
+    cp_async_wait<0>();
+    named_sync(1 + group, kTileGroup);
+    turns.take();
+#pragma unroll 4
+    for (int k = 0; k < ks; ++k) {
+      const double a[4] = {ap[8 * k], ap[8 * k + ldw], ap[8 * k + 4], ap[8 * k + ldw + 4]};
+#pragma unroll
+      for (int j = 0; j < NT; ++j) mma_m16n8k8(acc[j], a, bp[2 * j * ld + 8 * k], bp[2 * j * ld + 8 * k + 4]);
+    }
+    const int64_t u = (tile * RT + wr * 40 + t * 10) / Q;
+    const bool live = u * Q < total && c < cout;
+    if constexpr (DIM == 2) {
+      double h0[Q], h1[Q];
+      if (live) forward_jets<DIM, ACT>(acc, b0, b1, u, c, rows, cout, aux, c + 1 < cout, h0, h1);
+      __syncwarp();
+      turns.pass();
+      named_sync(1 + group, kTileGroup);  // every warp has read the tile
+      if (tile + 2 * per < tiles)
+        load_rows(tile_at, ld, hidden, (tile + 2 * per) * RT, RT, total, cin, vec_in, warp, 8, lane);
+      cp_async_commit();
+      if (live) forward_store<DIM>(h0, h1, u, c, rows, cout, residual, out, activated, vec_out, c + 1 < cout);
+    }
+    __syncwarp();
+  }
+  turns.close(count(first), count(blockIdx.x / blocks + (1 - group) * per));
   cp_async_wait<0>();
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-template <int DIM, bool ACT, int NG, int NS, bool STREAM>
+template <int DIM, bool ACT, int NG, int GW, int NS, bool STREAM>
 cudaError_t launch_forward(const double* hidden, const double* weight, const double* bias, const double* residual,
                            double* out, double* activated, double* aux, Packed rows, int cin, int cout,
                            cudaStream_t stream) {
-  const auto kernel = affine_forward<DIM, ACT, NG, NS, STREAM>;
-  const size_t smem = fw_smem<DIM, NG, NS, STREAM>(cin);
+  const auto kernel = affine_forward<DIM, ACT, NG, GW, NS, STREAM>;
+  const size_t smem = fw_smem<DIM, NG, GW, NS, STREAM>(cin);
   int sms = 0;
   cudaError_t e = sm_count(&sms);
   // a per-device attribute: set on every call, so that each device gets it
   if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
   if (e != cudaSuccess) return e;
   const int64_t blocks = (int64_t(cout) + kFwCB - 1) / kFwCB;
-  const int64_t tiles = (rows.units<Jet<DIM>::Q>() + kFwUnits - 1) / kFwUnits;
+  const int64_t tiles = (rows.units<Jet<DIM>::Q>() + GW - 1) / GW;
   const int64_t most = sms / blocks > 0 ? sms / blocks : 1, per = tiles < most ? tiles : most;
   const bool vec_in = cin % 2 == 0 && aligned16(hidden) && aligned16(weight);
   const bool vec_out = cout % 2 == 0 && aligned16(out) && aligned16(residual) && aligned16(activated);
-  kernel<<<unsigned(per * blocks), NG * kFwGroup, smem, stream>>>(hidden, weight, bias, residual, out, activated, aux,
+  kernel<<<unsigned(per * blocks), NG * GW * 32, smem, stream>>>(hidden, weight, bias, residual, out, activated, aux,
                                                                  rows, cin, cout, vec_in, vec_out);
+  return cudaGetLastError();
+}
+
+template <int DIM, bool ACT, int WC>
+cudaError_t launch_forward_tile(const double* hidden, const double* weight, const double* bias, const double* residual,
+                                double* out, double* activated, double* aux, Packed rows, int cin, int cout,
+                                cudaStream_t stream) {
+  const auto kernel = affine_forward_tile<DIM, ACT, WC>;
+  const size_t smem = tile_smem(WC, cin);
+  int sms = 0;
+  cudaError_t e = sm_count(&sms);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+  if (e != cudaSuccess) return e;
+  const int64_t blocks = (int64_t(cout) + 16 * WC - 1) / (16 * WC), total = rows.full * Jet<DIM>::Q + rows.value;
+  const int64_t tiles = (total + tile_rows(WC) - 1) / tile_rows(WC);
+  const int64_t most = sms / blocks > 0 ? sms / blocks : 1, per = tiles < most ? tiles : most;
+  const bool vec_in = cin % 2 == 0 && aligned16(hidden) && aligned16(weight);
+  const bool vec_out = cout % 2 == 0 && aligned16(out) && aligned16(residual) && aligned16(activated);
+  kernel<<<unsigned(per * blocks), 2 * kTileGroup, smem, stream>>>(hidden, weight, bias, residual, out, activated, aux,
+                                                                  rows, cin, cout, vec_in, vec_out);
   return cudaGetLastError();
 }
 
 // W's block beside as many groups and stages as 227 KB hold
 template <int DIM, bool ACT, typename... Args>
-cudaError_t forward(int cin, Args... args) {
+cudaError_t forward(int cin, int cout, Args... args) {
   if constexpr (DIM == 2) {
-    if (cin <= 160) return launch_forward<2, ACT, 4, 3, false>(args...);
-    if (cin <= 256) return launch_forward<2, ACT, 4, 2, false>(args...);
-    return launch_forward<2, ACT, 4, 2, true>(args...);
+    if (cout <= 64 && tile_smem(4, cin) <= kTileSmem) return launch_forward_tile<2, ACT, 4>(args...);
+    if (tile_smem(8, cin) <= kTileSmem) return launch_forward_tile<2, ACT, 8>(args...);
+    if (cin <= 160) return launch_forward<2, ACT, 4, 4, 3, false>(args...);
+    if (cin <= 256) return launch_forward<2, ACT, 4, 4, 2, false>(args...);
+    return launch_forward<2, ACT, 4, 4, 2, true>(args...);
   } else {
-    if (cin <= 160) return launch_forward<3, ACT, 3, 2, false>(args...);
-    if (cin <= 256) return launch_forward<3, ACT, 2, 2, false>(args...);
-    return launch_forward<3, ACT, 2, 2, true>(args...);
+    if (cin <= 160) return launch_forward<3, ACT, 3, 4, 2, false>(args...);
+    if (cin <= 256) return launch_forward<3, ACT, 2, 4, 2, false>(args...);
+    return launch_forward<3, ACT, 2, 4, 2, true>(args...);
   }
 }
 
@@ -428,7 +564,7 @@ int flashns_b200_affine(int dim, int activation, const double* hidden, const dou
       ranges_overlap(activated, bytes, hidden, in) || ranges_overlap(activated, bytes, residual, bytes) ||
       ranges_overlap(out, bytes, activated, bytes))
     return int(cudaErrorInvalidValue);
-  const auto run = [&](auto launch) { return int(launch(cin, hidden, weight, bias, residual, out, activated, aux, rows, cin, cout, stream)); };
+  const auto run = [&](auto launch) { return int(launch(cin, cout, hidden, weight, bias, residual, out, activated, aux, rows, cin, cout, stream)); };
   if (dim == 2) return activation ? run([](auto... a) { return forward<2, true>(a...); }) : run([](auto... a) { return forward<2, false>(a...); });
   return activation ? run([](auto... a) { return forward<3, true>(a...); }) : run([](auto... a) { return forward<3, false>(a...); });
 }
