@@ -9,6 +9,16 @@
 #include "layers.cuh"
 
 namespace flashns_b200 {
+// set by a kernel whose bounded wait on a copy gave up (read with eval.cu's word)
+__device__ int g_affine_fault = 0;
+cudaError_t affine_fault(int* fault, bool clear) {
+  cudaError_t e = cudaMemcpyFromSymbol(fault, g_affine_fault, sizeof(int));
+  if (e == cudaSuccess && clear) {
+    const int zero = 0;
+    e = cudaMemcpyToSymbol(g_affine_fault, &zero, sizeof(int));
+  }
+  return e;
+}
 namespace {
 
 constexpr int kAffThreads = 256;
@@ -296,67 +306,83 @@ __global__ void __launch_bounds__(NG* GW * 32, 1)
 }
 
 // ---------------------------------------------------------------- forward, resident tiles
-// The same product where W's block and two whole tiles fit in shared memory (cin <= 132): two
+// The same product where W's block and two whole tiles fit in shared memory (cin <= 128): two
 // groups of 8 warps, WC of them across channels (16 each) and 8 / WC across rows (40 each, as
 // four blocks of 10; a 3-D unit is two blocks).  A group waits for its whole tile before it
 // takes its turn, runs MMAs and tanh jets in one stretch, hands the turn on, and only then
 // loads its next tile and stores: between take and pass there is no barrier and no memory
-// access, and the partner's turn covers the group's.  The jets stay inside the turn because DMMA
-// and DFMA share one datapath with DMMA first: outside it they crawl behind the partner's MMAs.
+// access, and the partner's turn covers the group's.  The jets stay inside the turn because
+// DMMA and DFMA share one datapath with DMMA first: outside it they crawl behind the partner's
+// MMAs (16,384 + 4,096 points, 64 -> 64 with residual: 110 us against 88).  A tile is one TMA
+// box of 36 columns for each 32 (the 4 more are the padding that frees the fragment loads of
+// bank conflicts): issued by threads, the same copies slow the partner's MMAs.
 constexpr int kTileGroup = 256, kTileSmem = 227 * 1024;
 constexpr int tile_rows(int wc) { return 320 / wc; }
-__host__ __device__ constexpr int tile_ld(int cin) { return (cin + 7) / 8 * 8 + 4; }   // 4 or 12 (mod 16)
+__host__ __device__ constexpr int tile_planes(int cin) { return (cin + kFwKC - 1) / kFwKC; }
 __host__ __device__ constexpr int tile_ldw(int cin) { return (cin + 7) / 8 * 8 + 2; }  // 2 (mod 8)
 constexpr size_t tile_smem(int wc, int cin) {
-  return sizeof(double) * (2 * size_t(tile_rows(wc)) * tile_ld(cin) + size_t(16 * wc) * tile_ldw(cin));
+  return sizeof(double) * (2 * size_t(tile_rows(wc)) * tile_planes(cin) * kFwLD + size_t(16 * wc) * tile_ldw(cin) + 2);
 }
 
-// rows r0 .. r0 + count - 1 (< total) and columns 0 .. cin8 - 1 (zeros past cin) of src into
-// dst [count][ld]: one row a warp
+// rows r0 .. r0 + count - 1 (zeros from `total` on) and columns 0 .. cin8 - 1 (zeros past cin)
+// of src into dst [count][ld]: one row a warp
 __device__ __forceinline__ void load_rows(double* dst, int ld, const double* __restrict__ src, int64_t r0, int count,
                                           int64_t total, int cin, bool vec, int warp, int warps, int lane) {
   const int cin8 = (cin + 7) / 8 * 8;
-  const double* row = src + (r0 + warp) * cin;
-  double* to = dst + warp * ld;
-  const int64_t step = opaque(int64_t(warps) * cin);
-  for (int r = warp; r < count; r += warps, row += step, to += warps * ld) {
+  for (int r = warp; r < count; r += warps) {
     const bool live = r0 + r < total;
+    const double* row = live ? src + (r0 + r) * cin : src;
     if (vec) {
-      for (int k = 2 * lane; k < cin8; k += 64) cp_async16(to + k, live && k < cin ? row + k : src, live && k < cin);
+      for (int k = 2 * lane; k < cin8; k += 64) cp_async16(dst + r * ld + k, k < cin ? row + k : src, live && k < cin);
     } else {
-      for (int k = lane; k < cin8; k += 32) cp_async8(to + k, live && k < cin ? row + k : src, live && k < cin);
+      for (int k = lane; k < cin8; k += 32) cp_async8(dst + r * ld + k, k < cin ? row + k : src, live && k < cin);
     }
   }
 }
 
 template <int DIM, bool ACT, int WC>
 __global__ void __launch_bounds__(2 * kTileGroup, 1)
-    affine_forward_tile(const double* __restrict__ hidden, const double* __restrict__ weight,
+    affine_forward_tile(const __grid_constant__ CUtensorMap hidden, const double* __restrict__ weight,
                         const double* __restrict__ bias, const double* __restrict__ residual, double* __restrict__ out,
                         double* __restrict__ activated, double* __restrict__ aux, Packed rows, int cin, int cout,
-                        bool vec_in, bool vec_out) {
-  constexpr int Q = Jet<DIM>::Q, NT = 5, RT = tile_rows(WC), CB = 16 * WC, UB = Q / 10;  // blocks of 10 rows a unit
-  extern __shared__ __align__(16) double smem[];
+                        bool vec_w, bool vec_out) {
+  constexpr int Q = Jet<DIM>::Q, NT = 5, RT = tile_rows(WC), CB = 16 * WC, LD = kFwLD, PLANE = RT * LD;
+  extern __shared__ __align__(128) double smem[];
   const int tid = threadIdx.x, group = tid / kTileGroup, gt = tid % kTileGroup, warp = gt >> 5, wc = warp % WC, wr = warp / WC;
   const int lane = tid & 31, g = lane >> 2, t = lane & 3;
+  if (smem_u32(smem) & 127) {  // TMA destinations need it: refuse, never fault
+    if (tid == 0) atomicExch(&g_affine_fault, 2);
+    return;
+  }
   const int blocks = (cout + CB - 1) / CB, c0 = blockIdx.x % blocks * CB;
   const int64_t per = gridDim.x / blocks, total = rows.full * Q + rows.value;
   const int64_t tiles = (total + RT - 1) / RT, first = blockIdx.x / blocks + group * per;
   const auto count = [&](int64_t from) { return from < tiles ? (tiles - 1 - from) / (2 * per) + 1 : 0; };
-  const int ld = tile_ld(cin), ldw = tile_ldw(cin), ks = (cin + 7) / 8;
-  double *tile_at = smem + group * RT * ld, *sw = smem + 2 * RT * ld;
+  const int planes = tile_planes(cin), ldw = tile_ldw(cin), ks = (cin + 7) / 8;
+  double *tile_at = smem + group * planes * PLANE, *sw = smem + 2 * planes * PLANE;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sw + CB * ldw);
+  auto load = [&](int64_t tile) {  // by one thread, once every warp has read the last tile
+    fence_proxy_async();
+    mbar_arrive_expect_tx(bars + group, unsigned(planes * PLANE * sizeof(double)));
+    for (int k = 0; k < planes; ++k) tma_load_2d(tile_at + k * PLANE, &hidden, k * kFwKC, int(tile * RT), bars + group);
+  };
 
-  load_rows(sw, ldw, weight, c0, CB, cout, cin, vec_in, tid >> 5, 16, lane);
-  if (first < tiles) load_rows(tile_at, ld, hidden, first * RT, RT, total, cin, vec_in, warp, 8, lane);
+  load_rows(sw, ldw, weight, c0, CB, cout, cin, vec_w, tid >> 5, 16, lane);
   cp_async_commit();
+  if (tid == 0) {
+    mbar_init(bars, 1);
+    mbar_init(bars + 1, 1);
+  }
   cp_async_wait<0>();
   __syncthreads();
+  if (gt == 0 && first < tiles) load(first);
 
   const int ch = wc * 16 + 2 * g, c = c0 + ch;  // this thread's channels c, c + 1
   const double b0 = c < cout ? bias[c] : 0.0, b1 = c + 1 < cout ? bias[c + 1] : 0.0;
-  const double* ap = sw + ch * ldw + t;
-  const double* bp = tile_at + (wr * 40 + (g >> 1) * 10 + (g & 1)) * ld + t;
+  const double *ap = sw + ch * ldw + t, *bp = tile_at + (wr * 40 + (g >> 1) * 10 + (g & 1)) * LD + t;
   const Turns<2, kTileGroup> turns(group);
+  unsigned phase = 0;
+  bool dead = false;  // a copy's bounded wait gave up: the group keeps the turns and does no work
   for (int64_t tile = first; tile < tiles; tile += 2 * per) {
     double acc[NT][4];
 #pragma unroll
@@ -364,38 +390,48 @@ __global__ void __launch_bounds__(2 * kTileGroup, 1)
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[j][e] = 0.0;
     if (residual) {  // towards L2, for this tile's stores
-      const int width = cout - c0 < CB ? cout - c0 : CB;
-      for (int e = gt; e < RT * WC; e += kTileGroup) {
-        const int64_t r = tile * RT + e / WC;
-        if (r < total && e % WC * 16 < width) prefetch_line(residual + r * cout + c0 + e % WC * 16);
+      const int64_t r0 = tile * RT, left = total - r0;
+      if (vec_out && blocks == 1) {
+        if (gt == 0) prefetch_l2(residual + r0 * cout, unsigned((left < RT ? left : RT) * cout * sizeof(double)));
+      } else {
+        const int width = cout - c0 < CB ? cout - c0 : CB;
+        for (int e = gt; e < RT * WC; e += kTileGroup)
+          if (e / WC < left && e % WC * 16 < width) prefetch_line(residual + (r0 + e / WC) * cout + c0 + e % WC * 16);
       }
     }
-    cp_async_wait<0>();
-    named_sync(1 + group, kTileGroup);
+    if (!dead) {
+      dead = named_sync_or(1 + group, kTileGroup, !mbar_wait(bars + group, phase));
+      if (dead && gt == 0) atomicExch(&g_affine_fault, 1);
+    }
+    phase ^= 1;
     turns.take();
-#pragma unroll 4
-    for (int k = 0; k < ks; ++k) {
-      const double a[4] = {ap[8 * k], ap[8 * k + ldw], ap[8 * k + 4], ap[8 * k + ldw + 4]};
+    if (!dead) {
+      for (int p = 0; p < planes; ++p) {
+        const double *a_at = ap + p * kFwKC, *b_at = bp + p * PLANE;
+        const int left = ks - 4 * p;
+        if (left >= 4) {
 #pragma unroll
-      for (int j = 0; j < NT; ++j) mma_m16n8k8(acc[j], a, bp[2 * j * ld + 8 * k], bp[2 * j * ld + 8 * k + 4]);
+          for (int k = 0; k < 4; ++k) forward_step<NT>(acc, a_at + 8 * k, ldw, b_at + 8 * k);
+        } else {
+#pragma unroll 1
+          for (int k = 0; k < left; ++k) forward_step<NT>(acc, a_at + 8 * k, ldw, b_at + 8 * k);
+        }
+      }
     }
     const int64_t u = (tile * RT + wr * 40 + t * 10) / Q;
-    const bool live = u * Q < total && c < cout;
+    const bool live = !dead && u * Q < total && c < cout;
     if constexpr (DIM == 2) {
       double h0[Q], h1[Q];
       if (live) forward_jets<DIM, ACT>(acc, b0, b1, u, c, rows, cout, aux, c + 1 < cout, h0, h1);
       __syncwarp();
       turns.pass();
       named_sync(1 + group, kTileGroup);  // every warp has read the tile
-      if (tile + 2 * per < tiles)
-        load_rows(tile_at, ld, hidden, (tile + 2 * per) * RT, RT, total, cin, vec_in, warp, 8, lane);
-      cp_async_commit();
+      if (gt == 0 && tile + 2 * per < tiles && !dead) load(tile + 2 * per);
       if (live) forward_store<DIM>(h0, h1, u, c, rows, cout, residual, out, activated, vec_out, c + 1 < cout);
     }
     __syncwarp();
   }
   turns.close(count(first), count(blockIdx.x / blocks + (1 - group) * per));
-  cp_async_wait<0>();
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -427,26 +463,27 @@ cudaError_t launch_forward_tile(const double* hidden, const double* weight, cons
                                 cudaStream_t stream) {
   const auto kernel = affine_forward_tile<DIM, ACT, WC>;
   const size_t smem = tile_smem(WC, cin);
-  int sms = 0;
-  cudaError_t e = sm_count(&sms);
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
-  if (e != cudaSuccess) return e;
   const int64_t blocks = (int64_t(cout) + 16 * WC - 1) / (16 * WC), total = rows.full * Jet<DIM>::Q + rows.value;
   const int64_t tiles = (total + tile_rows(WC) - 1) / tile_rows(WC);
+  int sms = 0;
+  CUtensorMap map;
+  cudaError_t e = sm_count(&sms);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+  if (e == cudaSuccess) e = matrix_map(&map, hidden, total, cin, kFwLD, tile_rows(WC));
+  if (e != cudaSuccess) return e;
   const int64_t most = sms / blocks > 0 ? sms / blocks : 1, per = tiles < most ? tiles : most;
-  const bool vec_in = cin % 2 == 0 && aligned16(hidden) && aligned16(weight);
   const bool vec_out = cout % 2 == 0 && aligned16(out) && aligned16(residual) && aligned16(activated);
-  kernel<<<unsigned(per * blocks), 2 * kTileGroup, smem, stream>>>(hidden, weight, bias, residual, out, activated, aux,
-                                                                  rows, cin, cout, vec_in, vec_out);
+  kernel<<<unsigned(per * blocks), 2 * kTileGroup, smem, stream>>>(map, weight, bias, residual, out, activated, aux, rows,
+                                                                  cin, cout, aligned16(weight), vec_out);
   return cudaGetLastError();
 }
 
 // W's block beside as many groups and stages as 227 KB hold
 template <int DIM, bool ACT, typename... Args>
-cudaError_t forward(int cin, int cout, Args... args) {
+cudaError_t forward(int cin, int cout, bool boxes, Args... args) {
   if constexpr (DIM == 2) {
-    if (cout <= 64 && tile_smem(4, cin) <= kTileSmem) return launch_forward_tile<2, ACT, 4>(args...);
-    if (tile_smem(8, cin) <= kTileSmem) return launch_forward_tile<2, ACT, 8>(args...);
+    if (boxes && cout <= 64 && tile_smem(4, cin) <= kTileSmem) return launch_forward_tile<2, ACT, 4>(args...);
+    if (boxes && tile_smem(8, cin) <= kTileSmem) return launch_forward_tile<2, ACT, 8>(args...);
     if (cin <= 160) return launch_forward<2, ACT, 4, 4, 3, false>(args...);
     if (cin <= 256) return launch_forward<2, ACT, 4, 4, 2, false>(args...);
     return launch_forward<2, ACT, 4, 4, 2, true>(args...);
@@ -564,7 +601,9 @@ int flashns_b200_affine(int dim, int activation, const double* hidden, const dou
       ranges_overlap(activated, bytes, hidden, in) || ranges_overlap(activated, bytes, residual, bytes) ||
       ranges_overlap(out, bytes, activated, bytes))
     return int(cudaErrorInvalidValue);
-  const auto run = [&](auto launch) { return int(launch(cin, cout, hidden, weight, bias, residual, out, activated, aux, rows, cin, cout, stream)); };
+  // TMA boxes: rows on 16-byte boundaries, row numbers that fit their 32-bit coordinate
+  const bool boxes = cin % 2 == 0 && aligned16(hidden) && count < INT_MAX - 1024;
+  const auto run = [&](auto launch) { return int(launch(cin, cout, boxes, hidden, weight, bias, residual, out, activated, aux, rows, cin, cout, stream)); };
   if (dim == 2) return activation ? run([](auto... a) { return forward<2, true>(a...); }) : run([](auto... a) { return forward<2, false>(a...); });
   return activation ? run([](auto... a) { return forward<3, true>(a...); }) : run([](auto... a) { return forward<3, false>(a...); });
 }

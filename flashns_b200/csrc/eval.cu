@@ -39,6 +39,7 @@ constexpr int LDC = KC + 4;  // padded chunk row: conflict-free FP64 fragment lo
 constexpr int kMaxAffine = 16;
 // set by a kernel whose bounded wait on a bulk copy gave up (read by flashns_b200_device_fault)
 __device__ int g_device_fault = 0;
+cudaError_t affine_fault(int* fault, bool clear);  // affine.cu
 // the dense dgrad (+ VJP) of a 64 -> 64 layer on the evaluation's backward kernels (defined
 // with the host launchers below; called by the reference-ABI hook in hooks.cu)
 cudaError_t dense_dgrad_64(int dim, bool fused, const double* d, const double* w, const double* h,
@@ -3899,6 +3900,9 @@ int flashns_b200_device_fault(int* fault, int clear) {
     const int zero = 0;
     e = cudaMemcpyToSymbol(g_device_fault, &zero, sizeof(int));
   }
+  int layers = 0;  // the layer kernels' word
+  if (e == cudaSuccess) e = affine_fault(&layers, clear != 0);
+  if (e == cudaSuccess && !*fault) *fault = layers;
   return int(e);
 }
 

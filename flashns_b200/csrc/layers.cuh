@@ -1,9 +1,12 @@
 // What the layer operators (norm.cu, affine.cu) share: packed units, jet products by
 // dimension, fixed-order sums over lanes, argument checks.
 #pragma once
+#include <cuda.h>
+
 #include <climits>
 #include <cstddef>
 #include <cstdint>
+#include <mutex>
 
 #include "common.cuh"
 #include "products_generated.cuh"
@@ -110,6 +113,31 @@ inline cudaError_t sm_count(int* sms) {
   int device = 0;
   const cudaError_t e = cudaGetDevice(&device);
   return e != cudaSuccess ? e : cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, device);
+}
+
+// Tensor map of [rows][cols] row-major FP64 read or written in boxes of box_rows x box_cols;
+// what a box holds past the matrix reads as zeros and is not written.  base and the rows on
+// 16-byte boundaries.
+inline cudaError_t matrix_map(CUtensorMap* map, const double* base, int64_t rows, int cols, int box_cols, int box_rows) {
+  using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static Encode encode = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {  // through the runtime, without a link against the driver library
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q{};
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      encode = reinterpret_cast<Encode>(p);
+  });
+  if (!encode) return cudaErrorNotSupported;
+  const cuuint64_t dims[2] = {cuuint64_t(cols), cuuint64_t(rows)}, pitch[1] = {cuuint64_t(cols) * sizeof(double)};
+  const cuuint32_t box[2] = {cuuint32_t(box_cols), cuuint32_t(box_rows)}, step[2] = {1, 1};
+  const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT64, 2, const_cast<double*>(base), dims, pitch, box, step,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
 // Launch that may start while the stream's previous kernel drains; the kernel waits
