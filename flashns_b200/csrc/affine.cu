@@ -4,6 +4,8 @@
 //   Z = H W^T, + b on order-0 rows;  A = tanh jet(Z), a1 = sech^2 Z_0;  Y = A (+ R)
 // (without the activation Y = Z (+ R)).  Adjoint at G, which is also R's gradient:
 //   dZ = VJP of the tanh jet at (A, a1), G;  dH = dZ W;  dW = dZ^T H;  db = sum of order-0 dZ.
+#include <algorithm>
+
 #include "flashns_b200.h"
 #include "jets_generated.cuh"
 #include "layers.cuh"
@@ -66,10 +68,18 @@ __device__ __forceinline__ void cp_async8(void* smem, const void* gmem, bool val
   asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;\n" ::"r"(smem_u32(smem)), "l"(gmem), "r"(valid ? 8 : 0));
 }
 
-// W rows c0 .. c0 + 63, columns k0 .. k0 + width - 1 into dst [64][ld], zero past the ends
+// Weights of output channels c0 .. c0 + 63 and input channels k0 .. k0 + width - 1 into dst
+// [64][ld], zero past the ends: w is [cout][cin], or with `across` [cin][cout] (the adjoint's
+// product with W instead of its transpose).
 __device__ __forceinline__ void load_weight(double* dst, int ld, const double* __restrict__ w, int c0, int k0, int width,
-                                            int cin, int cout, bool vec, int tid, int threads) {
-  if (vec) {
+                                            int cin, int cout, bool vec, bool across, int tid, int threads) {
+  if (across) {
+    for (int e = tid; e < kFwCB * width; e += threads) {
+      const int r = e % kFwCB, k = k0 + e / kFwCB;
+      const bool ok = c0 + r < cout && k < cin;
+      cp_async8(dst + r * ld + k - k0, ok ? w + int64_t(k) * cout + c0 + r : w, ok);
+    }
+  } else if (vec) {
     const int half = width / 2;
     for (int e = tid; e < kFwCB * half; e += threads) {
       const int r = e / half, k = k0 + 2 * (e % half);
@@ -199,7 +209,7 @@ template <int DIM, bool ACT, int NG, int GW, int NS, bool STREAM>
 __global__ void __launch_bounds__(NG* GW * 32, 1)
     affine_forward(const double* __restrict__ hidden, const double* __restrict__ weight, const double* __restrict__ bias,
                    const double* __restrict__ residual, double* __restrict__ out, double* __restrict__ activated,
-                   double* __restrict__ aux, Packed rows, int cin, int cout, bool vec_in, bool vec_out) {
+                   double* __restrict__ aux, Packed rows, int cin, int cout, bool vec_in, bool vec_out, bool across) {
   constexpr int Q = Jet<DIM>::Q, NT = Q / 2, US = fw_unit_stride<DIM>(), KC = kFwKC;
   constexpr int GT = 32 * GW, UT = GW, RT = UT * Q;  // a group's threads; units and rows of its tile
   extern __shared__ __align__(16) double smem[];
@@ -238,7 +248,7 @@ __global__ void __launch_bounds__(NG* GW * 32, 1)
       }
     }
     if constexpr (STREAM)
-      load_weight(sw + stage * kFwCB * ldw, ldw, weight, c0, k0, KC, cin, cout, vec_in, gt, GT);
+      load_weight(sw + stage * kFwCB * ldw, ldw, weight, c0, k0, KC, cin, cout, vec_in, across, gt, GT);
   };
   // the next chunk to load: its tile, K chunk and stage
   int64_t load_tile = first;
@@ -251,7 +261,7 @@ __global__ void __launch_bounds__(NG* GW * 32, 1)
     if (++load_kc == nk) load_kc = 0, load_tile += tile_step;
   };
 
-  if constexpr (!STREAM) load_weight(sw, ldw, weight, c0, 0, nk * KC, cin, cout, vec_in, tid, NG * GT);
+  if constexpr (!STREAM) load_weight(sw, ldw, weight, c0, 0, nk * KC, cin, cout, vec_in, across, tid, NG * GT);
   cp_async_commit();
 #pragma unroll
   for (int s = 0; s < NS - 1; ++s) load();
@@ -259,7 +269,7 @@ __global__ void __launch_bounds__(NG* GW * 32, 1)
   __syncthreads();  // W is there for every group
 
   const int ch = wc * 16 + 2 * g, c = c0 + ch;  // this thread's channels c, c + 1
-  const double b0 = c < cout ? bias[c] : 0.0, b1 = c + 1 < cout ? bias[c + 1] : 0.0;
+  const double b0 = bias && c < cout ? bias[c] : 0.0, b1 = bias && c + 1 < cout ? bias[c + 1] : 0.0;
   double acc[NT][4];
   const Turns<NG, GT> turns(group);
   int stage = 0;
@@ -378,7 +388,7 @@ __global__ void __launch_bounds__(2 * kTileGroup, 1)
   if (gt == 0 && first < tiles) load(first);
 
   const int ch = wc * 16 + 2 * g, c = c0 + ch;  // this thread's channels c, c + 1
-  const double b0 = c < cout ? bias[c] : 0.0, b1 = c + 1 < cout ? bias[c + 1] : 0.0;
+  const double b0 = bias && c < cout ? bias[c] : 0.0, b1 = bias && c + 1 < cout ? bias[c + 1] : 0.0;
   const double *ap = sw + ch * ldw + t, *bp = tile_at + (wr * 40 + (g >> 1) * 10 + (g & 1)) * LD + t;
   const Turns<2, kTileGroup> turns(group);
   unsigned phase = 0;
@@ -439,7 +449,7 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 template <int DIM, bool ACT, int NG, int GW, int NS, bool STREAM>
 cudaError_t launch_forward(const double* hidden, const double* weight, const double* bias, const double* residual,
                            double* out, double* activated, double* aux, Packed rows, int cin, int cout,
-                           cudaStream_t stream) {
+                           bool across, cudaStream_t stream) {
   const auto kernel = affine_forward<DIM, ACT, NG, GW, NS, STREAM>;
   const size_t smem = fw_smem<DIM, NG, GW, NS, STREAM>(cin);
   int sms = 0;
@@ -453,14 +463,14 @@ cudaError_t launch_forward(const double* hidden, const double* weight, const dou
   const bool vec_in = cin % 2 == 0 && aligned16(hidden) && aligned16(weight);
   const bool vec_out = cout % 2 == 0 && aligned16(out) && aligned16(residual) && aligned16(activated);
   kernel<<<unsigned(per * blocks), NG * GW * 32, smem, stream>>>(hidden, weight, bias, residual, out, activated, aux,
-                                                                 rows, cin, cout, vec_in, vec_out);
+                                                                 rows, cin, cout, vec_in, vec_out, across);
   return cudaGetLastError();
 }
 
 template <int DIM, bool ACT, int WC>
 cudaError_t launch_forward_tile(const double* hidden, const double* weight, const double* bias, const double* residual,
                                 double* out, double* activated, double* aux, Packed rows, int cin, int cout,
-                                cudaStream_t stream) {
+                                bool, cudaStream_t stream) {
   const auto kernel = affine_forward_tile<DIM, ACT, WC>;
   const size_t smem = tile_smem(WC, cin);
   const int64_t blocks = (int64_t(cout) + 16 * WC - 1) / (16 * WC), total = rows.full * Jet<DIM>::Q + rows.value;
@@ -494,7 +504,8 @@ cudaError_t forward(int cin, int cout, bool boxes, Args... args) {
   }
 }
 
-// dZ, one thread per (unit, output channel)
+// ---------------------------------------------------------------- adjoint
+// dZ, one thread per (unit, output channel): widths that the tiles below do not hold
 template <int DIM>
 __global__ void __launch_bounds__(kAffThreads)
     affine_seed(const double* __restrict__ activated, const double* __restrict__ aux, const double* __restrict__ seed,
@@ -522,51 +533,388 @@ __global__ void __launch_bounds__(kAffThreads)
   }
 }
 
-// dH = dZ W, one thread per element
-__global__ void __launch_bounds__(kAffThreads)
-    affine_dgrad(const double* __restrict__ dz, const double* __restrict__ weight, double* __restrict__ dh, int64_t rows,
-                 int cin, int cout) {
-  const int64_t total = rows * cin;
-  for (int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += int64_t(gridDim.x) * blockDim.x) {
-    const int64_t r = i / cin;
-    const int k = int(i % cin);
-    double s = 0.0;
-    for (int c = 0; c < cout; ++c) s += dz[r * cout + c] * weight[int64_t(c) * cin + k];
-    dh[i] = s;
+// dZ = VJP(A, a1; G) and dH = dZ W in one pass; FUSED (both widths <= 64): dW += dZ^T H too.
+//
+// Two groups of 8 warps, tiles of 320 / WC rows and 16 WC input channels, W resident.  Outside
+// its turn a group forms its next tile's dZ (a thread takes a unit's whole jet of one output
+// channel from global memory) in shared memory, where both products read it; inside it runs
+// only MMAs: dH^T = W^T dZ^T, with a thread's two input channels side by side (the pair of a
+// row of W is one 16-byte load, and dH leaves as 16-byte pairs), then dW = dZ^T H, whose
+// accumulators stay in registers over all of the CTA's tiles.  The partner's turn (11,000 or
+// 21,000 cycles) covers the loads, the VJP and the stores.  Unfused, dZ goes to global memory
+// for affine_wgrad_tile.
+constexpr size_t back_smem(int wc, bool fused, int cin, int cout) {
+  return sizeof(double) * (2 * size_t(tile_rows(wc)) * kFwLD * (tile_planes(cout) + (fused ? tile_planes(cin) : 0)) +
+                           size_t((cout + 7) / 8 * 8) * (16 * wc + 4) + 2);
+}
+
+template <int DIM, bool ACT, int WC, bool FUSED>
+__global__ void __launch_bounds__(2 * kTileGroup, 1)
+    affine_backward_tile(const __grid_constant__ CUtensorMap hidden_map, const double* __restrict__ hidden,
+                         const double* __restrict__ weight, const double* __restrict__ activated,
+                         const double* __restrict__ aux, const double* __restrict__ seed, double* __restrict__ dz,
+                         double* __restrict__ dh, double* __restrict__ partials, Packed rows, int cin, int cout,
+                         bool boxes, bool vec_out) {
+  constexpr int Q = Jet<DIM>::Q, RT = tile_rows(WC), CB = 16 * WC, LD = kFwLD, PLANE = RT * LD, LDW = CB + 4;
+  constexpr int NT = RT * WC / 64, UT = RT / Q, PAIRS = UT * CB / kTileGroup;  // n8 tiles a warp; jets a thread
+  static_assert(NT == 5 && PAIRS * kTileGroup == UT * CB && RT % 8 == 0, "");
+  extern __shared__ __align__(128) double smem[];
+  const int tid = threadIdx.x, group = tid / kTileGroup, gt = tid % kTileGroup, warp = gt >> 5, wc = warp % WC, wr = warp / WC;
+  const int lane = tid & 31, g = lane >> 2, t = lane & 3;
+  if (smem_u32(smem) & 127) {
+    if (tid == 0) atomicExch(&g_affine_fault, 2);
+    return;
+  }
+  const int blocks = (cin + CB - 1) / CB, i0 = blockIdx.x % blocks * CB;
+  const int64_t per = gridDim.x / blocks, total = rows.full * Q + rows.value, units = rows.units<Q>();
+  const int64_t tiles = (total + RT - 1) / RT, first = blockIdx.x / blocks + group * per;
+  const auto count = [&](int64_t from) { return from < tiles ? (tiles - 1 - from) / (2 * per) + 1 : 0; };
+  const int pz = tile_planes(cout), ph = FUSED ? tile_planes(cin) : 0, c8 = (cout + 7) / 8 * 8;
+  double *z_at = smem + group * (pz + ph) * PLANE, *h_at = z_at + pz * PLANE, *sw = smem + 2 * (pz + ph) * PLANE;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sw + c8 * LDW);
+
+  // the tile's H, once every warp has read the last one: one thread, or all where boxes cannot
+  auto load_hidden = [&](int64_t tile) {
+    if (boxes) {
+      if (gt == 0) {
+        fence_proxy_async();
+        mbar_arrive_expect_tx(bars + group, unsigned(ph * PLANE * sizeof(double)));
+        for (int p = 0; p < ph; ++p) tma_load_2d(h_at + p * PLANE, &hidden_map, p * kFwKC, int(tile * RT), bars + group);
+      }
+    } else {
+      for (int e = gt; e < RT * ph * kFwKC; e += kTileGroup) {
+        const int r = e / (ph * kFwKC), k = e % (ph * kFwKC);
+        const bool ok = tile * RT + r < total && k < cin;
+        cp_async8(h_at + k / kFwKC * PLANE + r * LD + k % kFwKC, ok ? hidden + (tile * RT + r) * cin + k : hidden, ok);
+      }
+      cp_async_commit();
+    }
+  };
+  // this thread's jets of a tile's dZ, channel cz
+  const int cz = gt % CB;
+  double db = 0.0;
+  auto form_dz = [&](int64_t tile) {
+    if (cz >= c8) return;
+#pragma unroll
+    for (int i = 0; i < PAIRS; ++i) {
+      const int ul = gt / CB + i * (kTileGroup / CB);
+      const int64_t u = tile * UT + ul;
+      double z[Q];
+#pragma unroll
+      for (int s = 0; s < Q; ++s) z[s] = 0.0;
+      if (u < units && cz < cout) {
+        const int n = rows.count<Q>(u);
+        const int64_t at = rows.row<Q>(u) * cout + cz, step = opaque(cout);
+        const double* from = seed + at;
+        if (u < rows.full) {
+          double gz[Q];
+#pragma unroll
+          for (int s = 0; s < Q; ++s, from += step) gz[s] = *from;
+          if constexpr (ACT) {
+            double h[Q];
+            const double* act = activated + at;
+#pragma unroll
+            for (int s = 0; s < Q; ++s, act += step) h[s] = *act;
+            tanh_vjp<DIM>(h, aux[u * cout + cz], gz, z);
+          } else {
+#pragma unroll
+            for (int s = 0; s < Q; ++s) z[s] = gz[s];
+          }
+          if constexpr (FUSED) db += z[0];
+        } else {
+          const double* a1 = ACT ? aux + (rows.full + (u - rows.full) * Q) * cout + cz : nullptr;
+#pragma unroll
+          for (int s = 0; s < Q; ++s)
+            if (s < n) {
+              z[s] = from[s * step];
+              if constexpr (ACT) z[s] *= a1[s * step];
+              if constexpr (FUSED) db += z[s];
+            }
+        }
+        if (!FUSED && dz && i0 == 0) {
+          double* to = dz + at;
+#pragma unroll
+          for (int s = 0; s < Q; ++s, to += step)
+            if (s < n) *to = z[s];
+        }
+      }
+      double* to = z_at + cz / kFwKC * PLANE + ul * Q * LD + cz % kFwKC;
+#pragma unroll
+      for (int s = 0; s < Q; ++s) to[s * LD] = z[s];
+    }
+  };
+
+  for (int e = tid; e < c8 * CB; e += 2 * kTileGroup) {  // W rows c, columns i0 .. i0 + CB - 1
+    const int c = e / CB, i = e % CB;
+    const bool ok = c < cout && i0 + i < cin;
+    cp_async8(sw + c * LDW + i, ok ? weight + int64_t(c) * cin + i0 + i : weight, ok);
+  }
+  cp_async_commit();
+  if (tid == 0) {
+    mbar_init(bars, 1);
+    mbar_init(bars + 1, 1);
+  }
+  cp_async_wait<0>();
+  __syncthreads();
+  if (first < tiles) {
+    if (FUSED) load_hidden(first);
+    form_dz(first);
+  }
+
+  const int ci = i0 + wc * 16 + 2 * g;  // this thread's input channels ci, ci + 1
+  const double* ap = sw + t * LDW + wc * 16 + 2 * g;
+  const double* bp = z_at + (wr * 40 + g) * LD + t;
+  // dW: output channels 16 (warp % 4) .., input channels 32 (warp / 4) ..
+  constexpr int WN = FUSED ? 4 : 1;
+  double wacc[WN][4];
+#pragma unroll
+  for (int j = 0; j < WN; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) wacc[j][e] = 0.0;
+  const int wz = warp % 4 * 16, wh = warp / 4;
+  const bool has_w = FUSED && wz < cout && wh < ph, has_h = i0 + wc * 16 < cin;
+  const double* wa = z_at + wz / kFwKC * PLANE + t * LD + wz % kFwKC + g;
+  const double* wb = h_at + wh * PLANE + t * LD + g;
+  const Turns<2, kTileGroup> turns(group);
+  unsigned phase = 0;
+  bool dead = false;  // a copy's bounded wait gave up: the group keeps the turns and does no work
+  for (int64_t tile = first; tile < tiles; tile += 2 * per) {
+    double acc[NT][4];
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[j][e] = 0.0;
+    if (FUSED && boxes) {
+      if (!dead) {
+        dead = named_sync_or(1 + group, kTileGroup, !mbar_wait(bars + group, phase));
+        if (dead && gt == 0) atomicExch(&g_affine_fault, 1);
+      }
+      phase ^= 1;
+    } else {
+      if (FUSED) cp_async_wait<0>();
+      named_sync(1 + group, kTileGroup);
+    }
+    turns.take();
+    if (!dead && has_h) {
+      for (int p = 0; p < pz; ++p) {
+        const double *a_at = ap + p * kFwKC * LDW, *b_at = bp + p * PLANE;
+        const int left = c8 / 8 - 4 * p;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (k >= left) break;
+          const double2 lo = *reinterpret_cast<const double2*>(a_at + 8 * k * LDW);
+          const double2 hi = *reinterpret_cast<const double2*>(a_at + (8 * k + 4) * LDW);
+          const double a[4] = {lo.x, lo.y, hi.x, hi.y};
+#pragma unroll
+          for (int j = 0; j < NT; ++j) mma_m16n8k8(acc[j], a, b_at[8 * j * LD + 8 * k], b_at[8 * j * LD + 8 * k + 4]);
+        }
+      }
+    }
+    if (!dead && has_w) {
+#pragma unroll
+      for (int r = 0; r < RT; r += 8) {
+        const double a[4] = {wa[r * LD], wa[r * LD + 8], wa[(r + 4) * LD], wa[(r + 4) * LD + 8]};
+#pragma unroll
+        for (int j = 0; j < WN; ++j) mma_m16n8k8(wacc[j], a, wb[r * LD + 8 * j], wb[(r + 4) * LD + 8 * j]);
+      }
+    }
+    turns.pass();
+    named_sync(1 + group, kTileGroup);  // every warp has read dZ and H
+    const int64_t next = tile + 2 * per;
+    if (FUSED && next < tiles && !dead) load_hidden(next);
+    if (!dead && ci < cin) {
+      const bool two = ci + 1 < cin;
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int64_t r = tile * RT + wr * 40 + 8 * j + 2 * t + e;
+          if (r >= total) continue;
+          double* to = dh + r * cin + ci;
+          if (vec_out) {
+            *reinterpret_cast<double2*>(to) = make_double2(acc[j][e], acc[j][2 + e]);
+          } else {
+            to[0] = acc[j][e];
+            if (two) to[1] = acc[j][2 + e];
+          }
+        }
+    }
+    if (next < tiles) form_dz(next);
+  }
+  turns.close(count(first), count(blockIdx.x / blocks + (1 - group) * per));
+  if constexpr (FUSED) {  // both groups' shares in order: this CTA's [cout][cin] and [cout]
+    cp_async_wait<0>();
+    __syncthreads();
+    double *sums = smem, *bias_sums = smem + CB * CB;
+    if (group == 1) {
+#pragma unroll
+      for (int j = 0; j < WN; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          sums[(wz + g + 8 * (e >> 1)) * CB + wh * 32 + 8 * j + 2 * t + (e & 1)] = wacc[j][e];
+    }
+    bias_sums[tid] = db;
+    __syncthreads();
+    double* mine = partials + int64_t(blockIdx.x) * cout * (int64_t(cin) + 1);
+    if (group == 0) {
+#pragma unroll
+      for (int j = 0; j < WN; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int c = wz + g + 8 * (e >> 1), i = wh * 32 + 8 * j + 2 * t + (e & 1);
+          if (c < cout && i < cin) mine[int64_t(c) * cin + i] = wacc[j][e] + sums[c * CB + i];
+        }
+    }
+    if (tid < cout) {
+      double s = 0.0;
+      for (int k = tid; k < 2 * kTileGroup; k += CB) s += bias_sums[k];
+      mine[int64_t(cout) * cin + tid] = s;
+    }
   }
 }
 
-constexpr int kWgTile = 16, kWgParts = 64;
-
-// partials[part][cout][cin + 1]: dW and, in the last column, db of the part's rows
-__global__ void __launch_bounds__(kWgTile* kWgTile)
-    affine_wgrad(const double* __restrict__ dz, const double* __restrict__ hidden, double* __restrict__ partials,
-                 int64_t rows, int64_t full_rows, int q, int cin, int cout) {
-  const int c = blockIdx.y * kWgTile + threadIdx.x / kWgTile, k = blockIdx.x * kWgTile + threadIdx.x % kWgTile;
-  if (c >= cout || k > cin) return;
-  const int64_t per = (rows + gridDim.z - 1) / gridDim.z, first = per * blockIdx.z;
-  const int64_t last = first + per < rows ? first + per : rows;
-  double s = 0.0;
-  if (k < cin) {
-    for (int64_t r = first; r < last; ++r) s += dz[r * cout + c] * hidden[r * cin + k];
-  } else {
-    for (int64_t r = first; r < last; ++r)
-      if (r >= full_rows || r % q == 0) s += dz[r * cout + c];
-  }
-  partials[(int64_t(blockIdx.z) * cout + c) * (cin + 1) + k] = s;
+// dW = dZ^T H and db: a CTA's block of 16 MT (16 / WI) output x 32 WI input channels over its
+// share of the rows, accumulators in registers throughout; 32-row stages of both operands by
+// TMA boxes (or cp.async), two ahead of the MMAs.  partials [share][cout * cin + cout].
+constexpr int kWgRows = 32, kWgStages = 3, kWgThreads = 512;
+constexpr int wg_cout(int mt, int wi) { return 16 * mt * (16 / wi); }
+constexpr size_t wg_smem(int mt, int wi) {
+  return sizeof(double) * (size_t(kWgStages) * kWgRows * kFwLD * (wg_cout(mt, wi) / kFwKC + wi) + kWgStages);
 }
 
-__global__ void __launch_bounds__(kAffThreads)
+template <int MT, int WI>
+__global__ void __launch_bounds__(kWgThreads, 1)
+    affine_wgrad_tile(const __grid_constant__ CUtensorMap dz_map, const __grid_constant__ CUtensorMap hidden_map,
+                      const double* __restrict__ dz, const double* __restrict__ hidden, double* __restrict__ partials,
+                      int64_t total, int64_t full_rows, int q, int cin, int cout, bool boxes) {
+  constexpr int CZ = wg_cout(MT, WI), CI = 32 * WI, PZ = CZ / kFwKC, P = PZ + WI, LD = kFwLD, PLANE = kWgRows * LD;
+  extern __shared__ __align__(128) double smem[];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  if (smem_u32(smem) & 127) {
+    if (tid == 0) atomicExch(&g_affine_fault, 2);
+    return;
+  }
+  const int bi = (cin + CI - 1) / CI, blocks = bi * ((cout + CZ - 1) / CZ), block = blockIdx.x % blocks;
+  const int c0 = block / bi * CZ, i0 = block % bi * CI;
+  const int64_t share = blockIdx.x / blocks, shares = gridDim.x / blocks, tiles = (total + kWgRows - 1) / kWgRows;
+  const int64_t mine = share < tiles ? (tiles - 1 - share) / shares + 1 : 0;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kWgStages * P * PLANE);
+  auto load = [&](int64_t k, int stage) {  // the k-th of this CTA's tiles
+    if (k >= mine) {
+      if (!boxes) cp_async_commit();
+      return;
+    }
+    const int64_t r0 = (share + k * shares) * kWgRows;
+    double* to = smem + stage * P * PLANE;
+    if (boxes) {
+      if (tid != 0) return;
+      fence_proxy_async();
+      mbar_arrive_expect_tx(bars + stage, unsigned(P * PLANE * sizeof(double)));
+      for (int p = 0; p < P; ++p)
+        tma_load_2d(to + p * PLANE, p < PZ ? &dz_map : &hidden_map, p < PZ ? c0 + p * kFwKC : i0 + (p - PZ) * kFwKC, int(r0),
+                    bars + stage);
+    } else {
+      for (int e = tid; e < P * kWgRows * kFwKC; e += kWgThreads) {
+        const int p = e / (kWgRows * kFwKC), r = e / kFwKC % kWgRows, k = e % kFwKC;
+        const bool z = p < PZ;
+        const int c = z ? c0 + p * kFwKC + k : i0 + (p - PZ) * kFwKC + k, width = z ? cout : cin;
+        const bool ok = r0 + r < total && c < width;
+        const double* from = z ? dz : hidden;
+        cp_async8(to + p * PLANE + r * LD + k, ok ? from + (r0 + r) * width + c : from, ok);
+      }
+      cp_async_commit();
+    }
+  };
+  if (tid == 0)
+    for (int s = 0; s < kWgStages; ++s) mbar_init(bars + s, 1);
+  __syncthreads();
+  load(0, 0);
+  load(1, 1);
+  const int wz = warp / WI * 16 * MT, wh = warp % WI;
+  const bool live = c0 + wz < cout && i0 + wh * 32 < cin;
+  double acc[MT][4][4], db = 0.0;
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[m][j][e] = 0.0;
+  int stage = 0;
+  unsigned phase = 0;
+  for (int64_t k = 0; k < mine; ++k) {
+    const bool ok = boxes ? mbar_wait(bars + stage, phase) : (cp_async_wait<1>(), true);
+    if (__syncthreads_or(!ok)) {  // a copy's bounded wait gave up
+      if (tid == 0) atomicExch(&g_affine_fault, 1);
+      return;
+    }
+    load(k + 2, stage == 0 ? 2 : stage - 1);  // the stage whose readers that barrier has let pass
+    const double* at = smem + stage * P * PLANE;
+    if (live) {
+      const double* za = at + wz / kFwKC * PLANE + t * LD + wz % kFwKC + g;
+      const double* hb = at + (PZ + wh) * PLANE + t * LD + g;
+#pragma unroll
+      for (int r = 0; r < kWgRows; r += 8) {
+        double a[MT][4], b[4][2];
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) a[m][e] = za[16 * m + (r + 4 * (e >> 1)) * LD + 8 * (e & 1)];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) b[j][0] = hb[r * LD + 8 * j], b[j][1] = hb[(r + 4) * LD + 8 * j];
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) mma_m16n8k8(acc[m][j], a[m], b[j][0], b[j][1]);
+      }
+    }
+    if (i0 == 0 && tid < CZ) {
+      const int64_t r0 = (share + k * shares) * kWgRows;
+      const double* z = at + tid / kFwKC * PLANE + tid % kFwKC;
+      // order-0 rows: every q-th of the full points', every value row
+      const int skip = int((q - r0 % q) % q);
+      for (int r = r0 + skip < full_rows ? skip : int(full_rows > r0 ? full_rows - r0 : 0); r < kWgRows;
+           r += r0 + r + q < full_rows ? q : r0 + r < full_rows ? int(full_rows - r0) - r : 1)
+        db += z[r * LD];
+    }
+    if (++stage == kWgStages) stage = 0, phase ^= 1;
+  }
+  if (!boxes) cp_async_wait<0>();
+  double* to = partials + share * cout * (int64_t(cin) + 1);
+  if (live) {
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int c = c0 + wz + 16 * m + g + 8 * (e >> 1), i = i0 + wh * 32 + 8 * j + 2 * t + (e & 1);
+          if (c < cout && i < cin) to[int64_t(c) * cin + i] = acc[m][j][e];
+        }
+  }
+  if (i0 == 0 && tid < CZ && c0 + tid < cout) to[int64_t(cout) * cin + c0 + tid] = db;
+}
+
+// dW [cout * cin] and db [cout] from partials [parts][cout * cin + cout]: 16 strands of parts a
+// value, each in order, then the strands in order
+constexpr int kFinStrands = 16, kFinLanes = 32;
+__global__ void __launch_bounds__(kFinStrands* kFinLanes)
     affine_finish(const double* __restrict__ partials, int parts, double* __restrict__ dw, double* __restrict__ db,
-                  int cin, int cout) {
-  const int64_t total = int64_t(cout) * (cin + 1);
-  for (int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += int64_t(gridDim.x) * blockDim.x) {
-    double s = 0.0;
-    for (int p = 0; p < parts; ++p) s += partials[p * total + i];
-    const int64_t c = i / (cin + 1);
-    const int k = int(i % (cin + 1));
-    if (k < cin) dw[c * cin + k] = s;
-    else db[c] = s;
+                  int64_t nw, int64_t n) {
+  __shared__ double shared[kFinStrands][kFinLanes];
+  const int lane = threadIdx.x % kFinLanes, strand = threadIdx.x / kFinLanes;
+  const int64_t i = int64_t(blockIdx.x) * kFinLanes + lane;
+  double s = 0.0;
+  pdl_wait();
+  if (i < n) {
+#pragma unroll 10
+    for (int k = strand; k < parts; k += kFinStrands) s += partials[k * n + i];
+  }
+  shared[strand][lane] = s;
+  __syncthreads();
+  if (strand == 0 && i < n) {
+    for (int k = 1; k < kFinStrands; ++k) s += shared[k][lane];
+    if (i < nw) dw[i] = s;
+    else db[i - nw] = s;
   }
 }
 
@@ -575,8 +923,103 @@ unsigned grid_for(int64_t count) {
   return unsigned(blocks < (1 << 20) ? blocks : (1 << 20));
 }
 
-size_t affine_scratch(int64_t count, int cin, int cout, bool act) {
-  return (size_t(kWgParts) * cout * (size_t(cin) + 1) + (act ? size_t(count) * cout : 0)) * sizeof(double);
+// What an adjoint call runs and the scratch that takes: dZ (unless it is the seed, or fused),
+// then the partials of dW and db.
+struct BackPlan {
+  bool fused, tiled;    // one kernel for everything; dZ and dH in one kernel
+  int64_t parts;        // partials
+  int64_t dz, doubles;  // scratch
+};
+BackPlan back_plan(int64_t count, int cin, int cout, bool act, int sms) {
+  BackPlan p;
+  p.fused = cin <= 64 && cout <= 64;
+  p.tiled = cout <= 128;
+  const int64_t n = cout * (int64_t(cin) + 1);
+  if (p.fused) {
+    p.parts = std::min<int64_t>((count + 79) / 80, sms);
+    p.dz = 0;
+  } else {
+    const int mt = cin <= 64 || cout <= 64 ? 1 : 2, wi = cin <= 64 ? 2 : 4;
+    const int64_t blocks = ((int64_t(cin) + 32 * wi - 1) / (32 * wi)) * ((int64_t(cout) + wg_cout(mt, wi) - 1) / wg_cout(mt, wi));
+    p.parts = std::min<int64_t>((count + kWgRows - 1) / kWgRows, std::max<int64_t>(sms / blocks, 1));
+    p.dz = act ? (count * cout + 15) / 16 * 16 : 0;
+  }
+  p.doubles = p.dz + p.parts * n;
+  return p;
+}
+
+template <int DIM, bool ACT, int WC, bool FUSED>
+cudaError_t launch_backward_tile(const double* hidden, const double* weight, const double* activated, const double* aux,
+                                 const double* seed, double* dz, double* dh, double* partials, int64_t parts, Packed rows,
+                                 int cin, int cout, bool boxes, int sms, cudaStream_t stream) {
+  const auto kernel = affine_backward_tile<DIM, ACT, WC, FUSED>;
+  const size_t smem = back_smem(WC, FUSED, cin, cout);
+  const int64_t total = rows.full * Jet<DIM>::Q + rows.value, tiles = (total + tile_rows(WC) - 1) / tile_rows(WC);
+  const int64_t blocks = (int64_t(cin) + 16 * WC - 1) / (16 * WC);
+  CUtensorMap map{};
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+  if (e == cudaSuccess && FUSED && boxes) e = matrix_map(&map, hidden, total, cin, kFwLD, tile_rows(WC));
+  if (e != cudaSuccess) return e;
+  const int64_t per = FUSED ? parts : std::min(tiles, std::max<int64_t>(sms / blocks, 1));
+  const bool vec_out = cin % 2 == 0 && aligned16(dh);
+  kernel<<<unsigned(per * blocks), 2 * kTileGroup, smem, stream>>>(map, hidden, weight, activated, aux, seed, dz, dh,
+                                                                  partials, rows, cin, cout, boxes, vec_out);
+  return cudaGetLastError();
+}
+
+template <int MT, int WI>
+cudaError_t launch_wgrad(const double* dz, const double* hidden, double* partials, int64_t parts, int64_t total,
+                         int64_t full_rows, int q, int cin, int cout, cudaStream_t stream) {
+  const auto kernel = affine_wgrad_tile<MT, WI>;
+  const size_t smem = wg_smem(MT, WI);
+  const int64_t blocks = ((int64_t(cin) + 32 * WI - 1) / (32 * WI)) * ((int64_t(cout) + wg_cout(MT, WI) - 1) / wg_cout(MT, WI));
+  const bool boxes = cin % 2 == 0 && cout % 2 == 0 && aligned16(dz) && aligned16(hidden) && total < INT_MAX - 1024;
+  CUtensorMap dz_map{}, hidden_map{};
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+  if (e == cudaSuccess && boxes) e = matrix_map(&dz_map, dz, total, cout, kFwLD, kWgRows);
+  if (e == cudaSuccess && boxes) e = matrix_map(&hidden_map, hidden, total, cin, kFwLD, kWgRows);
+  if (e != cudaSuccess) return e;
+  kernel<<<unsigned(parts * blocks), kWgThreads, smem, stream>>>(dz_map, hidden_map, dz, hidden, partials, total, full_rows,
+                                                                q, cin, cout, boxes);
+  return cudaGetLastError();
+}
+
+template <int DIM, bool ACT>
+cudaError_t backward(const double* hidden, const double* weight, const double* activated, const double* aux,
+                     const double* seed, double* dh, double* dw, double* db, double* scratch, const BackPlan& plan,
+                     Packed rows, int cin, int cout, int sms, cudaStream_t stream) {
+  constexpr int Q = Jet<DIM>::Q;
+  const int64_t total = rows.full * Q + rows.value;
+  double *dz = plan.dz ? scratch : nullptr, *partials = scratch + plan.dz;
+  const bool boxes = cin % 2 == 0 && aligned16(hidden) && total < INT_MAX - 1024;
+  cudaError_t e = cudaSuccess;
+  if (plan.fused) {
+    e = launch_backward_tile<DIM, ACT, 4, true>(hidden, weight, activated, aux, seed, dz, dh, partials, plan.parts, rows, cin,
+                                                cout, boxes, sms, stream);
+  } else {
+    const double* z = ACT ? dz : seed;
+    if (plan.tiled) {
+      e = launch_backward_tile<DIM, ACT, 8, false>(hidden, weight, activated, aux, seed, dz, dh, partials, plan.parts, rows,
+                                                   cin, cout, false, sms, stream);
+    } else {
+      if constexpr (ACT) {
+        affine_seed<DIM><<<grid_for(rows.units<Q>() * cout), kAffThreads, 0, stream>>>(activated, aux, seed, dz, rows, cout);
+        e = cudaGetLastError();
+      }
+      // dH = dZ W: the forward product over the output channels, with W read across
+      if (e == cudaSuccess)
+        e = forward<DIM, false>(cout, cin, false, z, weight, static_cast<const double*>(nullptr),
+                                static_cast<const double*>(nullptr), dh, static_cast<double*>(nullptr),
+                                static_cast<double*>(nullptr), rows, cout, cin, true, stream);
+    }
+    if (e != cudaSuccess) return e;
+    const auto wgrad = cin <= 64 ? launch_wgrad<1, 2> : cout <= 64 ? launch_wgrad<1, 4> : launch_wgrad<2, 4>;
+    e = wgrad(z, hidden, partials, plan.parts, total, rows.full * Q, Q, cin, cout, stream);
+  }
+  if (e != cudaSuccess) return e;
+  const int64_t nw = int64_t(cin) * cout, n = nw + cout;
+  return launch_dependent(affine_finish, unsigned((n + kFinLanes - 1) / kFinLanes), kFinStrands * kFinLanes, 0, stream,
+                          partials, int(plan.parts), dw, db, nw, n);
 }
 
 }  // namespace
@@ -603,7 +1046,7 @@ int flashns_b200_affine(int dim, int activation, const double* hidden, const dou
     return int(cudaErrorInvalidValue);
   // TMA boxes: rows on 16-byte boundaries, row numbers that fit their 32-bit coordinate
   const bool boxes = cin % 2 == 0 && aligned16(hidden) && count < INT_MAX - 1024;
-  const auto run = [&](auto launch) { return int(launch(cin, cout, boxes, hidden, weight, bias, residual, out, activated, aux, rows, cin, cout, stream)); };
+  const auto run = [&](auto launch) { return int(launch(cin, cout, boxes, hidden, weight, bias, residual, out, activated, aux, rows, cin, cout, false, stream)); };
   if (dim == 2) return activation ? run([](auto... a) { return forward<2, true>(a...); }) : run([](auto... a) { return forward<2, false>(a...); });
   return activation ? run([](auto... a) { return forward<3, true>(a...); }) : run([](auto... a) { return forward<3, false>(a...); });
 }
@@ -614,7 +1057,12 @@ int flashns_b200_affine_vjp_scratch(int dim, int activation, int64_t full_points
       (activation != 0 && activation != 1) || !bytes)
     return int(cudaErrorInvalidValue);
   const int64_t count = full_points * (dim == 2 ? 10 : 20) + value_points;
-  *bytes = count ? affine_scratch(count, cin, cout, activation != 0) : 0;
+  *bytes = 0;
+  if (count == 0) return int(cudaSuccess);
+  int sms = 0;
+  const cudaError_t e = sm_count(&sms);
+  if (e != cudaSuccess) return int(e);
+  *bytes = size_t(back_plan(count, cin, cout, activation != 0, sms).doubles) * sizeof(double);
   return int(cudaSuccess);
 }
 
@@ -636,24 +1084,18 @@ int flashns_b200_affine_vjp(int dim, int activation, const double* hidden, const
   if (!hidden || !weight || !seed || !d_hidden || !scratch || (activation && (!activated || !aux)))
     return int(cudaErrorInvalidValue);
   const size_t in = size_t(count) * cin * sizeof(double), bytes = size_t(count) * cout * sizeof(double);
-  if (scratch_bytes < affine_scratch(count, cin, cout, activation != 0) || ranges_overlap(d_hidden, in, hidden, in) ||
-      ranges_overlap(d_hidden, in, seed, bytes) || ranges_overlap(d_hidden, in, activated, bytes) ||
-      ranges_overlap(d_hidden, in, scratch, scratch_bytes))
+  if (ranges_overlap(d_hidden, in, hidden, in) || ranges_overlap(d_hidden, in, seed, bytes) ||
+      ranges_overlap(d_hidden, in, activated, bytes) || ranges_overlap(d_hidden, in, scratch, scratch_bytes))
     return int(cudaErrorInvalidValue);
-  double* partials = scratch;
-  const double* dz = seed;
-  if (activation) {
-    double* z = scratch + size_t(kWgParts) * cout * (size_t(cin) + 1);
-    const unsigned grid = grid_for((dim == 2 ? rows.units<10>() : rows.units<20>()) * cout);
-    if (dim == 2) affine_seed<2><<<grid, kAffThreads, 0, stream>>>(activated, aux, seed, z, rows, cout);
-    else affine_seed<3><<<grid, kAffThreads, 0, stream>>>(activated, aux, seed, z, rows, cout);
-    dz = z;
-  }
-  affine_dgrad<<<grid_for(count * cin), kAffThreads, 0, stream>>>(dz, weight, d_hidden, count, cin, cout);
-  const dim3 grid(unsigned(cin / kWgTile + 1), unsigned((cout + kWgTile - 1) / kWgTile), kWgParts);
-  affine_wgrad<<<grid, kWgTile * kWgTile, 0, stream>>>(dz, hidden, partials, count, full_points * q, q, cin, cout);
-  affine_finish<<<grid_for(int64_t(cout) * (cin + 1)), kAffThreads, 0, stream>>>(partials, kWgParts, d_weight, d_bias, cin, cout);
-  return int(cudaGetLastError());
+  int sms = 0;
+  const cudaError_t e = sm_count(&sms);
+  if (e != cudaSuccess) return int(e);
+  const BackPlan plan = back_plan(count, cin, cout, activation != 0, sms);
+  if (scratch_bytes < size_t(plan.doubles) * sizeof(double)) return int(cudaErrorInvalidValue);
+  const auto run = dim == 2 ? (activation ? backward<2, true> : backward<2, false>)
+                            : (activation ? backward<3, true> : backward<3, false>);
+  return int(run(hidden, weight, activated, aux, seed, d_hidden, d_weight, d_bias, scratch, plan, rows, cin, cout, sms,
+                 stream));
 }
 
 }  // extern "C"
