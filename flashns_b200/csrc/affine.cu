@@ -535,28 +535,36 @@ __global__ void __launch_bounds__(kAffThreads)
 
 // dZ = VJP(A, a1; G) and dH = dZ W in one pass; FUSED (both widths <= 64): dW += dZ^T H too.
 //
-// Two groups of 8 warps, tiles of 320 / WC rows and 16 WC input channels, W resident.  Outside
-// its turn a group forms its next tile's dZ (a thread takes a unit's whole jet of one output
-// channel from global memory) in shared memory, where both products read it; inside it runs
-// only MMAs: dH^T = W^T dZ^T, with a thread's two input channels side by side (the pair of a
-// row of W is one 16-byte load, and dH leaves as 16-byte pairs), then dW = dZ^T H, whose
-// accumulators stay in registers over all of the CTA's tiles.  The partner's turn (11,000 or
-// 21,000 cycles) covers the loads, the VJP and the stores.  Unfused, dZ goes to global memory
-// for affine_wgrad_tile.
+// Two groups of 8 warps, tiles of 320 / WC rows and 16 WC input channels, W resident.  Inside
+// its turn a group runs FP64 work alone: its tile's dZ, in G's place in shared memory (a thread
+// takes a unit's whole jet of one output channel); dH^T = W^T dZ^T from there, with a thread's
+// two input channels side by side (the pair of a row of W is one 16-byte load, and dH leaves as
+// 16-byte pairs); then dW = dZ^T H, whose accumulators stay in registers over all of the CTA's
+// tiles.  The partner's turn (12,000 cycles and more) covers what moves data: G and A in by
+// TMA boxes (unfused, A and a1 go to registers), dH out.  H takes A's place once the VJP has
+// read it, behind the MMAs of dH.  Outside the turn the VJP took 15,000 cycles behind the
+// partner's MMAs, against some 1,300 inside; copies issued by threads slow those MMAs.
+// Unfused, dZ also goes to global memory, for affine_wgrad_tile.
 constexpr size_t back_smem(int wc, bool fused, int cin, int cout) {
-  return sizeof(double) * (2 * size_t(tile_rows(wc)) * kFwLD * (tile_planes(cout) + (fused ? tile_planes(cin) : 0)) +
-                           size_t((cout + 7) / 8 * 8) * (16 * wc + 4) + 2);
+  const int other = cin > cout ? cin : cout;  // H and A share their place
+  return sizeof(double) * (2 * size_t(tile_rows(wc)) * kFwLD * (tile_planes(cout) + (fused ? tile_planes(other) : 0)) +
+                           size_t((cout + 7) / 8 * 8) * (16 * wc + 4) + 4);
 }
+
+struct BackMaps {
+  CUtensorMap seed, activated, hidden;
+};
 
 template <int DIM, bool ACT, int WC, bool FUSED>
 __global__ void __launch_bounds__(2 * kTileGroup, 1)
-    affine_backward_tile(const __grid_constant__ CUtensorMap hidden_map, const double* __restrict__ hidden,
+    affine_backward_tile(const __grid_constant__ BackMaps maps, const double* __restrict__ hidden,
                          const double* __restrict__ weight, const double* __restrict__ activated,
                          const double* __restrict__ aux, const double* __restrict__ seed, double* __restrict__ dz,
                          double* __restrict__ dh, double* __restrict__ partials, Packed rows, int cin, int cout,
                          bool boxes, bool vec_out) {
   constexpr int Q = Jet<DIM>::Q, RT = tile_rows(WC), CB = 16 * WC, LD = kFwLD, PLANE = RT * LD, LDW = CB + 4;
   constexpr int NT = RT * WC / 64, UT = RT / Q, PAIRS = UT * CB / kTileGroup;  // n8 tiles a warp; jets a thread
+  constexpr bool SWAP = FUSED && ACT;  // A first, then H in its place
   static_assert(NT == 5 && PAIRS * kTileGroup == UT * CB && RT % 8 == 0, "");
   extern __shared__ __align__(128) double smem[];
   const int tid = threadIdx.x, group = tid / kTileGroup, gt = tid % kTileGroup, warp = gt >> 5, wc = warp % WC, wr = warp / WC;
@@ -570,77 +578,112 @@ __global__ void __launch_bounds__(2 * kTileGroup, 1)
   const int64_t tiles = (total + RT - 1) / RT, first = blockIdx.x / blocks + group * per;
   const auto count = [&](int64_t from) { return from < tiles ? (tiles - 1 - from) / (2 * per) + 1 : 0; };
   const int pz = tile_planes(cout), ph = FUSED ? tile_planes(cin) : 0, c8 = (cout + 7) / 8 * 8;
-  double *z_at = smem + group * (pz + ph) * PLANE, *h_at = z_at + pz * PLANE, *sw = smem + 2 * (pz + ph) * PLANE;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sw + c8 * LDW);
+  const int px = FUSED ? (pz > ph ? pz : ph) : 0;  // planes of the place that A and H share
+  double *z_at = smem + group * (pz + px) * PLANE, *h_at = z_at + pz * PLANE, *sw = smem + 2 * (pz + px) * PLANE;
+  uint64_t *bar = reinterpret_cast<uint64_t*>(sw + c8 * LDW) + 2 * group, *bar_h = bar + 1;
 
-  // the tile's H, once every warp has read the last one: one thread, or all where boxes cannot
-  auto load_hidden = [&](int64_t tile) {
+  // a tile's planes of a [total][width] matrix, by TMA (one thread, after bar's expect) or by all
+  auto copy = [&](double* to, const CUtensorMap* map, const double* from, int64_t tile, int planes, int width, uint64_t* b) {
     if (boxes) {
-      if (gt == 0) {
-        fence_proxy_async();
-        mbar_arrive_expect_tx(bars + group, unsigned(ph * PLANE * sizeof(double)));
-        for (int p = 0; p < ph; ++p) tma_load_2d(h_at + p * PLANE, &hidden_map, p * kFwKC, int(tile * RT), bars + group);
-      }
+      for (int p = 0; p < planes; ++p) tma_load_2d(to + p * PLANE, map, p * kFwKC, int(tile * RT), b);
     } else {
-      for (int e = gt; e < RT * ph * kFwKC; e += kTileGroup) {
-        const int r = e / (ph * kFwKC), k = e % (ph * kFwKC);
-        const bool ok = tile * RT + r < total && k < cin;
-        cp_async8(h_at + k / kFwKC * PLANE + r * LD + k % kFwKC, ok ? hidden + (tile * RT + r) * cin + k : hidden, ok);
+#pragma unroll 1
+      for (int e = gt; e < RT * planes * kFwKC; e += kTileGroup) {
+        const int r = e / (planes * kFwKC), k = e % (planes * kFwKC);
+        const bool ok = tile * RT + r < total && k < width;
+        cp_async8(to + k / kFwKC * PLANE + r * LD + k % kFwKC, ok ? from + (tile * RT + r) * width + k : from, ok);
       }
-      cp_async_commit();
     }
   };
-  // this thread's jets of a tile's dZ, channel cz
+  // This thread's jets: channel cz of the tile's units ul(i).
   const int cz = gt % CB;
-  double db = 0.0;
-  auto form_dz = [&](int64_t tile) {
-    if (cz >= c8) return;
+  const bool has_z = cz < cout;
+  double* const z_mine = z_at + cz / kFwKC * PLANE + cz % kFwKC;
+  const double* const a_mine = h_at + cz / kFwKC * PLANE + cz % kFwKC;
+  const auto ul = [&](int i) { return gt / CB + i * (kTileGroup / CB); };
+  double kept[ACT && !FUSED ? PAIRS : 1][Q], a1[PAIRS], db = 0.0;
+  auto request = [&](int64_t tile) {  // once every warp has read the last tile's dZ and H
+    if (!boxes || gt == 0) {
+      if (boxes) {
+        fence_proxy_async();
+        mbar_arrive_expect_tx(bar, unsigned((pz + (SWAP ? pz : ph)) * PLANE * sizeof(double)));
+      }
+      copy(z_at, &maps.seed, seed, tile, pz, cout, bar);
+      if (SWAP) copy(h_at, &maps.activated, activated, tile, pz, cout, bar);
+      else if (FUSED) copy(h_at, &maps.hidden, hidden, tile, ph, cin, bar);
+      if (SWAP && boxes) {
+        const int64_t left = total - tile * RT;
+        prefetch_l2(hidden + tile * RT * cin, unsigned((left < RT ? left : RT) * cin * sizeof(double)));
+      }
+    }
+    cp_async_commit();
+    if constexpr (ACT) {
 #pragma unroll
-    for (int i = 0; i < PAIRS; ++i) {
-      const int ul = gt / CB + i * (kTileGroup / CB);
-      const int64_t u = tile * UT + ul;
-      double z[Q];
+      for (int i = 0; i < PAIRS; ++i) {
+        const int64_t u = tile * UT + ul(i);
+        const bool live = has_z && u < units, full = live && u < rows.full;
+        a1[i] = full ? aux[u * cout + cz] : 0.0;
+        if constexpr (!FUSED) {
+          const int n = live ? rows.count<Q>(u) : 0;
+          const int64_t step = opaque(cout);
+          const double* from = full ? activated + rows.row<Q>(u) * cout + cz  // value rows: their a1
+                                    : aux + (rows.full + (u - rows.full) * Q) * cout + cz;
 #pragma unroll
-      for (int s = 0; s < Q; ++s) z[s] = 0.0;
-      if (u < units && cz < cout) {
-        const int n = rows.count<Q>(u);
-        const int64_t at = rows.row<Q>(u) * cout + cz, step = opaque(cout);
-        const double* from = seed + at;
-        if (u < rows.full) {
-          double gz[Q];
-#pragma unroll
-          for (int s = 0; s < Q; ++s, from += step) gz[s] = *from;
-          if constexpr (ACT) {
-            double h[Q];
-            const double* act = activated + at;
-#pragma unroll
-            for (int s = 0; s < Q; ++s, act += step) h[s] = *act;
-            tanh_vjp<DIM>(h, aux[u * cout + cz], gz, z);
-          } else {
-#pragma unroll
-            for (int s = 0; s < Q; ++s) z[s] = gz[s];
-          }
-          if constexpr (FUSED) db += z[0];
-        } else {
-          const double* a1 = ACT ? aux + (rows.full + (u - rows.full) * Q) * cout + cz : nullptr;
-#pragma unroll
-          for (int s = 0; s < Q; ++s)
-            if (s < n) {
-              z[s] = from[s * step];
-              if constexpr (ACT) z[s] *= a1[s * step];
-              if constexpr (FUSED) db += z[s];
-            }
-        }
-        if (!FUSED && dz && i0 == 0) {
-          double* to = dz + at;
-#pragma unroll
-          for (int s = 0; s < Q; ++s, to += step)
-            if (s < n) *to = z[s];
+          for (int s = 0; s < Q; ++s, from += step) kept[i][s] = s < n ? *from : 0.0;
         }
       }
-      double* to = z_at + cz / kFwKC * PLANE + ul * Q * LD + cz % kFwKC;
+    }
+  };
+  auto form = [&](int64_t tile) {
+    if (!has_z) return;
 #pragma unroll
-      for (int s = 0; s < Q; ++s) to[s * LD] = z[s];
+    for (int i = 0; i < PAIRS; ++i) {
+      const int64_t u = tile * UT + ul(i);
+      double* at = z_mine + ul(i) * Q * LD;
+      double z[Q];
+      if constexpr (ACT) {
+        double gz[Q], h[Q];
+#pragma unroll
+        for (int s = 0; s < Q; ++s) {
+          gz[s] = at[s * LD];
+          h[s] = FUSED ? a_mine[(ul(i) * Q + s) * LD] : kept[FUSED ? 0 : i][s];
+        }
+        if (u < rows.full) {
+          tanh_vjp<DIM>(h, a1[i], gz, z);
+        } else {
+          const int n = u < units ? rows.count<Q>(u) : 0;
+          const double* from = aux + (rows.full + (u - rows.full) * Q) * cout + cz;
+#pragma unroll
+          for (int s = 0; s < Q; ++s) z[s] = gz[s] * (FUSED ? (s < n ? from[int64_t(s) * cout] : 0.0) : h[s]);
+        }
+#pragma unroll
+        for (int s = 0; s < Q; ++s) at[s * LD] = z[s];
+      } else if constexpr (FUSED) {
+#pragma unroll
+        for (int s = 0; s < Q; ++s) z[s] = at[s * LD];
+      }
+      if constexpr (FUSED) {
+        db += z[0];
+        if (u >= rows.full) {
+#pragma unroll
+          for (int s = 1; s < Q; ++s) db += z[s];
+        }
+      }
+    }
+  };
+  auto store_dz = [&](int64_t tile) {  // unfused: for affine_wgrad_tile
+    if (!ACT || FUSED || i0 != 0 || !has_z) return;
+#pragma unroll 1
+    for (int i = 0; i < PAIRS; ++i) {
+      const int64_t u = tile * UT + ul(i);
+      if (u >= units) continue;
+      const int n = rows.count<Q>(u);
+      const int64_t step = opaque(cout);
+      double* to = dz + rows.row<Q>(u) * cout + cz;
+      const double* from = z_mine + ul(i) * Q * LD;
+#pragma unroll
+      for (int s = 0; s < Q; ++s, to += step)
+        if (s < n) *to = from[s * LD];
     }
   };
 
@@ -650,16 +693,13 @@ __global__ void __launch_bounds__(2 * kTileGroup, 1)
     cp_async8(sw + c * LDW + i, ok ? weight + int64_t(c) * cin + i0 + i : weight, ok);
   }
   cp_async_commit();
-  if (tid == 0) {
-    mbar_init(bars, 1);
-    mbar_init(bars + 1, 1);
+  if (gt == 0) {
+    mbar_init(bar, 1);
+    mbar_init(bar_h, 1);
   }
   cp_async_wait<0>();
   __syncthreads();
-  if (first < tiles) {
-    if (FUSED) load_hidden(first);
-    form_dz(first);
-  }
+  if (first < tiles) request(first);
 
   const int ci = i0 + wc * 16 + 2 * g;  // this thread's input channels ci, ci + 1
   const double* ap = sw + t * LDW + wc * 16 + 2 * g;
@@ -677,24 +717,31 @@ __global__ void __launch_bounds__(2 * kTileGroup, 1)
   const double* wb = h_at + wh * PLANE + t * LD + g;
   const Turns<2, kTileGroup> turns(group);
   unsigned phase = 0;
-  bool dead = false;  // a copy's bounded wait gave up: the group keeps the turns and does no work
+  bool dead = false, late = false;  // a copy's bounded wait gave up: the group keeps the turns and does no work
   for (int64_t tile = first; tile < tiles; tile += 2 * per) {
     double acc[NT][4];
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[j][e] = 0.0;
-    if (FUSED && boxes) {
-      if (!dead) {
-        dead = named_sync_or(1 + group, kTileGroup, !mbar_wait(bars + group, phase));
-        if (dead && gt == 0) atomicExch(&g_affine_fault, 1);
-      }
-      phase ^= 1;
-    } else {
-      if (FUSED) cp_async_wait<0>();
-      named_sync(1 + group, kTileGroup);
+    cp_async_wait<0>();
+    if (!dead) {
+      dead = named_sync_or(1 + group, kTileGroup, late || (boxes && !mbar_wait(bar, phase)));
+      if (dead && gt == 0) atomicExch(&g_affine_fault, 1);
     }
     turns.take();
+    if (ACT || FUSED) form(tile);
+    if constexpr (ACT) {
+      named_sync(1 + group, kTileGroup);  // dZ is there, A has been read
+      if (SWAP && !dead && (!boxes || gt == 0)) {
+        if (boxes) {
+          fence_proxy_async();
+          mbar_arrive_expect_tx(bar_h, unsigned(ph * PLANE * sizeof(double)));
+        }
+        copy(h_at, &maps.hidden, hidden, tile, ph, cin, bar_h);
+        cp_async_commit();
+      }
+    }
     if (!dead && has_h) {
       for (int p = 0; p < pz; ++p) {
         const double *a_at = ap + p * kFwKC * LDW, *b_at = bp + p * PLANE;
@@ -710,7 +757,16 @@ __global__ void __launch_bounds__(2 * kTileGroup, 1)
         }
       }
     }
-    if (!dead && has_w) {
+    if (SWAP) {
+      if (!boxes) {
+        cp_async_wait<0>();
+        named_sync(1 + group, kTileGroup);
+      } else if (!dead) {
+        late = !mbar_wait(bar_h, phase);
+        if (late) atomicExch(&g_affine_fault, 1);
+      }
+    }
+    if (!dead && !late && has_w) {
 #pragma unroll
       for (int r = 0; r < RT; r += 8) {
         const double a[4] = {wa[r * LD], wa[r * LD + 8], wa[(r + 4) * LD], wa[(r + 4) * LD + 8]};
@@ -718,10 +774,13 @@ __global__ void __launch_bounds__(2 * kTileGroup, 1)
         for (int j = 0; j < WN; ++j) mma_m16n8k8(wacc[j], a, wb[r * LD + 8 * j], wb[(r + 4) * LD + 8 * j]);
       }
     }
+    phase ^= 1;
     turns.pass();
     named_sync(1 + group, kTileGroup);  // every warp has read dZ and H
     const int64_t next = tile + 2 * per;
-    if (FUSED && next < tiles && !dead) load_hidden(next);
+    store_dz(tile);
+    if (ACT && !FUSED) named_sync(1 + group, kTileGroup);  // dZ has been read for global memory
+    if (next < tiles && !dead) request(next);
     if (!dead && ci < cin) {
       const bool two = ci + 1 < cin;
 #pragma unroll
@@ -739,7 +798,6 @@ __global__ void __launch_bounds__(2 * kTileGroup, 1)
           }
         }
     }
-    if (next < tiles) form_dz(next);
   }
   turns.close(count(first), count(blockIdx.x / blocks + (1 - group) * per));
   if constexpr (FUSED) {  // both groups' shares in order: this CTA's [cout][cin] and [cout]
@@ -951,18 +1009,22 @@ BackPlan back_plan(int64_t count, int cin, int cout, bool act, int sms) {
 template <int DIM, bool ACT, int WC, bool FUSED>
 cudaError_t launch_backward_tile(const double* hidden, const double* weight, const double* activated, const double* aux,
                                  const double* seed, double* dz, double* dh, double* partials, int64_t parts, Packed rows,
-                                 int cin, int cout, bool boxes, int sms, cudaStream_t stream) {
+                                 int cin, int cout, int sms, cudaStream_t stream) {
   const auto kernel = affine_backward_tile<DIM, ACT, WC, FUSED>;
   const size_t smem = back_smem(WC, FUSED, cin, cout);
   const int64_t total = rows.full * Jet<DIM>::Q + rows.value, tiles = (total + tile_rows(WC) - 1) / tile_rows(WC);
   const int64_t blocks = (int64_t(cin) + 16 * WC - 1) / (16 * WC);
-  CUtensorMap map{};
+  const bool boxes = cout % 2 == 0 && aligned16(seed) && total < INT_MAX - 1024 &&
+                     (!FUSED || (cin % 2 == 0 && aligned16(hidden) && aligned16(activated)));
+  BackMaps maps{};
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
-  if (e == cudaSuccess && FUSED && boxes) e = matrix_map(&map, hidden, total, cin, kFwLD, tile_rows(WC));
+  if (e == cudaSuccess && boxes) e = matrix_map(&maps.seed, seed, total, cout, kFwLD, tile_rows(WC));
+  if (e == cudaSuccess && boxes && FUSED) e = matrix_map(&maps.hidden, hidden, total, cin, kFwLD, tile_rows(WC));
+  if (e == cudaSuccess && boxes && FUSED && ACT) e = matrix_map(&maps.activated, activated, total, cout, kFwLD, tile_rows(WC));
   if (e != cudaSuccess) return e;
   const int64_t per = FUSED ? parts : std::min(tiles, std::max<int64_t>(sms / blocks, 1));
   const bool vec_out = cin % 2 == 0 && aligned16(dh);
-  kernel<<<unsigned(per * blocks), 2 * kTileGroup, smem, stream>>>(map, hidden, weight, activated, aux, seed, dz, dh,
+  kernel<<<unsigned(per * blocks), 2 * kTileGroup, smem, stream>>>(maps, hidden, weight, activated, aux, seed, dz, dh,
                                                                   partials, rows, cin, cout, boxes, vec_out);
   return cudaGetLastError();
 }
@@ -991,16 +1053,15 @@ cudaError_t backward(const double* hidden, const double* weight, const double* a
   constexpr int Q = Jet<DIM>::Q;
   const int64_t total = rows.full * Q + rows.value;
   double *dz = plan.dz ? scratch : nullptr, *partials = scratch + plan.dz;
-  const bool boxes = cin % 2 == 0 && aligned16(hidden) && total < INT_MAX - 1024;
   cudaError_t e = cudaSuccess;
   if (plan.fused) {
     e = launch_backward_tile<DIM, ACT, 4, true>(hidden, weight, activated, aux, seed, dz, dh, partials, plan.parts, rows, cin,
-                                                cout, boxes, sms, stream);
+                                                cout, sms, stream);
   } else {
     const double* z = ACT ? dz : seed;
     if (plan.tiled) {
       e = launch_backward_tile<DIM, ACT, 8, false>(hidden, weight, activated, aux, seed, dz, dh, partials, plan.parts, rows,
-                                                   cin, cout, false, sms, stream);
+                                                   cin, cout, sms, stream);
     } else {
       if constexpr (ACT) {
         affine_seed<DIM><<<grid_for(rows.units<Q>() * cout), kAffThreads, 0, stream>>>(activated, aux, seed, dz, rows, cout);
