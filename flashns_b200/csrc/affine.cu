@@ -560,8 +560,8 @@ __global__ void __launch_bounds__(2 * kTileGroup, 1)
     affine_backward_tile(const __grid_constant__ BackMaps maps, const double* __restrict__ hidden,
                          const double* __restrict__ weight, const double* __restrict__ activated,
                          const double* __restrict__ aux, const double* __restrict__ seed, double* __restrict__ dz,
-                         double* __restrict__ dh, double* __restrict__ partials, Packed rows, int cin, int cout,
-                         bool boxes, bool vec_out) {
+                         double* __restrict__ dh, double* __restrict__ dw_parts, double* __restrict__ db_parts, Packed rows,
+                         int cin, int cout, bool boxes, bool vec_out) {
   constexpr int Q = Jet<DIM>::Q, RT = tile_rows(WC), CB = 16 * WC, LD = kFwLD, PLANE = RT * LD, LDW = CB + 4;
   constexpr int NT = RT * WC / 64, UT = RT / Q, PAIRS = UT * CB / kTileGroup;  // n8 tiles a warp; jets a thread
   constexpr bool SWAP = FUSED && ACT;  // A first, then H in its place
@@ -658,16 +658,14 @@ __global__ void __launch_bounds__(2 * kTileGroup, 1)
         }
 #pragma unroll
         for (int s = 0; s < Q; ++s) at[s * LD] = z[s];
-      } else if constexpr (FUSED) {
+      } else {
 #pragma unroll
         for (int s = 0; s < Q; ++s) z[s] = at[s * LD];
       }
-      if constexpr (FUSED) {
-        db += z[0];
-        if (u >= rows.full) {
+      db += z[0];
+      if (u >= rows.full) {
 #pragma unroll
-          for (int s = 1; s < Q; ++s) db += z[s];
-        }
+        for (int s = 1; s < Q; ++s) db += z[s];
       }
     }
   };
@@ -730,7 +728,7 @@ __global__ void __launch_bounds__(2 * kTileGroup, 1)
       if (dead && gt == 0) atomicExch(&g_affine_fault, 1);
     }
     turns.take();
-    if (ACT || FUSED) form(tile);
+    form(tile);
     if constexpr (ACT) {
       named_sync(1 + group, kTileGroup);  // dZ is there, A has been read
       if (SWAP && !dead && (!boxes || gt == 0)) {
@@ -800,10 +798,20 @@ __global__ void __launch_bounds__(2 * kTileGroup, 1)
     }
   }
   turns.close(count(first), count(blockIdx.x / blocks + (1 - group) * per));
-  if constexpr (FUSED) {  // both groups' shares in order: this CTA's [cout][cin] and [cout]
-    cp_async_wait<0>();
+  cp_async_wait<0>();
+  __syncthreads();
+  double* sums = smem;
+  if (i0 == 0) {  // this CTA's [cout] of db
+    sums[tid] = db;
     __syncthreads();
-    double *sums = smem, *bias_sums = smem + CB * CB;
+    if (tid < cout) {
+      double s = 0.0;
+      for (int k = tid; k < 2 * kTileGroup; k += CB) s += sums[k];
+      db_parts[blockIdx.x / blocks * cout + tid] = s;
+    }
+    __syncthreads();
+  }
+  if constexpr (FUSED) {  // and [cout][cin] of dW: the groups' shares in order
     if (group == 1) {
 #pragma unroll
       for (int j = 0; j < WN; ++j)
@@ -811,39 +819,35 @@ __global__ void __launch_bounds__(2 * kTileGroup, 1)
         for (int e = 0; e < 4; ++e)
           sums[(wz + g + 8 * (e >> 1)) * CB + wh * 32 + 8 * j + 2 * t + (e & 1)] = wacc[j][e];
     }
-    bias_sums[tid] = db;
     __syncthreads();
-    double* mine = partials + int64_t(blockIdx.x) * cout * (int64_t(cin) + 1);
+    double* mine = dw_parts + int64_t(blockIdx.x) * cout * cin;
     if (group == 0) {
 #pragma unroll
       for (int j = 0; j < WN; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int c = wz + g + 8 * (e >> 1), i = wh * 32 + 8 * j + 2 * t + (e & 1);
-          if (c < cout && i < cin) mine[int64_t(c) * cin + i] = wacc[j][e] + sums[c * CB + i];
+          if (c < cout && i < cin) mine[c * cin + i] = wacc[j][e] + sums[c * CB + i];
         }
-    }
-    if (tid < cout) {
-      double s = 0.0;
-      for (int k = tid; k < 2 * kTileGroup; k += CB) s += bias_sums[k];
-      mine[int64_t(cout) * cin + tid] = s;
     }
   }
 }
 
-// dW = dZ^T H and db: a CTA's block of 16 MT (16 / WI) output x 32 WI input channels over its
+// dW = dZ^T H, and db unless db_parts is null: a CTA's block of 16 MT (16 / WI) output x 32 WI input channels over its
 // share of the rows, accumulators in registers throughout; 32-row stages of both operands by
-// TMA boxes (or cp.async), two ahead of the MMAs.  partials [share][cout * cin + cout].
+// TMA boxes (or cp.async), two ahead of the MMAs.  dw_parts [share][cout][cin], db_parts
+// [share][cout].
 constexpr int kWgRows = 32, kWgStages = 3, kWgThreads = 512;
 constexpr int wg_cout(int mt, int wi) { return 16 * mt * (16 / wi); }
 constexpr size_t wg_smem(int mt, int wi) {
-  return sizeof(double) * (size_t(kWgStages) * kWgRows * kFwLD * (wg_cout(mt, wi) / kFwKC + wi) + kWgStages);
+  return sizeof(double) * (size_t(kWgStages) * kWgRows * kFwLD * (wg_cout(mt, wi) / kFwKC + wi) + 2 * kWgStages);
 }
 
 template <int MT, int WI>
 __global__ void __launch_bounds__(kWgThreads, 1)
     affine_wgrad_tile(const __grid_constant__ CUtensorMap dz_map, const __grid_constant__ CUtensorMap hidden_map,
-                      const double* __restrict__ dz, const double* __restrict__ hidden, double* __restrict__ partials,
+                      const double* __restrict__ dz, const double* __restrict__ hidden,
+                      double* __restrict__ dw_parts, double* __restrict__ db_parts,
                       int64_t total, int64_t full_rows, int q, int cin, int cout, bool boxes) {
   constexpr int CZ = wg_cout(MT, WI), CI = 32 * WI, PZ = CZ / kFwKC, P = PZ + WI, LD = kFwLD, PLANE = kWgRows * LD;
   extern __shared__ __align__(128) double smem[];
@@ -856,7 +860,7 @@ __global__ void __launch_bounds__(kWgThreads, 1)
   const int c0 = block / bi * CZ, i0 = block % bi * CI;
   const int64_t share = blockIdx.x / blocks, shares = gridDim.x / blocks, tiles = (total + kWgRows - 1) / kWgRows;
   const int64_t mine = share < tiles ? (tiles - 1 - share) / shares + 1 : 0;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kWgStages * P * PLANE);
+  uint64_t *bars = reinterpret_cast<uint64_t*>(smem + kWgStages * P * PLANE), *empty = bars + kWgStages;
   auto load = [&](int64_t k, int stage) {  // the k-th of this CTA's tiles
     if (k >= mine) {
       if (!boxes) cp_async_commit();
@@ -884,7 +888,10 @@ __global__ void __launch_bounds__(kWgThreads, 1)
     }
   };
   if (tid == 0)
-    for (int s = 0; s < kWgStages; ++s) mbar_init(bars + s, 1);
+    for (int s = 0; s < kWgStages; ++s) {
+      mbar_init(bars + s, 1);
+      mbar_init(empty + s, kWgThreads / 32);
+    }
   __syncthreads();
   load(0, 0);
   load(1, 1);
@@ -900,12 +907,23 @@ __global__ void __launch_bounds__(kWgThreads, 1)
   int stage = 0;
   unsigned phase = 0;
   for (int64_t k = 0; k < mine; ++k) {
-    const bool ok = boxes ? mbar_wait(bars + stage, phase) : (cp_async_wait<1>(), true);
-    if (__syncthreads_or(!ok)) {  // a copy's bounded wait gave up
-      if (tid == 0) atomicExch(&g_affine_fault, 1);
-      return;
+    const int ahead = stage == 0 ? 2 : stage - 1;  // tile k - 1's stage, tile k + 2's next
+    if (boxes) {
+      // the warps meet only at the stages: a warp that is done with one starts on the next
+      bool ok = mbar_wait(bars + stage, phase);
+      if (tid == 0 && k + 2 < mine) {
+        ok = ok && (k == 0 || mbar_wait(empty + ahead, unsigned((k - 1) / kWgStages) & 1));
+        if (ok) load(k + 2, ahead);
+      }
+      if (!__all_sync(0xffffffffu, ok)) {  // a bounded wait gave up; the other warps' will too
+        if (lane == 0) atomicExch(&g_affine_fault, 1);
+        return;
+      }
+    } else {
+      cp_async_wait<1>();
+      __syncthreads();
+      load(k + 2, ahead);
     }
-    load(k + 2, stage == 0 ? 2 : stage - 1);  // the stage whose readers that barrier has let pass
     const double* at = smem + stage * P * PLANE;
     if (live) {
       const double* za = at + wz / kFwKC * PLANE + t * LD + wz % kFwKC + g;
@@ -925,7 +943,7 @@ __global__ void __launch_bounds__(kWgThreads, 1)
           for (int j = 0; j < 4; ++j) mma_m16n8k8(acc[m][j], a[m], b[j][0], b[j][1]);
       }
     }
-    if (i0 == 0 && tid < CZ) {
+    if (db_parts && i0 == 0 && tid < CZ) {
       const int64_t r0 = (share + k * shares) * kWgRows;
       const double* z = at + tid / kFwKC * PLANE + tid % kFwKC;
       // order-0 rows: every q-th of the full points', every value row
@@ -934,10 +952,12 @@ __global__ void __launch_bounds__(kWgThreads, 1)
            r += r0 + r + q < full_rows ? q : r0 + r < full_rows ? int(full_rows - r0) - r : 1)
         db += z[r * LD];
     }
+    __syncwarp();
+    if (boxes && lane == 0) mbar_arrive(empty + stage);
     if (++stage == kWgStages) stage = 0, phase ^= 1;
   }
   if (!boxes) cp_async_wait<0>();
-  double* to = partials + share * cout * (int64_t(cin) + 1);
+  double* to = dw_parts + share * cout * cin;
   if (live) {
 #pragma unroll
     for (int m = 0; m < MT; ++m)
@@ -949,30 +969,34 @@ __global__ void __launch_bounds__(kWgThreads, 1)
           if (c < cout && i < cin) to[int64_t(c) * cin + i] = acc[m][j][e];
         }
   }
-  if (i0 == 0 && tid < CZ && c0 + tid < cout) to[int64_t(cout) * cin + c0 + tid] = db;
+  if (db_parts && i0 == 0 && tid < CZ && c0 + tid < cout) db_parts[share * cout + c0 + tid] = db;
 }
 
-// dW [cout * cin] and db [cout] from partials [parts][cout * cin + cout]: 16 strands of parts a
-// value, each in order, then the strands in order
+// dW [nw] and db [cout] from dw_parts [parts][nw] and db_parts [bias_parts][cout]: 16 strands of
+// parts a value, each in order, then the strands in order
 constexpr int kFinStrands = 16, kFinLanes = 32;
 __global__ void __launch_bounds__(kFinStrands* kFinLanes)
-    affine_finish(const double* __restrict__ partials, int parts, double* __restrict__ dw, double* __restrict__ db,
-                  int64_t nw, int64_t n) {
+    affine_finish(const double* __restrict__ dw_parts, int parts, const double* __restrict__ db_parts, int bias_parts,
+                  double* __restrict__ dw, double* __restrict__ db, int64_t nw, int cout) {
   __shared__ double shared[kFinStrands][kFinLanes];
   const int lane = threadIdx.x % kFinLanes, strand = threadIdx.x / kFinLanes;
   const int64_t i = int64_t(blockIdx.x) * kFinLanes + lane;
+  const bool bias = i >= nw, live = i < nw + cout;
+  const double* from = bias ? db_parts + (i - nw) : dw_parts + i;
+  const int64_t stride = bias ? cout : nw;
+  const int n = bias ? bias_parts : parts;
   double s = 0.0;
   pdl_wait();
-  if (i < n) {
+  if (live) {
 #pragma unroll 10
-    for (int k = strand; k < parts; k += kFinStrands) s += partials[k * n + i];
+    for (int k = strand; k < n; k += kFinStrands) s += from[k * stride];
   }
   shared[strand][lane] = s;
   __syncthreads();
-  if (strand == 0 && i < n) {
+  if (strand == 0 && live) {
     for (int k = 1; k < kFinStrands; ++k) s += shared[k][lane];
-    if (i < nw) dw[i] = s;
-    else db[i - nw] = s;
+    if (bias) db[i - nw] = s;
+    else dw[i] = s;
   }
 }
 
@@ -984,36 +1008,38 @@ unsigned grid_for(int64_t count) {
 // What an adjoint call runs and the scratch that takes: dZ (unless it is the seed, or fused),
 // then the partials of dW and db.
 struct BackPlan {
-  bool fused, tiled;    // one kernel for everything; dZ and dH in one kernel
-  int64_t parts;        // partials
-  int64_t dz, doubles;  // scratch
+  bool fused, tiled;         // one kernel for everything; dZ and dH in one kernel
+  int64_t parts, bias_parts; // partials of dW and db
+  int64_t dz, dw, doubles;   // scratch: dZ, then dW's partials, then db's
 };
 BackPlan back_plan(int64_t count, int cin, int cout, bool act, int sms) {
   BackPlan p;
   p.fused = cin <= 64 && cout <= 64;
   p.tiled = cout <= 128;
-  const int64_t n = cout * (int64_t(cin) + 1);
+  p.dz = 0;
   if (p.fused) {
-    p.parts = std::min<int64_t>((count + 79) / 80, sms);
-    p.dz = 0;
+    p.parts = p.bias_parts = std::min<int64_t>((count + tile_rows(4) - 1) / tile_rows(4), sms);
   } else {
     const int mt = cin <= 64 || cout <= 64 ? 1 : 2, wi = cin <= 64 ? 2 : 4;
     const int64_t blocks = ((int64_t(cin) + 32 * wi - 1) / (32 * wi)) * ((int64_t(cout) + wg_cout(mt, wi) - 1) / wg_cout(mt, wi));
     p.parts = std::min<int64_t>((count + kWgRows - 1) / kWgRows, std::max<int64_t>(sms / blocks, 1));
-    p.dz = act ? (count * cout + 15) / 16 * 16 : 0;
+    const int64_t across = (int64_t(cin) + 127) / 128;
+    p.bias_parts = p.tiled ? std::min<int64_t>((count + tile_rows(8) - 1) / tile_rows(8), std::max<int64_t>(sms / across, 1))
+                           : p.parts;
+    if (act) p.dz = (count * cout + 15) / 16 * 16;
   }
-  p.doubles = p.dz + p.parts * n;
+  p.dw = p.parts * cout * cin;
+  p.doubles = p.dz + p.dw + p.bias_parts * cout;
   return p;
 }
 
 template <int DIM, bool ACT, int WC, bool FUSED>
 cudaError_t launch_backward_tile(const double* hidden, const double* weight, const double* activated, const double* aux,
-                                 const double* seed, double* dz, double* dh, double* partials, int64_t parts, Packed rows,
-                                 int cin, int cout, int sms, cudaStream_t stream) {
+                                 const double* seed, double* dz, double* dh, double* dw_parts, double* db_parts, int64_t per,
+                                 Packed rows, int cin, int cout, cudaStream_t stream) {
   const auto kernel = affine_backward_tile<DIM, ACT, WC, FUSED>;
   const size_t smem = back_smem(WC, FUSED, cin, cout);
-  const int64_t total = rows.full * Jet<DIM>::Q + rows.value, tiles = (total + tile_rows(WC) - 1) / tile_rows(WC);
-  const int64_t blocks = (int64_t(cin) + 16 * WC - 1) / (16 * WC);
+  const int64_t total = rows.full * Jet<DIM>::Q + rows.value, blocks = (int64_t(cin) + 16 * WC - 1) / (16 * WC);
   const bool boxes = cout % 2 == 0 && aligned16(seed) && total < INT_MAX - 1024 &&
                      (!FUSED || (cin % 2 == 0 && aligned16(hidden) && aligned16(activated)));
   BackMaps maps{};
@@ -1022,16 +1048,15 @@ cudaError_t launch_backward_tile(const double* hidden, const double* weight, con
   if (e == cudaSuccess && boxes && FUSED) e = matrix_map(&maps.hidden, hidden, total, cin, kFwLD, tile_rows(WC));
   if (e == cudaSuccess && boxes && FUSED && ACT) e = matrix_map(&maps.activated, activated, total, cout, kFwLD, tile_rows(WC));
   if (e != cudaSuccess) return e;
-  const int64_t per = FUSED ? parts : std::min(tiles, std::max<int64_t>(sms / blocks, 1));
   const bool vec_out = cin % 2 == 0 && aligned16(dh);
   kernel<<<unsigned(per * blocks), 2 * kTileGroup, smem, stream>>>(maps, hidden, weight, activated, aux, seed, dz, dh,
-                                                                  partials, rows, cin, cout, boxes, vec_out);
+                                                                  dw_parts, db_parts, rows, cin, cout, boxes, vec_out);
   return cudaGetLastError();
 }
 
 template <int MT, int WI>
-cudaError_t launch_wgrad(const double* dz, const double* hidden, double* partials, int64_t parts, int64_t total,
-                         int64_t full_rows, int q, int cin, int cout, cudaStream_t stream) {
+cudaError_t launch_wgrad(const double* dz, const double* hidden, double* dw_parts, double* db_parts, int64_t parts,
+                         int64_t total, int64_t full_rows, int q, int cin, int cout, cudaStream_t stream) {
   const auto kernel = affine_wgrad_tile<MT, WI>;
   const size_t smem = wg_smem(MT, WI);
   const int64_t blocks = ((int64_t(cin) + 32 * WI - 1) / (32 * WI)) * ((int64_t(cout) + wg_cout(MT, WI) - 1) / wg_cout(MT, WI));
@@ -1041,27 +1066,27 @@ cudaError_t launch_wgrad(const double* dz, const double* hidden, double* partial
   if (e == cudaSuccess && boxes) e = matrix_map(&dz_map, dz, total, cout, kFwLD, kWgRows);
   if (e == cudaSuccess && boxes) e = matrix_map(&hidden_map, hidden, total, cin, kFwLD, kWgRows);
   if (e != cudaSuccess) return e;
-  kernel<<<unsigned(parts * blocks), kWgThreads, smem, stream>>>(dz_map, hidden_map, dz, hidden, partials, total, full_rows,
-                                                                q, cin, cout, boxes);
+  kernel<<<unsigned(parts * blocks), kWgThreads, smem, stream>>>(dz_map, hidden_map, dz, hidden, dw_parts, db_parts, total,
+                                                                full_rows, q, cin, cout, boxes);
   return cudaGetLastError();
 }
 
 template <int DIM, bool ACT>
 cudaError_t backward(const double* hidden, const double* weight, const double* activated, const double* aux,
                      const double* seed, double* dh, double* dw, double* db, double* scratch, const BackPlan& plan,
-                     Packed rows, int cin, int cout, int sms, cudaStream_t stream) {
+                     Packed rows, int cin, int cout, cudaStream_t stream) {
   constexpr int Q = Jet<DIM>::Q;
   const int64_t total = rows.full * Q + rows.value;
-  double *dz = plan.dz ? scratch : nullptr, *partials = scratch + plan.dz;
+  double *dz = plan.dz ? scratch : nullptr, *dw_parts = scratch + plan.dz, *db_parts = dw_parts + plan.dw;
   cudaError_t e = cudaSuccess;
   if (plan.fused) {
-    e = launch_backward_tile<DIM, ACT, 4, true>(hidden, weight, activated, aux, seed, dz, dh, partials, plan.parts, rows, cin,
-                                                cout, sms, stream);
+    e = launch_backward_tile<DIM, ACT, 4, true>(hidden, weight, activated, aux, seed, dz, dh, dw_parts, db_parts, plan.parts,
+                                                rows, cin, cout, stream);
   } else {
     const double* z = ACT ? dz : seed;
     if (plan.tiled) {
-      e = launch_backward_tile<DIM, ACT, 8, false>(hidden, weight, activated, aux, seed, dz, dh, partials, plan.parts, rows,
-                                                   cin, cout, sms, stream);
+      e = launch_backward_tile<DIM, ACT, 8, false>(hidden, weight, activated, aux, seed, dz, dh, dw_parts, db_parts,
+                                                   plan.bias_parts, rows, cin, cout, stream);
     } else {
       if constexpr (ACT) {
         affine_seed<DIM><<<grid_for(rows.units<Q>() * cout), kAffThreads, 0, stream>>>(activated, aux, seed, dz, rows, cout);
@@ -1075,12 +1100,12 @@ cudaError_t backward(const double* hidden, const double* weight, const double* a
     }
     if (e != cudaSuccess) return e;
     const auto wgrad = cin <= 64 ? launch_wgrad<1, 2> : cout <= 64 ? launch_wgrad<1, 4> : launch_wgrad<2, 4>;
-    e = wgrad(z, hidden, partials, plan.parts, total, rows.full * Q, Q, cin, cout, stream);
+    e = wgrad(z, hidden, dw_parts, plan.tiled ? nullptr : db_parts, plan.parts, total, rows.full * Q, Q, cin, cout, stream);
   }
   if (e != cudaSuccess) return e;
-  const int64_t nw = int64_t(cin) * cout, n = nw + cout;
-  return launch_dependent(affine_finish, unsigned((n + kFinLanes - 1) / kFinLanes), kFinStrands * kFinLanes, 0, stream,
-                          partials, int(plan.parts), dw, db, nw, n);
+  const int64_t nw = int64_t(cin) * cout;
+  return launch_dependent(affine_finish, unsigned((nw + cout + kFinLanes - 1) / kFinLanes), kFinStrands * kFinLanes, 0, stream,
+                          dw_parts, int(plan.parts), db_parts, int(plan.bias_parts), dw, db, nw, cout);
 }
 
 }  // namespace
@@ -1155,7 +1180,7 @@ int flashns_b200_affine_vjp(int dim, int activation, const double* hidden, const
   if (scratch_bytes < size_t(plan.doubles) * sizeof(double)) return int(cudaErrorInvalidValue);
   const auto run = dim == 2 ? (activation ? backward<2, true> : backward<2, false>)
                             : (activation ? backward<3, true> : backward<3, false>);
-  return int(run(hidden, weight, activated, aux, seed, d_hidden, d_weight, d_bias, scratch, plan, rows, cin, cout, sms,
+  return int(run(hidden, weight, activated, aux, seed, d_hidden, d_weight, d_bias, scratch, plan, rows, cin, cout,
                  stream));
 }
 
