@@ -377,15 +377,13 @@ __global__ void __launch_bounds__(2 * kTileGroup, 1)
     for (int k = 0; k < planes; ++k) tma_load_2d(tile_at + k * PLANE, &hidden, k * kFwKC, int(tile * RT), bars + group);
   };
 
-  load_rows(sw, ldw, weight, c0, CB, cout, cin, vec_w, tid >> 5, 16, lane);
-  cp_async_commit();
-  if (tid == 0) {
-    mbar_init(bars, 1);
-    mbar_init(bars + 1, 1);
-  }
-  cp_async_wait<0>();
+  if (gt == 0) mbar_init(bars + group, 1);
   __syncthreads();
   if (gt == 0 && first < tiles) load(first);
+  load_rows(sw, ldw, weight, c0, CB, cout, cin, vec_w, tid >> 5, 16, lane);
+  cp_async_commit();
+  cp_async_wait<0>();
+  __syncthreads();
 
   const int ch = wc * 16 + 2 * g, c = c0 + ch;  // this thread's channels c, c + 1
   const double b0 = bias && c < cout ? bias[c] : 0.0, b1 = bias && c + 1 < cout ? bias[c + 1] : 0.0;
@@ -561,7 +559,7 @@ __global__ void __launch_bounds__(2 * kTileGroup, 1)
                          const double* __restrict__ weight, const double* __restrict__ activated,
                          const double* __restrict__ aux, const double* __restrict__ seed, double* __restrict__ dz,
                          double* __restrict__ dh, double* __restrict__ dw_parts, double* __restrict__ db_parts, Packed rows,
-                         int cin, int cout, bool boxes, bool vec_out) {
+                         int cin, int cout, bool boxes, bool vec_out, bool vec_w) {
   constexpr int Q = Jet<DIM>::Q, RT = tile_rows(WC), CB = 16 * WC, LD = kFwLD, PLANE = RT * LD, LDW = CB + 4;
   constexpr int NT = RT * WC / 64, UT = RT / Q, PAIRS = UT * CB / kTileGroup;  // n8 tiles a warp; jets a thread
   constexpr bool SWAP = FUSED && ACT;  // A first, then H in its place
@@ -685,19 +683,29 @@ __global__ void __launch_bounds__(2 * kTileGroup, 1)
     }
   };
 
-  for (int e = tid; e < c8 * CB; e += 2 * kTileGroup) {  // W rows c, columns i0 .. i0 + CB - 1
-    const int c = e / CB, i = e % CB;
-    const bool ok = c < cout && i0 + i < cin;
-    cp_async8(sw + c * LDW + i, ok ? weight + int64_t(c) * cin + i0 + i : weight, ok);
-  }
-  cp_async_commit();
   if (gt == 0) {
     mbar_init(bar, 1);
     mbar_init(bar_h, 1);
   }
-  cp_async_wait<0>();
   __syncthreads();
   if (first < tiles) request(first);
+  for (int c = tid >> 5; c < c8; c += 2 * kTileGroup / 32) {  // W rows c, columns i0 .. i0 + CB - 1
+    const double* from = weight + int64_t(c) * cin + i0;
+    if (vec_w) {
+      for (int i = 2 * lane; i < CB; i += 64) {
+        const bool ok = c < cout && i0 + i < cin;
+        cp_async16(sw + c * LDW + i, ok ? from + i : weight, ok);
+      }
+    } else {
+      for (int i = lane; i < CB; i += 32) {
+        const bool ok = c < cout && i0 + i < cin;
+        cp_async8(sw + c * LDW + i, ok ? from + i : weight, ok);
+      }
+    }
+  }
+  cp_async_commit();
+  cp_async_wait<0>();
+  __syncthreads();
 
   const int ci = i0 + wc * 16 + 2 * g;  // this thread's input channels ci, ci + 1
   const double* ap = sw + t * LDW + wc * 16 + 2 * g;
@@ -1050,7 +1058,8 @@ cudaError_t launch_backward_tile(const double* hidden, const double* weight, con
   if (e != cudaSuccess) return e;
   const bool vec_out = cin % 2 == 0 && aligned16(dh);
   kernel<<<unsigned(per * blocks), 2 * kTileGroup, smem, stream>>>(maps, hidden, weight, activated, aux, seed, dz, dh,
-                                                                  dw_parts, db_parts, rows, cin, cout, boxes, vec_out);
+                                                                  dw_parts, db_parts, rows, cin, cout, boxes, vec_out,
+                                                                  cin % 2 == 0 && aligned16(weight));
   return cudaGetLastError();
 }
 
