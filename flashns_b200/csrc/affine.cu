@@ -549,6 +549,10 @@ constexpr size_t back_smem(int wc, bool fused, int cin, int cout) {
                            size_t((cout + 7) / 8 * 8) * (16 * wc + 4) + 4);
 }
 
+// The turn passes this many 8-row steps of dW (fused) or 8-channel steps of dH before a group's
+// last MMAs: the partner's VJP begins behind them.
+constexpr int kEarlyRows = 6, kEarlySteps = 6;
+
 struct BackMaps {
   CUtensorMap seed, activated, hidden;
 };
@@ -722,6 +726,7 @@ __global__ void __launch_bounds__(2 * kTileGroup, 1)
   const double* wa = z_at + wz / kFwKC * PLANE + t * LD + wz % kFwKC + g;
   const double* wb = h_at + wh * PLANE + t * LD + g;
   const Turns<2, kTileGroup> turns(group);
+  const int early = c8 / 8 > kEarlySteps ? c8 / 8 - kEarlySteps : 0;
   unsigned phase = 0;
   bool dead = false, late = false;  // a copy's bounded wait gave up: the group keeps the turns and does no work
   for (int64_t tile = first; tile < tiles; tile += 2 * per) {
@@ -755,6 +760,7 @@ __global__ void __launch_bounds__(2 * kTileGroup, 1)
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           if (k >= left) break;
+          if (!FUSED && 4 * p + k == early) turns.pass();
           const double2 lo = *reinterpret_cast<const double2*>(a_at + 8 * k * LDW);
           const double2 hi = *reinterpret_cast<const double2*>(a_at + (8 * k + 4) * LDW);
           const double a[4] = {lo.x, lo.y, hi.x, hi.y};
@@ -772,16 +778,18 @@ __global__ void __launch_bounds__(2 * kTileGroup, 1)
         if (late) atomicExch(&g_affine_fault, 1);
       }
     }
+    if (!FUSED && !(!dead && has_h)) turns.pass();
+    if (FUSED && !(!dead && !late && has_w)) turns.pass();
     if (!dead && !late && has_w) {
 #pragma unroll
       for (int r = 0; r < RT; r += 8) {
+        if (r == RT - 8 * kEarlyRows) turns.pass();
         const double a[4] = {wa[r * LD], wa[r * LD + 8], wa[(r + 4) * LD], wa[(r + 4) * LD + 8]};
 #pragma unroll
         for (int j = 0; j < WN; ++j) mma_m16n8k8(wacc[j], a, wb[r * LD + 8 * j], wb[(r + 4) * LD + 8 * j]);
       }
     }
     phase ^= 1;
-    turns.pass();
     named_sync(1 + group, kTileGroup);  // every warp has read dZ and H
     const int64_t next = tile + 2 * per;
     store_dz(tile);
