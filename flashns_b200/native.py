@@ -23,11 +23,11 @@ def _ptr(t):
 def _launch(name, args, tensors):
     """One call on the current stream of ``tensors[0]``'s device.  ``tensors``: what must outlive the
     launch where it came from another stream (tensors allocated for this call need not be named)."""
-    lib = _lib.library()
+    call = getattr(_lib.library(), name)
     index = tensors[0].get_device()
     with torch.cuda.device(index):
         stream = torch.cuda.current_stream(index)
-        status = getattr(lib, name)(*args, stream.cuda_stream)
+        status = call(*args, stream.cuda_stream)
         for t in tensors:
             if t is not None and t.numel():
                 t.record_stream(stream)
@@ -36,13 +36,13 @@ def _launch(name, args, tensors):
 
 
 def _check(tensors):
-    device = tensors[0].device
+    index, differentiable = tensors[0].get_device(), torch.is_grad_enabled()
     for t in tensors:
-        if not t.is_cuda or t.dtype != torch.float64 or t.device != device:
+        if t.get_device() != index or not t.is_cuda or t.dtype is not torch.float64:
             raise ValueError("same-device CUDA FP64 tensors required")
         if not t.is_contiguous():
             raise ValueError("contiguous tensors required")
-        if torch.is_grad_enabled() and t.requires_grad:
+        if differentiable and t.requires_grad:
             raise NotImplementedError("manual parameter VJP; double backward/HVP unsupported")
 
 
