@@ -180,10 +180,11 @@ __device__ __forceinline__ void forward_store(double (&h0)[Jet<DIM>::Q], double 
 
 // eight input channels of a tile: A rows ap and ap + ldw, B columns of n8 tile j at row 2 j
 template <int NT>
-__device__ __forceinline__ void forward_step(double (&acc)[NT][4], const double* ap, int ldw, const double* bp) {
+__device__ __forceinline__ void forward_step(double (&acc)[NT][4], const double* ap, int ldw, const double* bp,
+                                             int ld = kFwLD) {
   const double a[4] = {ap[0], ap[ldw], ap[4], ap[ldw + 4]};
 #pragma unroll
-  for (int j = 0; j < NT; ++j) mma_m16n8k8(acc[j], a, bp[2 * j * kFwLD], bp[2 * j * kFwLD + 4]);
+  for (int j = 0; j < NT; ++j) mma_m16n8k8(acc[j], a, bp[2 * j * ld], bp[2 * j * ld + 4]);
 }
 
 // The groups' turns on the tensor pipe: group g runs a tile's MMAs between take and pass, after
@@ -330,8 +331,12 @@ constexpr int kTileGroup = 256, kTileSmem = 227 * 1024;
 constexpr int tile_rows(int wc) { return 320 / wc; }
 __host__ __device__ constexpr int tile_planes(int cin) { return (cin + kFwKC - 1) / kFwKC; }
 __host__ __device__ constexpr int tile_ldw(int cin) { return (cin + 7) / 8 * 8 + 2; }  // 2 (mod 8)
+// a tile's rows: whole planes of 32 channels, then the rest, to 8, with its own padding (12, 20,
+// 28 or 36 doubles are all 4 or 12 (mod 16))
+__host__ __device__ constexpr int tail_ld(int cin) { return cin % kFwKC ? (cin % kFwKC + 7) / 8 * 8 + 4 : 0; }
+__host__ __device__ constexpr int tile_width(int cin) { return cin / kFwKC * kFwLD + tail_ld(cin); }
 constexpr size_t tile_smem(int wc, int cin) {
-  return sizeof(double) * (2 * size_t(tile_rows(wc)) * tile_planes(cin) * kFwLD + size_t(16 * wc) * tile_ldw(cin) + 2);
+  return sizeof(double) * (2 * size_t(tile_rows(wc)) * tile_width(cin) + size_t(16 * wc) * tile_ldw(cin) + 2);
 }
 
 // rows r0 .. r0 + count - 1 (zeros from `total` on) and columns 0 .. cin8 - 1 (zeros past cin)
@@ -350,9 +355,25 @@ __device__ __forceinline__ void load_rows(double* dst, int ld, const double* __r
   }
 }
 
+struct TileMaps {
+  CUtensorMap planes, tail;
+};
+
+// A 3-D unit's two blocks lie with neighbouring threads, each with ten rows of two channels;
+// they trade, and each goes on with one channel's twenty rows.
+__device__ __forceinline__ void trade_blocks(const double (&acc)[5][4], int t, double (&z)[20]) {
+#pragma unroll
+  for (int s = 0; s < 10; ++s) {
+    const double first = acc[s >> 1][s & 1], second = acc[s >> 1][2 + (s & 1)];
+    const double got = __shfl_xor_sync(0xffffffffu, t & 1 ? first : second, 1);
+    z[s] = t & 1 ? got : first;
+    z[10 + s] = t & 1 ? second : got;
+  }
+}
+
 template <int DIM, bool ACT, int WC>
 __global__ void __launch_bounds__(2 * kTileGroup, 1)
-    affine_forward_tile(const __grid_constant__ CUtensorMap hidden, const double* __restrict__ weight,
+    affine_forward_tile(const __grid_constant__ TileMaps hidden, const double* __restrict__ weight,
                         const double* __restrict__ bias, const double* __restrict__ residual, double* __restrict__ out,
                         double* __restrict__ activated, double* __restrict__ aux, Packed rows, int cin, int cout,
                         bool vec_w, bool vec_out) {
@@ -368,13 +389,14 @@ __global__ void __launch_bounds__(2 * kTileGroup, 1)
   const int64_t per = gridDim.x / blocks, total = rows.full * Q + rows.value;
   const int64_t tiles = (total + RT - 1) / RT, first = blockIdx.x / blocks + group * per;
   const auto count = [&](int64_t from) { return from < tiles ? (tiles - 1 - from) / (2 * per) + 1 : 0; };
-  const int planes = tile_planes(cin), ldw = tile_ldw(cin), ks = (cin + 7) / 8;
-  double *tile_at = smem + group * planes * PLANE, *sw = smem + 2 * planes * PLANE;
+  const int planes = cin / kFwKC, ldt = tail_ld(cin), ldw = tile_ldw(cin), size = RT * tile_width(cin);
+  double *tile_at = smem + group * size, *sw = smem + 2 * size;
   uint64_t* bars = reinterpret_cast<uint64_t*>(sw + CB * ldw);
   auto load = [&](int64_t tile) {  // by one thread, once every warp has read the last tile
     fence_proxy_async();
-    mbar_arrive_expect_tx(bars + group, unsigned(planes * PLANE * sizeof(double)));
-    for (int k = 0; k < planes; ++k) tma_load_2d(tile_at + k * PLANE, &hidden, k * kFwKC, int(tile * RT), bars + group);
+    mbar_arrive_expect_tx(bars + group, unsigned(size * sizeof(double)));
+    for (int k = 0; k < planes; ++k) tma_load_2d(tile_at + k * PLANE, &hidden.planes, k * kFwKC, int(tile * RT), bars + group);
+    if (ldt) tma_load_2d(tile_at + planes * PLANE, &hidden.tail, planes * kFwKC, int(tile * RT), bars + group);
   };
 
   if (gt == 0) mbar_init(bars + group, 1);
@@ -386,8 +408,9 @@ __global__ void __launch_bounds__(2 * kTileGroup, 1)
   __syncthreads();
 
   const int ch = wc * 16 + 2 * g, c = c0 + ch;  // this thread's channels c, c + 1
-  const double b0 = bias && c < cout ? bias[c] : 0.0, b1 = bias && c + 1 < cout ? bias[c + 1] : 0.0;
-  const double *ap = sw + ch * ldw + t, *bp = tile_at + (wr * 40 + (g >> 1) * 10 + (g & 1)) * LD + t;
+  const double b0 = c < cout ? bias[c] : 0.0, b1 = c + 1 < cout ? bias[c + 1] : 0.0;
+  const int brow = wr * 40 + (g >> 1) * 10 + (g & 1);
+  const double *ap = sw + ch * ldw + t, *bp = tile_at + brow * LD + t;
   const Turns<2, kTileGroup> turns(group);
   unsigned phase = 0;
   bool dead = false;  // a copy's bounded wait gave up: the group keeps the turns and does no work
@@ -413,29 +436,80 @@ __global__ void __launch_bounds__(2 * kTileGroup, 1)
     }
     phase ^= 1;
     turns.take();
-    if (!dead) {
+    if (!dead && c0 + wc * 16 < cout) {
       for (int p = 0; p < planes; ++p) {
-        const double *a_at = ap + p * kFwKC, *b_at = bp + p * PLANE;
-        const int left = ks - 4 * p;
-        if (left >= 4) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) forward_step<NT>(acc, a_at + 8 * k, ldw, b_at + 8 * k);
-        } else {
-#pragma unroll 1
-          for (int k = 0; k < left; ++k) forward_step<NT>(acc, a_at + 8 * k, ldw, b_at + 8 * k);
-        }
+        for (int k = 0; k < 4; ++k) forward_step<NT>(acc, ap + p * kFwKC + 8 * k, ldw, bp + p * PLANE + 8 * k);
       }
+      const double* tail = tile_at + planes * PLANE + brow * ldt + t;
+#pragma unroll 1
+      for (int k = 0; k < ldt / 8; ++k) forward_step<NT>(acc, ap + planes * kFwKC + 8 * k, ldw, tail + 8 * k, ldt);
     }
-    const int64_t u = (tile * RT + wr * 40 + t * 10) / Q;
-    const bool live = !dead && u * Q < total && c < cout;
+    const bool more = tile + 2 * per < tiles && !dead;
     if constexpr (DIM == 2) {
+      const int64_t u = tile * (RT / Q) + wr * 4 + t;
+      const bool live = !dead && u * Q < total && c < cout;
       double h0[Q], h1[Q];
       if (live) forward_jets<DIM, ACT>(acc, b0, b1, u, c, rows, cout, aux, c + 1 < cout, h0, h1);
       __syncwarp();
       turns.pass();
       named_sync(1 + group, kTileGroup);  // every warp has read the tile
-      if (gt == 0 && tile + 2 * per < tiles && !dead) load(tile + 2 * per);
+      if (gt == 0 && more) load(tile + 2 * per);
       if (live) forward_store<DIM>(h0, h1, u, c, rows, cout, residual, out, activated, vec_out, c + 1 < cout);
+    } else {
+      const int64_t u = tile * (RT / Q) + wr * 2 + (t >> 1), row = u * Q;
+      const int cc = c + (t & 1);
+      const bool live = !dead && row < total && cc < cout, full = u < rows.full;
+      const int n = live ? rows.count<Q>(u) : 0;
+      double z[Q];
+      trade_blocks(acc, t, z);
+      if (live) {
+        const double b = t & 1 ? b1 : b0;
+#pragma unroll
+        for (int s = 0; s < Q; ++s) z[s] += s == 0 || !full ? b : 0.0;
+        if constexpr (ACT) {
+          double a1;
+          if (full) {
+            tanh_forward<DIM>(z, z, a1);
+            if (aux) aux[u * cout + cc] = a1;
+          } else {
+            double* ax = aux ? aux + (rows.full + (u - rows.full) * Q) * cout + cc : nullptr;
+#pragma unroll
+            for (int s = 0; s < Q; ++s) {
+              jet_fwd_2d0(z + s, z + s, a1);
+              if (ax && s < n) ax[int64_t(s) * cout] = a1;
+            }
+          }
+        }
+      }
+      __syncwarp();
+      turns.pass();
+      named_sync(1 + group, kTileGroup);
+      if (gt == 0 && more) load(tile + 2 * per);
+      if (live) {
+        const int64_t step = opaque(cout);
+        double* to = out + row * cout + cc;
+        if (activated) {
+          double* also = activated + row * cout + cc;
+#pragma unroll
+          for (int s = 0; s < Q; ++s, also += step)
+            if (s < n) *also = z[s];
+        }
+        if (residual) {
+          const double* from = residual + row * cout + cc;
+#pragma unroll
+          for (int half = 0; half < Q; half += 10) {  // ten rows requested at once
+            double r[10];
+#pragma unroll
+            for (int s = 0; s < 10; ++s, from += step) r[s] = half + s < n ? *from : 0.0;
+#pragma unroll
+            for (int s = 0; s < 10; ++s) z[half + s] += r[s];
+          }
+        }
+#pragma unroll
+        for (int s = 0; s < Q; ++s, to += step)
+          if (s < n) *to = z[s];
+      }
     }
     __syncwarp();
   }
@@ -474,14 +548,15 @@ cudaError_t launch_forward_tile(const double* hidden, const double* weight, cons
   const int64_t blocks = (int64_t(cout) + 16 * WC - 1) / (16 * WC), total = rows.full * Jet<DIM>::Q + rows.value;
   const int64_t tiles = (total + tile_rows(WC) - 1) / tile_rows(WC);
   int sms = 0;
-  CUtensorMap map;
+  TileMaps maps{};
   cudaError_t e = sm_count(&sms);
   if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
-  if (e == cudaSuccess) e = matrix_map(&map, hidden, total, cin, kFwLD, tile_rows(WC));
+  if (e == cudaSuccess && cin >= kFwKC) e = matrix_map(&maps.planes, hidden, total, cin, kFwLD, tile_rows(WC));
+  if (e == cudaSuccess && cin % kFwKC) e = matrix_map(&maps.tail, hidden, total, cin, tail_ld(cin), tile_rows(WC));
   if (e != cudaSuccess) return e;
   const int64_t most = sms / blocks > 0 ? sms / blocks : 1, per = tiles < most ? tiles : most;
   const bool vec_out = cout % 2 == 0 && aligned16(out) && aligned16(residual) && aligned16(activated);
-  kernel<<<unsigned(per * blocks), 2 * kTileGroup, smem, stream>>>(map, weight, bias, residual, out, activated, aux, rows,
+  kernel<<<unsigned(per * blocks), 2 * kTileGroup, smem, stream>>>(maps, weight, bias, residual, out, activated, aux, rows,
                                                                   cin, cout, aligned16(weight), vec_out);
   return cudaGetLastError();
 }
@@ -489,9 +564,9 @@ cudaError_t launch_forward_tile(const double* hidden, const double* weight, cons
 // W's block beside as many groups and stages as 227 KB hold
 template <int DIM, bool ACT, typename... Args>
 cudaError_t forward(int cin, int cout, bool boxes, Args... args) {
+  if (boxes && cout <= 64 && tile_smem(4, cin) <= kTileSmem) return launch_forward_tile<DIM, ACT, 4>(args...);
+  if (boxes && cout > 64 && tile_smem(8, cin) <= kTileSmem) return launch_forward_tile<DIM, ACT, 8>(args...);
   if constexpr (DIM == 2) {
-    if (boxes && cout <= 64 && tile_smem(4, cin) <= kTileSmem) return launch_forward_tile<2, ACT, 4>(args...);
-    if (boxes && tile_smem(8, cin) <= kTileSmem) return launch_forward_tile<2, ACT, 8>(args...);
     if (cin <= 160) return launch_forward<2, ACT, 4, 4, 3, false>(args...);
     if (cin <= 256) return launch_forward<2, ACT, 4, 4, 2, false>(args...);
     return launch_forward<2, ACT, 4, 4, 2, true>(args...);
