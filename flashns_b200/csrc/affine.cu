@@ -192,11 +192,11 @@ __device__ __forceinline__ void forward_step(double (&acc)[NT][4], const double*
 // predecessor arriving; the last group opens the ring with one arrival, and a group whose
 // predecessor arrived once more than it synced closes with one more sync (tiles are dealt in
 // turn, so the groups' counts differ by at most one).
-template <int NG, int THREADS>
+template <int NG, int THREADS, bool TURNS = true>
 struct Turns {
   int g;
   __device__ explicit Turns(int group) : g(group) {
-    if (g == NG - 1) named_arrive(1 + NG, 2 * THREADS);
+    if (TURNS && g == NG - 1) named_arrive(1 + NG, 2 * THREADS);
   }
   __device__ void take() const { named_sync(1 + NG + g, 2 * THREADS); }
   __device__ void pass() const { named_arrive(1 + NG + (g + 1) % NG, 2 * THREADS); }
@@ -206,7 +206,60 @@ struct Turns {
   }
 };
 
-template <int DIM, bool ACT, int NG, int GW, int NS, bool STREAM>
+// Ten value rows from `row` on, channels c and c + 1, where there are no full points: two rows a
+// round, the accumulators moving up, so that the loop holds four tanhs and not twenty (the
+// unrolled form waits for instructions).
+template <bool ACT>
+__device__ __forceinline__ void forward_values(double (&acc)[5][4], double b0, double b1, int64_t row, int64_t total, int c,
+                                               int cout, const double* __restrict__ residual, double* __restrict__ out,
+                                               double* __restrict__ activated, double* __restrict__ aux, bool vec) {
+  const bool two = c + 1 < cout;
+  int64_t at = row * cout + c;
+#pragma unroll 1
+  for (int j = 0; j < 5; ++j, row += 2, at += 2 * int64_t(cout)) {
+    double h[4] = {acc[0][0] + b0, acc[0][2] + b1, acc[0][1] + b0, acc[0][3] + b1}, a[4];  // (row, channel)
+#pragma unroll
+    for (int i = 0; i + 1 < 5; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[i][e] = acc[i + 1][e];
+    double2 r[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      r[e] = make_double2(0.0, 0.0);
+      if (residual && row + e < total) {
+        const double* from = residual + at + e * int64_t(cout);
+        if (vec) r[e] = *reinterpret_cast<const double2*>(from);
+        else r[e] = make_double2(from[0], two ? from[1] : 0.0);
+      }
+    }
+    if constexpr (ACT) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) jet_fwd_2d0(h + i, h + i, a[i]);
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      if (row + e >= total) break;
+      const int64_t i = at + e * int64_t(cout);
+      const double y0 = residual ? h[2 * e] + r[e].x : h[2 * e], y1 = residual ? h[2 * e + 1] + r[e].y : h[2 * e + 1];
+      if (vec) {
+        if (activated) *reinterpret_cast<double2*>(activated + i) = make_double2(h[2 * e], h[2 * e + 1]);
+        if (ACT && aux) *reinterpret_cast<double2*>(aux + i) = make_double2(a[2 * e], a[2 * e + 1]);
+        *reinterpret_cast<double2*>(out + i) = make_double2(y0, y1);
+      } else {
+        if (activated) activated[i] = h[2 * e];
+        if (ACT && aux) aux[i] = a[2 * e];
+        out[i] = y0;
+        if (two) {
+          if (activated) activated[i + 1] = h[2 * e + 1];
+          if (ACT && aux) aux[i + 1] = a[2 * e + 1];
+          out[i + 1] = y1;
+        }
+      }
+    }
+  }
+}
+
+template <int DIM, bool ACT, int NG, int GW, int NS, bool STREAM, bool VALUES, bool TURNS>
 __global__ void __launch_bounds__(NG* GW * 32, 1)
     affine_forward(const double* __restrict__ hidden, const double* __restrict__ weight, const double* __restrict__ bias,
                    const double* __restrict__ residual, double* __restrict__ out, double* __restrict__ activated,
@@ -272,7 +325,7 @@ __global__ void __launch_bounds__(NG* GW * 32, 1)
   const int ch = wc * 16 + 2 * g, c = c0 + ch;  // this thread's channels c, c + 1
   const double b0 = bias && c < cout ? bias[c] : 0.0, b1 = bias && c + 1 < cout ? bias[c + 1] : 0.0;
   double acc[NT][4];
-  const Turns<NG, GT> turns(group);
+  const Turns<NG, GT, TURNS> turns(group);
   int stage = 0;
   for (int64_t tile = first; tile < tiles; tile += tile_step) {
 #pragma unroll
@@ -291,7 +344,7 @@ __global__ void __launch_bounds__(NG* GW * 32, 1)
       cp_async_wait<NS - 2>();
       named_sync(1 + group, GT);  // the chunk is there, the stage loaded next is read out
       load();
-      if (kc == 0) turns.take();
+      if (TURNS && kc == 0) turns.take();
       const double* bp = ring + stage * UT * US + (wr * 4 + (g >> 1)) * US + (g & 1) * kFwLD + t;
       const double* ap = sw + (STREAM ? stage * kFwCB * ldw : kc * KC) + ch * ldw + t;
       const int left = cin - kc * KC;
@@ -304,15 +357,22 @@ __global__ void __launch_bounds__(NG* GW * 32, 1)
       }
       stage = stage + 1 == NS ? 0 : stage + 1;
     }
-    turns.pass();
+    if (TURNS) turns.pass();
     const int64_t u = tile * UT + wr * 4 + t;
-    const bool live = u < units && c < cout;
-    double h0[Q], h1[Q];
-    if (live) forward_jets<DIM, ACT>(acc, b0, b1, u, c, rows, cout, aux, c + 1 < cout, h0, h1);
-    if (live) forward_store<DIM>(h0, h1, u, c, rows, cout, residual, out, activated, vec_out, c + 1 < cout);
+    if constexpr (VALUES) {
+      if (u * Q < total && c < cout)
+        forward_values<ACT>(acc, b0, b1, u * Q, total, c, cout, residual, out, activated, aux, vec_out);
+    } else {
+      const bool live = u < units && c < cout;
+      double h0[Q], h1[Q];
+      if (live) {
+        forward_jets<DIM, ACT>(acc, b0, b1, u, c, rows, cout, aux, c + 1 < cout, h0, h1);
+        forward_store<DIM>(h0, h1, u, c, rows, cout, residual, out, activated, vec_out, c + 1 < cout);
+      }
+    }
     __syncwarp();
   }
-  turns.close(mine, count(blockIdx.x / blocks + (group + NG - 1) % NG * per));
+  if (TURNS) turns.close(mine, count(blockIdx.x / blocks + (group + NG - 1) % NG * per));
   cp_async_wait<0>();
 }
 
@@ -518,11 +578,11 @@ __global__ void __launch_bounds__(2 * kTileGroup, 1)
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-template <int DIM, bool ACT, int NG, int GW, int NS, bool STREAM>
+template <int DIM, bool ACT, int NG, int GW, int NS, bool STREAM, bool VALUES = false, bool TURNS = true>
 cudaError_t launch_forward(const double* hidden, const double* weight, const double* bias, const double* residual,
                            double* out, double* activated, double* aux, Packed rows, int cin, int cout,
                            bool across, cudaStream_t stream) {
-  const auto kernel = affine_forward<DIM, ACT, NG, GW, NS, STREAM>;
+  const auto kernel = affine_forward<DIM, ACT, NG, GW, NS, STREAM, VALUES, TURNS>;
   const size_t smem = fw_smem<DIM, NG, GW, NS, STREAM>(cin);
   int sms = 0;
   cudaError_t e = sm_count(&sms);
@@ -533,7 +593,7 @@ cudaError_t launch_forward(const double* hidden, const double* weight, const dou
   const int64_t tiles = (rows.units<Jet<DIM>::Q>() + GW - 1) / GW;
   const int64_t most = sms / blocks > 0 ? sms / blocks : 1, per = tiles < most ? tiles : most;
   const bool vec_in = cin % 2 == 0 && aligned16(hidden) && aligned16(weight);
-  const bool vec_out = cout % 2 == 0 && aligned16(out) && aligned16(residual) && aligned16(activated);
+  const bool vec_out = cout % 2 == 0 && aligned16(out) && aligned16(residual) && aligned16(activated) && aligned16(aux);
   kernel<<<unsigned(per * blocks), NG * GW * 32, smem, stream>>>(hidden, weight, bias, residual, out, activated, aux,
                                                                  rows, cin, cout, vec_in, vec_out, across);
   return cudaGetLastError();
@@ -555,7 +615,7 @@ cudaError_t launch_forward_tile(const double* hidden, const double* weight, cons
   if (e == cudaSuccess && cin % kFwKC) e = matrix_map(&maps.tail, hidden, total, cin, tail_ld(cin), tile_rows(WC));
   if (e != cudaSuccess) return e;
   const int64_t most = sms / blocks > 0 ? sms / blocks : 1, per = tiles < most ? tiles : most;
-  const bool vec_out = cout % 2 == 0 && aligned16(out) && aligned16(residual) && aligned16(activated);
+  const bool vec_out = cout % 2 == 0 && aligned16(out) && aligned16(residual) && aligned16(activated) && aligned16(aux);
   kernel<<<unsigned(per * blocks), 2 * kTileGroup, smem, stream>>>(maps, weight, bias, residual, out, activated, aux, rows,
                                                                   cin, cout, aligned16(weight), vec_out);
   return cudaGetLastError();
@@ -563,7 +623,16 @@ cudaError_t launch_forward_tile(const double* hidden, const double* weight, cons
 
 // W's block beside as many groups and stages as 227 KB hold
 template <int DIM, bool ACT, typename... Args>
-cudaError_t forward(int cin, int cout, bool boxes, Args... args) {
+cudaError_t forward(int cin, int cout, bool values, bool boxes, Args... args) {
+  // tanhs of value rows alone (a point a row: the dimension does not matter) go with the small
+  // groups, without turns: 40,401 rows 64 -> 64 take 27 us, in whole tiles 35
+  if constexpr (ACT) {
+    if (values) {
+      if (cin <= 160) return launch_forward<2, true, 4, 4, 3, false, true, false>(args...);
+      if (cin <= 256) return launch_forward<2, true, 4, 4, 2, false, true, false>(args...);
+      return launch_forward<2, true, 4, 4, 2, true, true, false>(args...);
+    }
+  }
   if (boxes && cout <= 64 && tile_smem(4, cin) <= kTileSmem) return launch_forward_tile<DIM, ACT, 4>(args...);
   if (boxes && cout > 64 && tile_smem(8, cin) <= kTileSmem) return launch_forward_tile<DIM, ACT, 8>(args...);
   if constexpr (DIM == 2) {
@@ -1186,7 +1255,7 @@ cudaError_t backward(const double* hidden, const double* weight, const double* a
       }
       // dH = dZ W: the forward product over the output channels, with W read across
       if (e == cudaSuccess)
-        e = forward<DIM, false>(cout, cin, false, z, weight, static_cast<const double*>(nullptr),
+        e = forward<DIM, false>(cout, cin, false, false, z, weight, static_cast<const double*>(nullptr),
                                 static_cast<const double*>(nullptr), dh, static_cast<double*>(nullptr),
                                 static_cast<double*>(nullptr), rows, cout, cin, true, stream);
     }
@@ -1224,7 +1293,7 @@ int flashns_b200_affine(int dim, int activation, const double* hidden, const dou
     return int(cudaErrorInvalidValue);
   // TMA boxes: rows on 16-byte boundaries, row numbers that fit their 32-bit coordinate
   const bool boxes = cin % 2 == 0 && aligned16(hidden) && count < INT_MAX - 1024;
-  const auto run = [&](auto launch) { return int(launch(cin, cout, boxes, hidden, weight, bias, residual, out, activated, aux, rows, cin, cout, false, stream)); };
+  const auto run = [&](auto launch) { return int(launch(cin, cout, full_points == 0, boxes, hidden, weight, bias, residual, out, activated, aux, rows, cin, cout, false, stream)); };
   if (dim == 2) return activation ? run([](auto... a) { return forward<2, true>(a...); }) : run([](auto... a) { return forward<2, false>(a...); });
   return activation ? run([](auto... a) { return forward<3, true>(a...); }) : run([](auto... a) { return forward<3, false>(a...); });
 }
