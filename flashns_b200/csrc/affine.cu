@@ -1238,7 +1238,9 @@ cudaError_t backward(const double* hidden, const double* weight, const double* a
                      Packed rows, int cin, int cout, cudaStream_t stream) {
   constexpr int Q = Jet<DIM>::Q;
   const int64_t total = rows.full * Q + rows.value;
-  double *dz = plan.dz ? scratch : nullptr, *dw_parts = scratch + plan.dz, *db_parts = dw_parts + plan.dw;
+  const bool whole = plan.parts == 1 && plan.bias_parts == 1;  // a single share is the gradient
+  double *dz = plan.dz ? scratch : nullptr, *dw_parts = whole ? dw : scratch + plan.dz;
+  double* db_parts = whole ? db : scratch + plan.dz + plan.dw;
   cudaError_t e = cudaSuccess;
   if (plan.fused) {
     e = launch_backward_tile<DIM, ACT, 4, true>(hidden, weight, activated, aux, seed, dz, dh, dw_parts, db_parts, plan.parts,
@@ -1263,7 +1265,7 @@ cudaError_t backward(const double* hidden, const double* weight, const double* a
     const auto wgrad = cin <= 64 ? launch_wgrad<1, 2> : cout <= 64 ? launch_wgrad<1, 4> : launch_wgrad<2, 4>;
     e = wgrad(z, hidden, dw_parts, plan.tiled ? nullptr : db_parts, plan.parts, total, rows.full * Q, Q, cin, cout, stream);
   }
-  if (e != cudaSuccess) return e;
+  if (e != cudaSuccess || whole) return e;
   const int64_t nw = int64_t(cin) * cout;
   return launch_dependent(affine_finish, unsigned((nw + cout + kFinLanes - 1) / kFinLanes), kFinStrands * kFinLanes, 0, stream,
                           dw_parts, int(plan.parts), db_parts, int(plan.bias_parts), dw, db, nw, cout);
@@ -1334,6 +1336,8 @@ int flashns_b200_affine_vjp(int dim, int activation, const double* hidden, const
   if (ranges_overlap(d_hidden, in, hidden, in) || ranges_overlap(d_hidden, in, seed, bytes) ||
       ranges_overlap(d_hidden, in, activated, bytes) || ranges_overlap(d_hidden, in, scratch, scratch_bytes))
     return int(cudaErrorInvalidValue);
+  // at least one share of dW and db, whatever the device
+  if (scratch_bytes < (size_t(cin) + 1) * cout * sizeof(double)) return int(cudaErrorInvalidValue);
   int sms = 0;
   const cudaError_t e = sm_count(&sms);
   if (e != cudaSuccess) return int(e);

@@ -111,16 +111,16 @@ __global__ void __launch_bounds__(kNormThreads)
   }
 }
 
-// any width; partials [grid][2][channels]: this block's dgain and dbias
+// any width; gain_parts, bias_parts [grid][channels]: this block's dgain and dbias
 template <int DIM>
 __global__ void __launch_bounds__(kNormThreads)
     norm_backward(const double* __restrict__ x, const double* __restrict__ gain, const double* __restrict__ stats,
                   const double* __restrict__ seed, const double* __restrict__ skip, double* __restrict__ dx,
-                  double* __restrict__ partials, Packed rows, int channels) {
+                  double* __restrict__ gain_parts, double* __restrict__ bias_parts, Packed rows, int channels) {
   constexpr int Q = Jet<DIM>::Q;
   __shared__ double shared[(kNormThreads / 32) * 2 * Q];
-  double* mine = partials + int64_t(blockIdx.x) * 2 * channels;
-  for (int c = threadIdx.x; c < channels; c += blockDim.x) mine[c] = mine[channels + c] = 0.0;
+  double *gains = gain_parts + int64_t(blockIdx.x) * channels, *biases = bias_parts + int64_t(blockIdx.x) * channels;
+  for (int c = threadIdx.x; c < channels; c += blockDim.x) gains[c] = biases[c] = 0.0;
   const int64_t units = rows.units<Q>();
   for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
     const bool full = u < rows.full;
@@ -159,8 +159,8 @@ __global__ void __launch_bounds__(kNormThreads)
         sums[s] += gc * p[s];
         sums[Q + s] += gc * g[s];
       }
-      mine[c] += dgain;
-      mine[channels + c] += dbias;
+      gains[c] += dgain;
+      biases[c] += dbias;
     }
     block_sums(sums, shared);
     if (full) {
@@ -428,7 +428,8 @@ template <typename At>
 __global__ void __launch_bounds__(At::kBlock, 1)
     norm_backward_unit(const double* __restrict__ x, const double* __restrict__ gain, const double* __restrict__ stats,
                        const double* __restrict__ seed, const double* __restrict__ skip, double* __restrict__ dx,
-                       double* __restrict__ partials, Packed rows, int channels, bool vec) {
+                       double* __restrict__ gain_parts, double* __restrict__ bias_parts, Packed rows, int channels,
+                       bool vec) {
   constexpr int DIM = At::kDim, Q = At::Q, K = At::K, L = At::L, TH = At::kThreads;
   extern __shared__ __align__(16) double smem[];
   const At at;
@@ -563,31 +564,32 @@ __global__ void __launch_bounds__(At::kBlock, 1)
     const int which = i / (K * L), c = i % (K * L);
     double s = 0.0;
     for (int q = 0; q < At::kBlock / L; ++q) s += smem[which * K * At::kBlock + q * K * L + c];
-    if (c < channels) partials[(int64_t(blockIdx.x) * 2 + which) * channels + c] = s;
+    if (c < channels) (which ? bias_parts : gain_parts)[int64_t(blockIdx.x) * channels + c] = s;
   }
 }
 
-// dgain, dbias [channels] each from partials [parts][2][channels]: 32 strands of parts a value,
-// each in order, then the strands in order
+// dgain, dbias [channels] each from their [parts][channels]: 32 strands of parts a value, each in
+// order, then the strands in order
 constexpr int kFinishStrands = 32, kFinishLanes = 32;
 __global__ void __launch_bounds__(kFinishStrands* kFinishLanes)
-    norm_finish(const double* __restrict__ partials, int parts, double* __restrict__ dgain, double* __restrict__ dbias,
-                int channels) {
+    norm_finish(const double* __restrict__ gain_parts, const double* __restrict__ bias_parts, int parts,
+                double* __restrict__ dgain, double* __restrict__ dbias, int channels) {
   __shared__ double shared[kFinishStrands][kFinishLanes];
   const int lane = threadIdx.x % kFinishLanes, strand = threadIdx.x / kFinishLanes;
-  const int64_t i = int64_t(blockIdx.x) * kFinishLanes + lane, n = 2 * int64_t(channels);
+  const int64_t i = int64_t(blockIdx.x) * kFinishLanes + lane, c = i < channels ? i : i - channels;
+  const bool live = i < 2 * int64_t(channels);
+  const double* from = (i < channels ? gain_parts : bias_parts) + c;
   double s = 0.0;
   pdl_wait();
-  if (i < n) {
+  if (live) {
 #pragma unroll 8
-    for (int k = strand; k < parts; k += kFinishStrands) s += partials[k * n + i];
+    for (int k = strand; k < parts; k += kFinishStrands) s += from[int64_t(k) * channels];
   }
   shared[strand][lane] = s;
   __syncthreads();
-  if (strand == 0 && i < n) {
+  if (strand == 0 && live) {
     for (int k = 1; k < kFinishStrands; ++k) s += shared[k][lane];
-    if (i < channels) dgain[i] = s;
-    else dbias[i - channels] = s;
+    (i < channels ? dgain : dbias)[c] = s;
   }
 }
 
@@ -616,7 +618,7 @@ bool with_lanes(int channels, bool aligned, const F& f) {
 }
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// blocks of the adjoint, each of which keeps one [2][channels] partial: one a multiprocessor
+// blocks of the adjoint, each of which keeps a [channels] of dgain and of dbias: one a multiprocessor
 // where units are streamed, eight of the small ones elsewhere; at most one a unit
 template <int DIM>
 int64_t norm_parts(Packed rows, int channels, int sms) {
@@ -653,6 +655,8 @@ cudaError_t launch_norm_vjp(const double* x, const double* gain, const double* s
                             const double* skip, double* dx, double* dgain, double* dbias, double* partials, Packed rows,
                             int channels, int sms, cudaStream_t stream) {
   const int parts = int(norm_parts<DIM>(rows, channels, sms));
+  double *gain_parts = dgain, *bias_parts = dbias;  // a single block's sums are the gradients
+  if (parts > 1) gain_parts = partials, bias_parts = partials + int64_t(parts) * channels;
   cudaError_t e = cudaSuccess;
   const bool aligned = aligned16(x) && aligned16(seed) && aligned16(skip);
   const bool done = with_lanes<DIM, true>(channels, aligned, [&](auto place) {
@@ -661,16 +665,17 @@ cudaError_t launch_norm_vjp(const double* x, const double* gain, const double* s
     const int smem = int(sizeof(double)) * At::kGroups * At::kDoubles;
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e == cudaSuccess)
-      kernel<<<parts, At::kBlock, smem, stream>>>(x, gain, stats, seed, skip, dx, partials, rows, channels,
+      kernel<<<parts, At::kBlock, smem, stream>>>(x, gain, stats, seed, skip, dx, gain_parts, bias_parts, rows, channels,
                                                   aligned && channels % 2 == 0);
   });
   if (!done)
-    norm_backward<DIM><<<parts, kNormThreads, 0, stream>>>(x, gain, stats, seed, skip, dx, partials, rows, channels);
+    norm_backward<DIM><<<parts, kNormThreads, 0, stream>>>(x, gain, stats, seed, skip, dx, gain_parts, bias_parts, rows,
+                                                         channels);
   if (e == cudaSuccess) e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
+  if (e != cudaSuccess || parts == 1) return e;
   const unsigned blocks = unsigned((2 * int64_t(channels) + kFinishLanes - 1) / kFinishLanes);
-  return launch_dependent(norm_finish, blocks, kFinishStrands * kFinishLanes, 0, stream, partials, parts, dgain, dbias,
-                          channels);
+  return launch_dependent(norm_finish, blocks, kFinishStrands * kFinishLanes, 0, stream, gain_parts, bias_parts, parts,
+                          dgain, dbias, channels);
 }
 
 }  // namespace

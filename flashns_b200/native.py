@@ -25,14 +25,28 @@ def _launch(name, args, tensors):
     launch where it came from another stream (tensors allocated for this call need not be named)."""
     call = getattr(_lib.library(), name)
     index = tensors[0].get_device()
-    with torch.cuda.device(index):
-        stream = torch.cuda.current_stream(index)
-        status = call(*args, stream.cuda_stream)
-        for t in tensors:
-            if t is not None and t.numel():
-                t.record_stream(stream)
+    if index == torch.cuda.current_device():
+        status = _on_stream(call, args, tensors, index)
+    else:
+        with torch.cuda.device(index):
+            status = _on_stream(call, args, tensors, index)
     if status:
         raise RuntimeError(f"{name} returned CUDA error {status}")
+
+
+_streams = {}  # (device, handle) -> Stream: making the object again costs more than a small launch
+
+
+def _on_stream(call, args, tensors, index):
+    handle = torch._C._cuda_getCurrentRawStream(index)
+    stream = _streams.get((index, handle))
+    if stream is None:
+        stream = _streams[index, handle] = torch.cuda.current_stream(index)
+    status = call(*args, handle)
+    for t in tensors:
+        if t is not None and t.numel():
+            t.record_stream(stream)
+    return status
 
 
 def _check(tensors):
@@ -209,13 +223,13 @@ class NativeCUDA:
         and reciprocal-deviation coefficients for ``layer_norm_vjp``."""
         _check((value, gain, bias))
         layout.check(value)
-        channels = value.shape[1]
+        rows, channels = value.shape
         if gain.shape != (channels,) or bias.shape != (channels,):
             raise ValueError("expected gain[C], bias[C]")
         eps = float(eps)
         if not 0.0 < eps <= 1e300:
             raise ValueError("positive finite eps required")
-        out, stats = torch.empty_like(value), value.new_empty((layout.rows, 2))
+        out, stats = torch.empty_like(value), value.new_empty((rows, 2))
         _launch("flashns_b200_layer_norm", [layout.dimension, *map(_ptr, (value, gain, bias, out, stats)), eps,
                                             layout.full_points, layout.value_points, channels],
                 (value, gain, bias))
@@ -227,8 +241,8 @@ class NativeCUDA:
         given = (value, gain, stats, seed) if skip is None else (value, gain, stats, seed, skip)
         _check(given)
         layout.check(value)
-        channels = value.shape[1]
-        if gain.shape != (channels,) or stats.shape != (layout.rows, 2) or seed.shape != value.shape \
+        rows, channels = value.shape
+        if gain.shape != (channels,) or stats.shape != (rows, 2) or seed.shape != value.shape \
                 or (skip is not None and skip.shape != value.shape):
             raise ValueError("expected X/bar_Y[rows,C], gain[C], stats[rows,2]")
         out, dgain, dbias = torch.empty_like(value), torch.empty_like(gain), torch.empty_like(gain)
@@ -271,19 +285,17 @@ class NativeCUDA:
     def affine_activation_vjp(self, layout, hidden, weight, activated, aux, seed):
         """``(d_hidden, d_weight, d_bias)`` of ``affine_activation`` at ``seed`` (which is the residual's
         gradient too)."""
-        _check((activated, aux, seed))
-        if activated.shape != seed.shape or aux.shape != (layout.points, seed.shape[-1]):
-            raise ValueError("auxiliary/adjoint shape mismatch")
         return self._affine_vjp(layout, hidden, weight, activated, aux, seed)
 
     def _affine_vjp(self, layout, hidden, weight, activated, aux, seed):
         given = (hidden, weight, seed) if activated is None else (hidden, weight, seed, activated, aux)
         _check(given)
         layout.check(hidden)
-        layout.check(seed)
         cout, cin = _affine_shape(hidden, weight)
-        if seed.shape[1] != cout:
+        if seed.shape != (hidden.shape[0], cout):
             raise ValueError("expected H[rows,Cin], W[Cout,Cin], bar_Y[rows,Cout]")
+        if activated is not None and (activated.shape != seed.shape or aux.shape != (layout.points, cout)):
+            raise ValueError("auxiliary/adjoint shape mismatch")
         activation = int(activated is not None)
         out, dw, db = torch.empty_like(hidden), torch.empty_like(weight), weight.new_empty((cout,))
         scratch = _scratch("flashns_b200_affine_vjp_scratch", hidden, layout.dimension, activation,
