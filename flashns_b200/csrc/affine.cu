@@ -266,7 +266,7 @@ __global__ void __launch_bounds__(NG* GW * 32, 1)
                    double* __restrict__ aux, Packed rows, int cin, int cout, bool vec_in, bool vec_out, bool across) {
   constexpr int Q = Jet<DIM>::Q, NT = Q / 2, US = fw_unit_stride<DIM>(), KC = kFwKC;
   constexpr int GT = 32 * GW, UT = GW, RT = UT * Q;  // a group's threads; units and rows of its tile
-  extern __shared__ __align__(16) double smem[];
+  extern __shared__ __align__(128) double smem[];
   const int tid = threadIdx.x, group = tid / GT, gt = tid % GT, wc = (gt >> 5) & 3, wr = gt >> 7;
   const int lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int blocks = (cout + kFwCB - 1) / kFwCB, cb = blockIdx.x % blocks, c0 = cb * kFwCB;
