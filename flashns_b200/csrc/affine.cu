@@ -416,8 +416,46 @@ __device__ __forceinline__ void load_rows(double* dst, int ld, const double* __r
 }
 
 struct TileMaps {
-  CUtensorMap planes, tail;
+  CUtensorMap planes, tail, out, activated;
 };
+
+// How a tile's outputs leave.  A warp's 40 rows x 16 channels go through a box in shared memory
+// and out by TMA: the same bytes as stores of the threads keep the load/store unit busy for
+// 1,400 cycles a tile (5,000 with the residual and a second output), in which the partner's
+// fragment loads, and with them its MMAs, hardly advance.  The boxes have room of their own, or
+// lie in the tile that has been read, whose successor then arrives a little later.
+enum Leave { kByThreads, kInTile, kOwnBoxes };
+constexpr int kBoxDoubles = 40 * 16, kBoxesBytes = 8 * kBoxDoubles * 8;  // a warp's; a group's
+
+// pairs (h0, h1) of rows row + s, channels 2 g, 2 g + 1, in a warp's box
+template <int Q>
+__device__ __forceinline__ void box_pairs(double* box, const double (&h0)[Q], const double (&h1)[Q], int row, int g) {
+#pragma unroll
+  for (int s = 0; s < Q; ++s) {
+    const int r = row + s;
+    *reinterpret_cast<double2*>(box + r * 16 + ((g ^ (r & 7)) << 1)) = make_double2(h0[s], h1[s]);
+  }
+}
+// one channel's rows
+template <int Q>
+__device__ __forceinline__ void box_single(double* box, const double (&z)[Q], int row, int channel) {
+#pragma unroll
+  for (int s = 0; s < Q; ++s) {
+    const int r = row + s;
+    box[r * 16 + (((channel >> 1) ^ (r & 7)) << 1) + (channel & 1)] = z[s];
+  }
+}
+// a warp's box to columns x .., rows y ..; back when the box may be written again
+__device__ __forceinline__ void send_box(const CUtensorMap* map, const double* box, int x, int y, int lane) {
+  fence_proxy_async();
+  __syncwarp();
+  if (lane == 0) {
+    tma_store_2d(map, x, y, box);
+    bulk_commit();
+    bulk_wait_read();
+  }
+  __syncwarp();
+}
 
 // A 3-D unit's two blocks lie with neighbouring threads, each with ten rows of two channels;
 // they trade, and each goes on with one channel's twenty rows.
@@ -433,10 +471,10 @@ __device__ __forceinline__ void trade_blocks(const double (&acc)[5][4], int t, d
 
 template <int DIM, bool ACT, int WC>
 __global__ void __launch_bounds__(2 * kTileGroup, 1)
-    affine_forward_tile(const __grid_constant__ TileMaps hidden, const double* __restrict__ weight,
+    affine_forward_tile(const __grid_constant__ TileMaps maps, const double* __restrict__ weight,
                         const double* __restrict__ bias, const double* __restrict__ residual, double* __restrict__ out,
                         double* __restrict__ activated, double* __restrict__ aux, Packed rows, int cin, int cout,
-                        bool vec_w, bool vec_out) {
+                        bool vec_w, bool vec_out, Leave leave) {
   constexpr int Q = Jet<DIM>::Q, NT = 5, RT = tile_rows(WC), CB = 16 * WC, LD = kFwLD, PLANE = RT * LD;
   extern __shared__ __align__(128) double smem[];
   const int tid = threadIdx.x, group = tid / kTileGroup, gt = tid % kTileGroup, warp = gt >> 5, wc = warp % WC, wr = warp / WC;
@@ -452,11 +490,14 @@ __global__ void __launch_bounds__(2 * kTileGroup, 1)
   const int planes = cin / kFwKC, ldt = tail_ld(cin), ldw = tile_ldw(cin), size = RT * tile_width(cin);
   double *tile_at = smem + group * size, *sw = smem + 2 * size;
   uint64_t* bars = reinterpret_cast<uint64_t*>(sw + CB * ldw);
+  double* box = leave == kOwnBoxes ? sw + CB * ldw + 2 : tile_at;
+  box += (1024 - (smem_u32(box) & 1023)) % 1024 / 8;
+  box += ((leave == kOwnBoxes ? group * 8 : 0) + warp) * kBoxDoubles;
   auto load = [&](int64_t tile) {  // by one thread, once every warp has read the last tile
     fence_proxy_async();
     mbar_arrive_expect_tx(bars + group, unsigned(size * sizeof(double)));
-    for (int k = 0; k < planes; ++k) tma_load_2d(tile_at + k * PLANE, &hidden.planes, k * kFwKC, int(tile * RT), bars + group);
-    if (ldt) tma_load_2d(tile_at + planes * PLANE, &hidden.tail, planes * kFwKC, int(tile * RT), bars + group);
+    for (int k = 0; k < planes; ++k) tma_load_2d(tile_at + k * PLANE, &maps.planes, k * kFwKC, int(tile * RT), bars + group);
+    if (ldt) tma_load_2d(tile_at + planes * PLANE, &maps.tail, planes * kFwKC, int(tile * RT), bars + group);
   };
 
   if (gt == 0) mbar_init(bars + group, 1);
@@ -514,8 +555,31 @@ __global__ void __launch_bounds__(2 * kTileGroup, 1)
       __syncwarp();
       turns.pass();
       named_sync(1 + group, kTileGroup);  // every warp has read the tile
-      if (gt == 0 && more) load(tile + 2 * per);
-      if (live) forward_store<DIM>(h0, h1, u, c, rows, cout, residual, out, activated, vec_out, c + 1 < cout);
+      if (gt == 0 && more && leave != kInTile) load(tile + 2 * per);
+      if (leave == kByThreads) {
+        if (live) forward_store<DIM>(h0, h1, u, c, rows, cout, residual, out, activated, vec_out, c + 1 < cout);
+      } else {
+        const int x = c0 + wc * 16, y = int(tile * RT) + wr * 40;
+        if (x < cout) {
+          if (activated) {
+            box_pairs(box, h0, h1, t * 10, g);
+            send_box(&maps.activated, box, x, y, lane);
+          }
+          if (residual && live) {
+            const int n = rows.count<Q>(u);
+            const int64_t step = opaque(cout);
+            const double* from = residual + u * Q * cout + c;
+            double2 r[Q];  // cout is even here: c + 1 < cout
+#pragma unroll
+            for (int s = 0; s < Q; ++s, from += step)
+              r[s] = s < n ? *reinterpret_cast<const double2*>(from) : make_double2(0.0, 0.0);
+#pragma unroll
+            for (int s = 0; s < Q; ++s) h0[s] += r[s].x, h1[s] += r[s].y;
+          }
+          box_pairs(box, h0, h1, t * 10, g);
+          send_box(&maps.out, box, x, y, lane);
+        }
+      }
     } else {
       const int64_t u = tile * (RT / Q) + wr * 2 + (t >> 1), row = u * Q;
       const int cc = c + (t & 1);
@@ -545,11 +609,16 @@ __global__ void __launch_bounds__(2 * kTileGroup, 1)
       __syncwarp();
       turns.pass();
       named_sync(1 + group, kTileGroup);
-      if (gt == 0 && more) load(tile + 2 * per);
+      if (gt == 0 && more && leave != kInTile) load(tile + 2 * per);
+      const int x = c0 + wc * 16, y = int(tile * RT) + wr * 40;
+      if (leave != kByThreads && activated && x < cout) {
+        box_single(box, z, (t >> 1) * 20, 2 * g + (t & 1));
+        send_box(&maps.activated, box, x, y, lane);
+      }
       if (live) {
         const int64_t step = opaque(cout);
         double* to = out + row * cout + cc;
-        if (activated) {
+        if (activated && leave == kByThreads) {
           double* also = activated + row * cout + cc;
 #pragma unroll
           for (int s = 0; s < Q; ++s, also += step)
@@ -566,13 +635,24 @@ __global__ void __launch_bounds__(2 * kTileGroup, 1)
             for (int s = 0; s < 10; ++s) z[half + s] += r[s];
           }
         }
+        if (leave == kByThreads) {
 #pragma unroll
-        for (int s = 0; s < Q; ++s, to += step)
-          if (s < n) *to = z[s];
+          for (int s = 0; s < Q; ++s, to += step)
+            if (s < n) *to = z[s];
+        }
+      }
+      if (leave != kByThreads && x < cout) {
+        box_single(box, z, (t >> 1) * 20, 2 * g + (t & 1));
+        send_box(&maps.out, box, x, y, lane);
       }
     }
     __syncwarp();
+    if (leave == kInTile) {
+      named_sync(1 + group, kTileGroup);  // every box has left the tile's place
+      if (gt == 0 && more) load(tile + 2 * per);
+    }
   }
+  if (lane == 0) bulk_wait();
   turns.close(count(first), count(blockIdx.x / blocks + (1 - group) * per));
 }
 
@@ -604,20 +684,28 @@ cudaError_t launch_forward_tile(const double* hidden, const double* weight, cons
                                 double* out, double* activated, double* aux, Packed rows, int cin, int cout,
                                 bool, cudaStream_t stream) {
   const auto kernel = affine_forward_tile<DIM, ACT, WC>;
-  const size_t smem = tile_smem(WC, cin);
+  size_t smem = tile_smem(WC, cin);
   const int64_t blocks = (int64_t(cout) + 16 * WC - 1) / (16 * WC), total = rows.full * Jet<DIM>::Q + rows.value;
   const int64_t tiles = (total + tile_rows(WC) - 1) / tile_rows(WC);
   int sms = 0;
   TileMaps maps{};
   cudaError_t e = sm_count(&sms);
-  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
   if (e == cudaSuccess && cin >= kFwKC) e = matrix_map(&maps.planes, hidden, total, cin, kFwLD, tile_rows(WC));
   if (e == cudaSuccess && cin % kFwKC) e = matrix_map(&maps.tail, hidden, total, cin, tail_ld(cin), tile_rows(WC));
+  const bool vec_out = cout % 2 == 0 && aligned16(out) && aligned16(residual) && aligned16(activated) && aligned16(aux);
+  const size_t boxes = smem + 2 * kBoxesBytes + 1024;
+  const Leave leave = !vec_out                                                              ? kByThreads
+                      : boxes <= kTileSmem                                                  ? kOwnBoxes
+                      : sizeof(double) * tile_rows(WC) * tile_width(cin) >= kBoxesBytes + 1024 ? kInTile
+                                                                                            : kByThreads;
+  if (leave == kOwnBoxes) smem = boxes;
+  if (e == cudaSuccess && leave != kByThreads) e = matrix_map(&maps.out, out, total, cout, 16, 40, true);
+  if (e == cudaSuccess && leave != kByThreads && activated) e = matrix_map(&maps.activated, activated, total, cout, 16, 40, true);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
   if (e != cudaSuccess) return e;
   const int64_t most = sms / blocks > 0 ? sms / blocks : 1, per = tiles < most ? tiles : most;
-  const bool vec_out = cout % 2 == 0 && aligned16(out) && aligned16(residual) && aligned16(activated) && aligned16(aux);
   kernel<<<unsigned(per * blocks), 2 * kTileGroup, smem, stream>>>(maps, weight, bias, residual, out, activated, aux, rows,
-                                                                  cin, cout, aligned16(weight), vec_out);
+                                                                  cin, cout, aligned16(weight), vec_out, leave);
   return cudaGetLastError();
 }
 

@@ -117,8 +117,9 @@ inline cudaError_t sm_count(int* sms) {
 
 // Tensor map of [rows][cols] row-major FP64 read or written in boxes of box_rows x box_cols;
 // what a box holds past the matrix reads as zeros and is not written.  base and the rows on
-// 16-byte boundaries.
-inline cudaError_t matrix_map(CUtensorMap* map, const double* base, int64_t rows, int cols, int box_cols, int box_rows) {
+// 16-byte boundaries.  swizzle: 16-byte piece c of a box's 128-byte row r lies at c ^ (r & 7).
+inline cudaError_t matrix_map(CUtensorMap* map, const double* base, int64_t rows, int cols, int box_cols, int box_rows,
+                              bool swizzle = false) {
   using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                               const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                               CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -135,8 +136,8 @@ inline cudaError_t matrix_map(CUtensorMap* map, const double* base, int64_t rows
   const cuuint64_t dims[2] = {cuuint64_t(cols), cuuint64_t(rows)}, pitch[1] = {cuuint64_t(cols) * sizeof(double)};
   const cuuint32_t box[2] = {cuuint32_t(box_cols), cuuint32_t(box_rows)}, step[2] = {1, 1};
   const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT64, 2, const_cast<double*>(base), dims, pitch, box, step,
-                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
 }
 
