@@ -396,7 +396,7 @@ __host__ __device__ constexpr int tile_ldw(int cin) { return (cin + 7) / 8 * 8 +
 __host__ __device__ constexpr int tail_ld(int cin) { return cin % kFwKC ? (cin % kFwKC + 7) / 8 * 8 + 4 : 0; }
 __host__ __device__ constexpr int tile_width(int cin) { return cin / kFwKC * kFwLD + tail_ld(cin); }
 constexpr size_t tile_smem(int wc, int cin) {
-  return sizeof(double) * (2 * size_t(tile_rows(wc)) * tile_width(cin) + size_t(16 * wc) * tile_ldw(cin) + 2);
+  return sizeof(double) * (2 * size_t(tile_rows(wc)) * tile_width(cin) + size_t(16 * wc) * tile_ldw(cin) + 18);  // 18 barriers
 }
 
 // rows r0 .. r0 + count - 1 (zeros from `total` on) and columns 0 .. cin8 - 1 (zeros past cin)
@@ -416,33 +416,52 @@ __device__ __forceinline__ void load_rows(double* dst, int ld, const double* __r
 }
 
 struct TileMaps {
-  CUtensorMap planes, tail, out, activated;
+  CUtensorMap planes, tail, out, activated, residual;
 };
 
-// How a tile's outputs leave.  A warp's 40 rows x 16 channels go through a box in shared memory
-// and out by TMA: the same bytes as stores of the threads keep the load/store unit busy for
-// 1,400 cycles a tile (5,000 with the residual and a second output), in which the partner's
-// fragment loads, and with them its MMAs, hardly advance.  The boxes have room of their own, or
-// lie in the tile that has been read, whose successor then arrives a little later.
+// How a tile's outputs leave and its residual comes.  A warp's 40 rows x 16 channels go through
+// a box in shared memory, in and out by TMA: the same bytes as loads and stores of the threads
+// keep the load/store unit busy for 1,400 cycles a tile (5,000 with the residual and a second
+// output), in which the partner's fragment loads, and with them its MMAs, hardly advance.  The
+// boxes have room of their own, or lie in the tile that has been read, whose successor (and the
+// residual) then arrives a little later.
 enum Leave { kByThreads, kInTile, kOwnBoxes };
 constexpr int kBoxDoubles = 40 * 16, kBoxesBytes = 8 * kBoxDoubles * 8;  // a warp's; a group's
 
-// pairs (h0, h1) of rows row + s, channels 2 g, 2 g + 1, in a warp's box
+// pairs (h0, h1) of rows row + s, channels 2 g, 2 g + 1, into a warp's box, or onto what is there
 template <int Q>
-__device__ __forceinline__ void box_pairs(double* box, const double (&h0)[Q], const double (&h1)[Q], int row, int g) {
+__device__ __forceinline__ void box_pairs(double* box, const double (&h0)[Q], const double (&h1)[Q], int row, int g,
+                                          bool onto) {
+  const auto at = [&](int r) { return reinterpret_cast<double2*>(box + r * 16 + ((g ^ (r & 7)) << 1)); };
+  if (onto) {
 #pragma unroll
-  for (int s = 0; s < Q; ++s) {
-    const int r = row + s;
-    *reinterpret_cast<double2*>(box + r * 16 + ((g ^ (r & 7)) << 1)) = make_double2(h0[s], h1[s]);
+    for (int s = 0; s < Q; ++s) {
+      const double2 v = *at(row + s);
+      *at(row + s) = make_double2(h0[s] + v.x, h1[s] + v.y);
+    }
+  } else {
+#pragma unroll
+    for (int s = 0; s < Q; ++s) *at(row + s) = make_double2(h0[s], h1[s]);
   }
 }
 // one channel's rows
 template <int Q>
-__device__ __forceinline__ void box_single(double* box, const double (&z)[Q], int row, int channel) {
+__device__ __forceinline__ void box_single(double* box, const double (&z)[Q], int row, int channel, bool onto) {
+  const auto at = [&](int r) -> double& { return box[r * 16 + (((channel >> 1) ^ (r & 7)) << 1) + (channel & 1)]; };
+  if (onto) {
 #pragma unroll
-  for (int s = 0; s < Q; ++s) {
-    const int r = row + s;
-    box[r * 16 + (((channel >> 1) ^ (r & 7)) << 1) + (channel & 1)] = z[s];
+    for (int s = 0; s < Q; ++s) at(row + s) += z[s];
+  } else {
+#pragma unroll
+    for (int s = 0; s < Q; ++s) at(row + s) = z[s];
+  }
+}
+// a warp's box from columns x .., rows y ..
+__device__ __forceinline__ void fetch_box(const CUtensorMap* map, double* box, int x, int y, uint64_t* bar, int lane) {
+  if (lane == 0) {
+    fence_proxy_async();
+    mbar_arrive_expect_tx(bar, kBoxDoubles * sizeof(double));
+    tma_load_2d(box, map, x, y, bar);
   }
 }
 // a warp's box to columns x .., rows y ..; back when the box may be written again
@@ -490,7 +509,8 @@ __global__ void __launch_bounds__(2 * kTileGroup, 1)
   const int planes = cin / kFwKC, ldt = tail_ld(cin), ldw = tile_ldw(cin), size = RT * tile_width(cin);
   double *tile_at = smem + group * size, *sw = smem + 2 * size;
   uint64_t* bars = reinterpret_cast<uint64_t*>(sw + CB * ldw);
-  double* box = leave == kOwnBoxes ? sw + CB * ldw + 2 : tile_at;
+  uint64_t* bar_box = bars + 2 + (tid >> 5);
+  double* box = leave == kOwnBoxes ? sw + CB * ldw + 18 : tile_at;
   box += (1024 - (smem_u32(box) & 1023)) % 1024 / 8;
   box += ((leave == kOwnBoxes ? group * 8 : 0) + warp) * kBoxDoubles;
   auto load = [&](int64_t tile) {  // by one thread, once every warp has read the last tile
@@ -501,6 +521,7 @@ __global__ void __launch_bounds__(2 * kTileGroup, 1)
   };
 
   if (gt == 0) mbar_init(bars + group, 1);
+  if (lane == 0) mbar_init(bar_box, 1);
   __syncthreads();
   if (gt == 0 && first < tiles) load(first);
   load_rows(sw, ldw, weight, c0, CB, cout, cin, vec_w, tid >> 5, 16, lane);
@@ -521,7 +542,9 @@ __global__ void __launch_bounds__(2 * kTileGroup, 1)
     for (int j = 0; j < NT; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[j][e] = 0.0;
-    if (residual) {  // towards L2, for this tile's stores
+    const int x = c0 + wc * 16, y = int(tile * RT) + wr * 40;  // this warp's box
+    if (residual && leave == kOwnBoxes && x < cout) fetch_box(&maps.residual, box, x, y, bar_box, lane);
+    if (residual && leave != kOwnBoxes) {  // towards L2, for this tile's epilogue
       const int64_t r0 = tile * RT, left = total - r0;
       if (vec_out && blocks == 1) {
         if (gt == 0) prefetch_l2(residual + r0 * cout, unsigned((left < RT ? left : RT) * cout * sizeof(double)));
@@ -535,7 +558,6 @@ __global__ void __launch_bounds__(2 * kTileGroup, 1)
       dead = named_sync_or(1 + group, kTileGroup, !mbar_wait(bars + group, phase));
       if (dead && gt == 0) atomicExch(&g_affine_fault, 1);
     }
-    phase ^= 1;
     turns.take();
     if (!dead && c0 + wc * 16 < cout) {
       for (int p = 0; p < planes; ++p) {
@@ -559,25 +581,17 @@ __global__ void __launch_bounds__(2 * kTileGroup, 1)
       if (leave == kByThreads) {
         if (live) forward_store<DIM>(h0, h1, u, c, rows, cout, residual, out, activated, vec_out, c + 1 < cout);
       } else {
-        const int x = c0 + wc * 16, y = int(tile * RT) + wr * 40;
         if (x < cout) {
+          if (residual) {
+            if (leave == kInTile) fetch_box(&maps.residual, box, x, y, bar_box, lane);
+            if (!mbar_wait(bar_box, phase)) atomicExch(&g_affine_fault, 1);
+          }
+          box_pairs(box, h0, h1, t * 10, g, residual != nullptr);
+          send_box(&maps.out, box, x, y, lane);
           if (activated) {
-            box_pairs(box, h0, h1, t * 10, g);
+            box_pairs(box, h0, h1, t * 10, g, false);
             send_box(&maps.activated, box, x, y, lane);
           }
-          if (residual && live) {
-            const int n = rows.count<Q>(u);
-            const int64_t step = opaque(cout);
-            const double* from = residual + u * Q * cout + c;
-            double2 r[Q];  // cout is even here: c + 1 < cout
-#pragma unroll
-            for (int s = 0; s < Q; ++s, from += step)
-              r[s] = s < n ? *reinterpret_cast<const double2*>(from) : make_double2(0.0, 0.0);
-#pragma unroll
-            for (int s = 0; s < Q; ++s) h0[s] += r[s].x, h1[s] += r[s].y;
-          }
-          box_pairs(box, h0, h1, t * 10, g);
-          send_box(&maps.out, box, x, y, lane);
         }
       }
     } else {
@@ -610,42 +624,46 @@ __global__ void __launch_bounds__(2 * kTileGroup, 1)
       turns.pass();
       named_sync(1 + group, kTileGroup);
       if (gt == 0 && more && leave != kInTile) load(tile + 2 * per);
-      const int x = c0 + wc * 16, y = int(tile * RT) + wr * 40;
-      if (leave != kByThreads && activated && x < cout) {
-        box_single(box, z, (t >> 1) * 20, 2 * g + (t & 1));
-        send_box(&maps.activated, box, x, y, lane);
-      }
-      if (live) {
-        const int64_t step = opaque(cout);
-        double* to = out + row * cout + cc;
-        if (activated && leave == kByThreads) {
-          double* also = activated + row * cout + cc;
+      if (leave == kByThreads) {
+        if (live) {
+          const int64_t step = opaque(cout);
+          double* to = out + row * cout + cc;
+          if (activated) {
+            double* also = activated + row * cout + cc;
 #pragma unroll
-          for (int s = 0; s < Q; ++s, also += step)
-            if (s < n) *also = z[s];
-        }
-        if (residual) {
-          const double* from = residual + row * cout + cc;
-#pragma unroll
-          for (int half = 0; half < Q; half += 10) {  // ten rows requested at once
-            double r[10];
-#pragma unroll
-            for (int s = 0; s < 10; ++s, from += step) r[s] = half + s < n ? *from : 0.0;
-#pragma unroll
-            for (int s = 0; s < 10; ++s) z[half + s] += r[s];
+            for (int s = 0; s < Q; ++s, also += step)
+              if (s < n) *also = z[s];
           }
-        }
-        if (leave == kByThreads) {
+          if (residual) {
+            const double* from = residual + row * cout + cc;
+#pragma unroll
+            for (int half = 0; half < Q; half += 10) {  // ten rows requested at once
+              double r[10];
+#pragma unroll
+              for (int s = 0; s < 10; ++s, from += step) r[s] = half + s < n ? *from : 0.0;
+#pragma unroll
+              for (int s = 0; s < 10; ++s) z[half + s] += r[s];
+            }
+          }
 #pragma unroll
           for (int s = 0; s < Q; ++s, to += step)
             if (s < n) *to = z[s];
         }
-      }
-      if (leave != kByThreads && x < cout) {
-        box_single(box, z, (t >> 1) * 20, 2 * g + (t & 1));
+      } else if (x < cout) {
+        const int r0 = (t >> 1) * 20, channel = 2 * g + (t & 1);
+        if (residual) {
+          if (leave == kInTile) fetch_box(&maps.residual, box, x, y, bar_box, lane);
+          if (!mbar_wait(bar_box, phase)) atomicExch(&g_affine_fault, 1);
+        }
+        box_single(box, z, r0, channel, residual != nullptr);
         send_box(&maps.out, box, x, y, lane);
+        if (activated) {
+          box_single(box, z, r0, channel, false);
+          send_box(&maps.activated, box, x, y, lane);
+        }
       }
     }
+    phase ^= 1;
     __syncwarp();
     if (leave == kInTile) {
       named_sync(1 + group, kTileGroup);  // every box has left the tile's place
@@ -701,6 +719,7 @@ cudaError_t launch_forward_tile(const double* hidden, const double* weight, cons
   if (leave == kOwnBoxes) smem = boxes;
   if (e == cudaSuccess && leave != kByThreads) e = matrix_map(&maps.out, out, total, cout, 16, 40, true);
   if (e == cudaSuccess && leave != kByThreads && activated) e = matrix_map(&maps.activated, activated, total, cout, 16, 40, true);
+  if (e == cudaSuccess && leave != kByThreads && residual) e = matrix_map(&maps.residual, residual, total, cout, 16, 40, true);
   if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
   if (e != cudaSuccess) return e;
   const int64_t most = sms / blocks > 0 ? sms / blocks : 1, per = tiles < most ? tiles : most;
