@@ -435,9 +435,12 @@ __device__ __forceinline__ void box_pairs(double* box, const double (&h0)[Q], co
   const auto at = [&](int r) { return reinterpret_cast<double2*>(box + r * 16 + ((g ^ (r & 7)) << 1)); };
   if (onto) {
 #pragma unroll
-    for (int s = 0; s < Q; ++s) {
-      const double2 v = *at(row + s);
-      *at(row + s) = make_double2(h0[s] + v.x, h1[s] + v.y);
+    for (int half = 0; half < Q; half += 5) {  // loads first: the stores could not pass them
+      double2 v[5];
+#pragma unroll
+      for (int s = 0; s < 5; ++s) v[s] = *at(row + half + s);
+#pragma unroll
+      for (int s = 0; s < 5; ++s) *at(row + half + s) = make_double2(h0[half + s] + v[s].x, h1[half + s] + v[s].y);
     }
   } else {
 #pragma unroll
@@ -450,7 +453,13 @@ __device__ __forceinline__ void box_single(double* box, const double (&z)[Q], in
   const auto at = [&](int r) -> double& { return box[r * 16 + (((channel >> 1) ^ (r & 7)) << 1) + (channel & 1)]; };
   if (onto) {
 #pragma unroll
-    for (int s = 0; s < Q; ++s) at(row + s) += z[s];
+    for (int half = 0; half < Q; half += 10) {  // loads first: the stores could not pass them
+      double v[10];
+#pragma unroll
+      for (int s = 0; s < 10; ++s) v[s] = at(row + half + s);
+#pragma unroll
+      for (int s = 0; s < 10; ++s) at(row + half + s) = z[half + s] + v[s];
+    }
   } else {
 #pragma unroll
     for (int s = 0; s < Q; ++s) at(row + s) = z[s];
@@ -712,9 +721,12 @@ cudaError_t launch_forward_tile(const double* hidden, const double* weight, cons
   if (e == cudaSuccess && cin % kFwKC) e = matrix_map(&maps.tail, hidden, total, cin, tail_ld(cin), tile_rows(WC));
   const bool vec_out = cout % 2 == 0 && aligned16(out) && aligned16(residual) && aligned16(activated) && aligned16(aux);
   const size_t boxes = smem + 2 * kBoxesBytes + 1024;
+  // a 3-D tile's residual in the tile's place comes too late for its next tile (100 -> 60 at
+  // 8,193 + 2,049 points: 112 us, by threads 105)
+  const bool late = DIM == 3 && residual;
   const Leave leave = !vec_out                                                              ? kByThreads
                       : boxes <= kTileSmem                                                  ? kOwnBoxes
-                      : sizeof(double) * tile_rows(WC) * tile_width(cin) >= kBoxesBytes + 1024 ? kInTile
+                      : !late && sizeof(double) * tile_rows(WC) * tile_width(cin) >= kBoxesBytes + 1024 ? kInTile
                                                                                             : kByThreads;
   if (leave == kOwnBoxes) smem = boxes;
   if (e == cudaSuccess && leave != kByThreads) e = matrix_map(&maps.out, out, total, cout, 16, 40, true);
