@@ -817,7 +817,7 @@ constexpr size_t back_smem(int wc, bool fused, int cin, int cout) {
 constexpr int kEarlyRows = 6, kEarlySteps = 6;
 
 struct BackMaps {
-  CUtensorMap seed, activated, hidden;
+  CUtensorMap seed, activated, hidden, dh;
 };
 
 template <int DIM, bool ACT, int WC, bool FUSED>
@@ -826,7 +826,7 @@ __global__ void __launch_bounds__(2 * kTileGroup, 1)
                          const double* __restrict__ weight, const double* __restrict__ activated,
                          const double* __restrict__ aux, const double* __restrict__ seed, double* __restrict__ dz,
                          double* __restrict__ dh, double* __restrict__ dw_parts, double* __restrict__ db_parts, Packed rows,
-                         int cin, int cout, bool boxes, bool vec_out, bool vec_w) {
+                         int cin, int cout, bool boxes, bool vec_out, bool vec_w, Leave leave) {
   constexpr int Q = Jet<DIM>::Q, RT = tile_rows(WC), CB = 16 * WC, LD = kFwLD, PLANE = RT * LD, LDW = CB + 4;
   constexpr int NT = RT * WC / 64, UT = RT / Q, PAIRS = UT * CB / kTileGroup;  // n8 tiles a warp; jets a thread
   constexpr bool SWAP = FUSED && ACT;  // A first, then H in its place
@@ -846,6 +846,9 @@ __global__ void __launch_bounds__(2 * kTileGroup, 1)
   const int px = FUSED ? (pz > ph ? pz : ph) : 0;  // planes of the place that A and H share
   double *z_at = smem + group * (pz + px) * PLANE, *h_at = z_at + pz * PLANE, *sw = smem + 2 * (pz + px) * PLANE;
   uint64_t *bar = reinterpret_cast<uint64_t*>(sw + c8 * LDW) + 2 * group, *bar_h = bar + 1;
+  double* box = leave == kOwnBoxes ? sw + c8 * LDW + 4 : z_at;  // this warp's 40 rows x 16 channels
+  box += (1024 - (smem_u32(box) & 1023)) % 1024 / 8;
+  box += ((leave == kOwnBoxes ? group * 8 : 0) + warp) * kBoxDoubles;
 
   // a tile's planes of a [total][width] matrix, by TMA (one thread, after bar's expect) or by all
   auto copy = [&](double* to, const CUtensorMap* map, const double* from, int64_t tile, int planes, int width, uint64_t* b) {
@@ -935,18 +938,18 @@ __global__ void __launch_bounds__(2 * kTileGroup, 1)
     }
   };
   auto store_dz = [&](int64_t tile) {  // unfused: for affine_wgrad_tile
-    if (!ACT || FUSED || i0 != 0 || !has_z) return;
-#pragma unroll 1
-    for (int i = 0; i < PAIRS; ++i) {
-      const int64_t u = tile * UT + ul(i);
-      if (u >= units) continue;
-      const int n = rows.count<Q>(u);
-      const int64_t step = opaque(cout);
-      double* to = dz + rows.row<Q>(u) * cout + cz;
-      const double* from = z_mine + ul(i) * Q * LD;
-#pragma unroll
-      for (int s = 0; s < Q; ++s, to += step)
-        if (s < n) *to = from[s * LD];
+    if (!ACT || FUSED || i0 != 0) return;
+    const int64_t left = total - tile * RT;
+    const int n = left < RT ? int(left) : RT;
+    double* to = dz + tile * RT * cout;  // dz is 16-byte aligned, RT even
+    if (cout % 2 == 0) {
+      for (int r = warp; r < n; r += kTileGroup / 32)
+        for (int c = 2 * lane; c < cout; c += 64)
+          *reinterpret_cast<double2*>(to + r * cout + c) =
+              *reinterpret_cast<const double2*>(z_at + c / kFwKC * PLANE + r * LD + c % kFwKC);
+    } else {
+      for (int r = warp; r < n; r += kTileGroup / 32)
+        for (int c = lane; c < cout; c += 32) to[r * cout + c] = z_at[c / kFwKC * PLANE + r * LD + c % kFwKC];
     }
   };
 
@@ -1055,27 +1058,49 @@ __global__ void __launch_bounds__(2 * kTileGroup, 1)
     phase ^= 1;
     named_sync(1 + group, kTileGroup);  // every warp has read dZ and H
     const int64_t next = tile + 2 * per;
-    store_dz(tile);
-    if (ACT && !FUSED) named_sync(1 + group, kTileGroup);  // dZ has been read for global memory
-    if (next < tiles && !dead) request(next);
-    if (!dead && ci < cin) {
-      const bool two = ci + 1 < cin;
+    if (leave == kByThreads) {
+      store_dz(tile);
+      if (ACT && !FUSED) named_sync(1 + group, kTileGroup);  // dZ has been read for global memory
+      if (next < tiles && !dead) request(next);
+      if (!dead && ci < cin) {
+        const bool two = ci + 1 < cin;
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
+        for (int j = 0; j < NT; ++j)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int64_t r = tile * RT + wr * 40 + 8 * j + 2 * t + e;
-          if (r >= total) continue;
-          double* to = dh + r * cin + ci;
-          if (vec_out) {
-            *reinterpret_cast<double2*>(to) = make_double2(acc[j][e], acc[j][2 + e]);
-          } else {
-            to[0] = acc[j][e];
-            if (two) to[1] = acc[j][2 + e];
+          for (int e = 0; e < 2; ++e) {
+            const int64_t r = tile * RT + wr * 40 + 8 * j + 2 * t + e;
+            if (r >= total) continue;
+            double* to = dh + r * cin + ci;
+            if (vec_out) {
+              *reinterpret_cast<double2*>(to) = make_double2(acc[j][e], acc[j][2 + e]);
+            } else {
+              to[0] = acc[j][e];
+              if (two) to[1] = acc[j][2 + e];
+            }
           }
-        }
+      }
+    } else {
+      const int y = int(tile * RT) + wr * 40;
+      store_dz(tile);
+      if (ACT && !FUSED) named_sync(1 + group, kTileGroup);  // dZ has been read for global memory
+      if (leave == kOwnBoxes && next < tiles && !dead) request(next);
+      if (!dead && i0 + wc * 16 < cin) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int r = 8 * j + 2 * t + e;
+            *reinterpret_cast<double2*>(box + r * 16 + ((g ^ (r & 7)) << 1)) = make_double2(acc[j][e], acc[j][2 + e]);
+          }
+        send_box(&maps.dh, box, i0 + wc * 16, y, lane);
+      }
+      if (leave == kInTile) {
+        named_sync(1 + group, kTileGroup);  // every box has left
+        if (next < tiles && !dead) request(next);
+      }
     }
   }
+  if (lane == 0) bulk_wait();
   turns.close(count(first), count(blockIdx.x / blocks + (1 - group) * per));
   cp_async_wait<0>();
   __syncthreads();
@@ -1317,20 +1342,29 @@ cudaError_t launch_backward_tile(const double* hidden, const double* weight, con
                                  const double* seed, double* dz, double* dh, double* dw_parts, double* db_parts, int64_t per,
                                  Packed rows, int cin, int cout, cudaStream_t stream) {
   const auto kernel = affine_backward_tile<DIM, ACT, WC, FUSED>;
-  const size_t smem = back_smem(WC, FUSED, cin, cout);
+  size_t smem = back_smem(WC, FUSED, cin, cout);
   const int64_t total = rows.full * Jet<DIM>::Q + rows.value, blocks = (int64_t(cin) + 16 * WC - 1) / (16 * WC);
   const bool boxes = cout % 2 == 0 && aligned16(seed) && total < INT_MAX - 1024 &&
                      (!FUSED || (cin % 2 == 0 && aligned16(hidden) && aligned16(activated)));
   BackMaps maps{};
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
-  if (e == cudaSuccess && boxes) e = matrix_map(&maps.seed, seed, total, cout, kFwLD, tile_rows(WC));
+  cudaError_t e = cudaSuccess;
+  if (boxes) e = matrix_map(&maps.seed, seed, total, cout, kFwLD, tile_rows(WC));
   if (e == cudaSuccess && boxes && FUSED) e = matrix_map(&maps.hidden, hidden, total, cin, kFwLD, tile_rows(WC));
   if (e == cudaSuccess && boxes && FUSED && ACT) e = matrix_map(&maps.activated, activated, total, cout, kFwLD, tile_rows(WC));
-  if (e != cudaSuccess) return e;
   const bool vec_out = cin % 2 == 0 && aligned16(dh);
+  const int planes = tile_planes(cout) + (FUSED ? std::max(tile_planes(cin), tile_planes(cout)) : 0);
+  const size_t own = smem + 2 * kBoxesBytes + 1024;
+  const Leave leave = !vec_out || total >= INT_MAX - 1024                                            ? kByThreads
+                      : own <= kTileSmem                                                             ? kOwnBoxes
+                      : sizeof(double) * planes * tile_rows(WC) * kFwLD >= size_t(kBoxesBytes) + 1024 ? kInTile
+                                                                                                     : kByThreads;
+  if (leave == kOwnBoxes) smem = own;
+  if (e == cudaSuccess && leave != kByThreads) e = matrix_map(&maps.dh, dh, total, cin, 16, 40, true);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+  if (e != cudaSuccess) return e;
   kernel<<<unsigned(per * blocks), 2 * kTileGroup, smem, stream>>>(maps, hidden, weight, activated, aux, seed, dz, dh,
                                                                   dw_parts, db_parts, rows, cin, cout, boxes, vec_out,
-                                                                  cin % 2 == 0 && aligned16(weight));
+                                                                  cin % 2 == 0 && aligned16(weight), leave);
   return cudaGetLastError();
 }
 
@@ -1449,7 +1483,7 @@ int flashns_b200_affine_vjp(int dim, int activation, const double* hidden, const
     if (e == cudaSuccess) e = cudaMemsetAsync(d_bias, 0, size_t(cout) * sizeof(double), stream);
     return int(e);
   }
-  if (!hidden || !weight || !seed || !d_hidden || !scratch || (activation && (!activated || !aux)))
+  if (!hidden || !weight || !seed || !d_hidden || !scratch || !aligned16(scratch) || (activation && (!activated || !aux)))
     return int(cudaErrorInvalidValue);
   const size_t in = size_t(count) * cin * sizeof(double), bytes = size_t(count) * cout * sizeof(double);
   if (ranges_overlap(d_hidden, in, hidden, in) || ranges_overlap(d_hidden, in, seed, bytes) ||

@@ -223,7 +223,8 @@ int flashns_b200_affine(int dim, int activation, const double* hidden, const dou
                         const double* residual, double* out, double* activated, double* aux, int64_t full_points,
                         int64_t value_points, int cin, int cout, cudaStream_t stream);
 /* Adjoint at seed = dL/d out (which is the residual's gradient too): d_hidden, d_weight,
- * d_bias; activated and aux are the forward's (activation = 0: not read). */
+ * d_bias; activated and aux are the forward's (activation = 0: not read).  The scratch starts on
+ * a 16-byte boundary; its size depends on the current device. */
 int flashns_b200_affine_vjp_scratch(int dim, int activation, int64_t full_points, int64_t value_points, int cin,
                                     int cout, size_t* bytes);
 int flashns_b200_affine_vjp(int dim, int activation, const double* hidden, const double* weight,

@@ -181,7 +181,7 @@ def test_layer_entry_points_check_arguments_before_any_launch():
         full=3, value=2, cin=8, cout=4: lib.flashns_b200_affine_vjp(
             dim, act, h, p[1], a, aux, seed, dh, dw, p[7], scratch, n, full, value, cin, cout, None)
     for bad in (dict(dim=5), dict(act=-1), dict(h=None), dict(a=None), dict(aux=None), dict(seed=None), dict(dh=None),
-                dict(dw=None), dict(scratch=None), dict(n=0), dict(full=-1), dict(cin=0), dict(cout=-3),
+                dict(dw=None), dict(scratch=None), dict(scratch=ctypes.c_void_p((9 << 24) + 8)), dict(n=0), dict(full=-1), dict(cin=0), dict(cout=-3),
                 dict(dh=p[0]), dict(dh=p[4]), dict(dh=p[2])):
         assert avjp(**bad) == 1, bad
 
