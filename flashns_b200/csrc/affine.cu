@@ -683,6 +683,7 @@ __global__ void __launch_bounds__(2 * kTileGroup, 1)
   turns.close(count(first), count(blockIdx.x / blocks + (1 - group) * per));
 }
 
+constexpr int64_t kMostWeights = int64_t(1) << 40;  // what scratch sizes multiply stays in 64 bits
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 template <int DIM, bool ACT, int NG, int GW, int NS, bool STREAM, bool VALUES = false, bool TURNS = true>
@@ -1435,7 +1436,7 @@ int flashns_b200_affine(int dim, int activation, const double* hidden, const dou
                         const double* residual, double* out, double* activated, double* aux, int64_t full_points,
                         int64_t value_points, int cin, int cout, cudaStream_t stream) {
   if (!layer_sizes_ok(dim, full_points, value_points, cin) || !layer_sizes_ok(dim, full_points, value_points, cout) ||
-      (activation != 0 && activation != 1) || (!activation && (activated || aux)))
+      int64_t(cin) * cout > kMostWeights || (activation != 0 && activation != 1) || (!activation && (activated || aux)))
     return int(cudaErrorInvalidValue);
   const Packed rows{full_points, value_points};
   const int64_t count = full_points * (dim == 2 ? 10 : 20) + value_points;
@@ -1456,7 +1457,7 @@ int flashns_b200_affine(int dim, int activation, const double* hidden, const dou
 int flashns_b200_affine_vjp_scratch(int dim, int activation, int64_t full_points, int64_t value_points, int cin,
                                     int cout, size_t* bytes) {
   if (!layer_sizes_ok(dim, full_points, value_points, cin) || !layer_sizes_ok(dim, full_points, value_points, cout) ||
-      (activation != 0 && activation != 1) || !bytes)
+      int64_t(cin) * cout > kMostWeights || (activation != 0 && activation != 1) || !bytes)
     return int(cudaErrorInvalidValue);
   const int64_t count = full_points * (dim == 2 ? 10 : 20) + value_points;
   *bytes = 0;
@@ -1473,7 +1474,7 @@ int flashns_b200_affine_vjp(int dim, int activation, const double* hidden, const
                             double* d_weight, double* d_bias, double* scratch, size_t scratch_bytes,
                             int64_t full_points, int64_t value_points, int cin, int cout, cudaStream_t stream) {
   if (!layer_sizes_ok(dim, full_points, value_points, cin) || !layer_sizes_ok(dim, full_points, value_points, cout) ||
-      (activation != 0 && activation != 1) || !d_weight || !d_bias)
+      int64_t(cin) * cout > kMostWeights || (activation != 0 && activation != 1) || !d_weight || !d_bias)
     return int(cudaErrorInvalidValue);
   const Packed rows{full_points, value_points};
   const int q = dim == 2 ? 10 : 20;

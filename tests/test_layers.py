@@ -171,7 +171,7 @@ def test_layer_entry_points_check_arguments_before_any_launch():
         assert vjp(**bad) == 1, bad
     aff = lambda dim=2, act=1, h=p[0], res=p[3], out=p[4], a=p[5], aux=p[6], full=3, value=2, cin=8, cout=4: \
         lib.flashns_b200_affine(dim, act, h, p[1], p[2], res, out, a, aux, full, value, cin, cout, None)
-    for bad in (dict(dim=0), dict(act=2), dict(act=0), dict(h=None), dict(out=None), dict(full=-1), dict(cin=0),
+    for bad in (dict(dim=0), dict(act=2), dict(act=0), dict(full=0, cin=1 << 30, cout=1 << 30), dict(h=None), dict(out=None), dict(full=-1), dict(cin=0),
                 dict(cout=0), dict(out=p[0]), dict(out=p[3]), dict(a=p[4]), dict(a=p[0])):
         assert aff(**bad) == 1, bad
     assert aff(full=0, value=0, h=None, out=None) == 0

@@ -118,6 +118,78 @@ def test_affine_matches_oracle_at_many_points(cuda, dim, full, value, cin, cout)
     check_affine(cuda, dim, full, value, cin, cout, cout != 3)
 
 
+@pytest.mark.parametrize("dim", [2, 3])
+@pytest.mark.parametrize("cin,cout", [(64, 64), (33, 17), (128, 100), (200, 66), (257, 20), (8, 5)])
+def test_value_rows_alone_match_oracle(cuda, dim, cin, cout):
+    for value in (1, 41, 333):
+        check_affine(cuda, dim, 0, value, cin, cout, True, residual=value != 41)
+
+
+@pytest.mark.parametrize("dim", [2, 3])
+def test_one_tensor_may_be_several_inputs(cuda, dim):
+    """The block's input is its own residual; the norm's input is its own seed and skip."""
+    full, value, c = 21, 13, 64
+    k, n = affine_case(dim, full, value, c, c), norm_case(dim, full, value, c)
+    nat, layout = parts(dim, full, value)
+    h, w, b, gain, bias = (T(v, cuda) for v in (k["h"], k["w"], k["b"], n["gain"], n["bias"]))
+    out, act, aux = nat.affine_activation(layout, h, w, b, residual=h)
+    other = nat.affine_activation(layout, h, w, b, residual=h.clone())
+    assert all(torch.equal(p, q) for p, q in zip((out, act, aux), other))
+    for p, q in zip(nat.affine_activation_vjp(layout, act, w, act, aux, act),
+                    nat.affine_activation_vjp(layout, act.clone(), w, act, aux, act.clone())):
+        assert torch.equal(p, q)
+    _, stats = nat.layer_norm(layout, h, gain, bias)
+    for p, q in zip(nat.layer_norm_vjp(layout, h, gain, stats, h, skip=h),
+                    nat.layer_norm_vjp(layout, h, gain, stats, h.clone(), skip=h.clone())):
+        assert torch.equal(p, q)
+
+
+def test_offsets_past_32_bits(cuda):
+    """More than 2^31 values in a tensor: the last rows match the oracle within the counted
+    roundings (their bits may differ from those of the same rows alone: a row's place in its unit
+    decides which products are fused into the sums)."""
+    if torch.cuda.mem_get_info()[0] < 90 << 30:
+        pytest.skip("90 GB of free device memory needed")
+    f64 = dict(dtype=torch.float64, device=cuda)
+    tail, c = 4096, 64
+    rows = (1 << 31) // c + 81 * 1000 + tail
+    nat, layout = parts(2, 0, rows)
+    x = torch.empty(rows, c, **f64).uniform_(-1, 1)
+    gain, bias, w = torch.rand(c, **f64), torch.rand(c, **f64), torch.randn(c, c, **f64) / 8
+    end, n_gain, n_bias, n_w = (t.cpu().numpy() for t in (x[-tail:], gain, bias, w))
+    out, stats = nat.layer_norm(layout, x, gain, bias, eps=EPS)
+    for got, e, m in zip((out, stats), L.layer_norm(end, n_gain, n_bias, EPS, 2, 0),
+                         L.layer_norm(end, n_gain, n_bias, EPS, 2, 0, magnitude=True)):
+        assert worst(got[-tail:].cpu(), e, m, norm_roundings(c)) <= 1
+    del out, got
+    n_stats = stats[-tail:].cpu().numpy()
+    dx, _, dbias = nat.layer_norm_vjp(layout, x, gain, stats, x)
+    e, m = (L.layer_norm_vjp(end, n_gain, n_stats, end, None, 2, 0, magnitude=v)[0] for v in (False, True))
+    assert worst(dx[-tail:].cpu(), e, m, norm_vjp_roundings(c)) <= 1
+    # every row is summed once: rows roundings of values below 1
+    assert float((dbias - x.sum(0)).abs().max()) <= 2 * rows * HALF * rows
+    del dx, stats
+    for act in (True, False):
+        got = nat.affine_activation(layout, x, w, bias, residual=x, keep=False) if act else \
+            nat.affine(layout, x, w, bias, residual=x)
+        e, m = (L.affine(end, n_w, n_bias, end, 2, 0, act, magnitude=v)[0] for v in (False, True))
+        assert worst(got[-tail:].cpu(), e, m, affine_roundings(c)) <= 1
+        del got
+    dh, _, _ = nat.affine_vjp(layout, x, w, x)
+    e, m = (L.affine_vjp(end, n_w, None, None, end, 2, 0, magnitude=v)[0] for v in (False, True))
+    assert worst(dh[-tail:].cpu(), e, m, affine_vjp_roundings(c)) <= 1
+
+
+def test_layer_kernels_raise_no_device_fault(cuda):
+    """Their bounded waits on copies all end in time: the word that a wait that gives up sets is clear."""
+    from flashns_b200 import _lib
+    for case in ((2, 1500, 400, 64, 64), (3, 300, 90, 100, 128), (2, 0, 900, 64, 64)):
+        calls(cuda, *case)()
+    torch.cuda.synchronize()
+    fault = ctypes.c_int(-1)
+    assert _lib.library().flashns_b200_device_fault(ctypes.byref(fault), 0) == 0 and fault.value == 0
+
+
 def test_no_points_give_empty_outputs_and_zero_gradients(cuda):
     for dim in (2, 3):
         nat, layout = parts(dim, 0, 0)
