@@ -42,11 +42,15 @@ __device__ __forceinline__ void tanh_vjp(const double* h, double a1, const doubl
 // channel 2g (g < 8) or 2(g - 8) + 1, which makes a thread's two channels neighbours: the
 // residual and the outputs move as 16-byte pairs.
 //
-// A CTA keeps a block of 64 output channels' W in shared memory and runs NG groups of 4 warps
-// that share it and nothing else: each streams its own tiles (4 units x 32 input channels a
-// stage, NS stages of cp.async) and meets only its own named barrier, so one group's epilogue
-// runs under the others' MMAs and loads.  Rows are padded to 36 doubles, W's to 2 (mod 8), and
-// a 3-D unit by 8 more: every fragment load is free of bank conflicts.
+// This form is for layers whose whole tiles do not fit (below), odd input widths, unaligned
+// tensors, and value rows alone.  A CTA keeps a block of 64 output channels' W in shared memory
+// (wider inputs than 256 stream it) and runs NG groups of GW warps that share it: each streams
+// its own tiles (GW units x 32 input channels a stage, NS stages of cp.async).  Left to
+// themselves the groups fall into step, sharing the one FP64 datapath evenly, and then wait for
+// memory together, so they take turns on it (Turns: 64 -> 64 with tanh and residual at 16,384 +
+// 4,096 points takes 89 us in a ring of four, 95 with two turns at a time).  Rows are padded to
+// 36 doubles, W's to 2 (mod 8), and a 3-D unit by 8 more: every fragment load is free of bank
+// conflicts.
 constexpr int kFwKC = 32, kFwLD = kFwKC + 4, kFwCB = 64;
 
 template <int DIM>
@@ -377,16 +381,17 @@ __global__ void __launch_bounds__(NG* GW * 32, 1)
 }
 
 // ---------------------------------------------------------------- forward, resident tiles
-// The same product where W's block and two whole tiles fit in shared memory (cin <= 128): two
-// groups of 8 warps, WC of them across channels (16 each) and 8 / WC across rows (40 each, as
+// The same product where W's block and two whole tiles fit in shared memory (cin <= 112 for up
+// to 64 outputs, 128 for more): two groups of 8 warps, WC of them across channels (16 each) and 8 / WC across rows (40 each, as
 // four blocks of 10; a 3-D unit is two blocks).  A group waits for its whole tile before it
 // takes its turn, runs MMAs and tanh jets in one stretch, hands the turn on, and only then
 // loads its next tile and stores: between take and pass there is no barrier and no memory
 // access, and the partner's turn covers the group's.  The jets stay inside the turn because
 // DMMA and DFMA share one datapath with DMMA first: outside it they crawl behind the partner's
-// MMAs (16,384 + 4,096 points, 64 -> 64 with residual: 110 us against 88).  A tile is one TMA
-// box of 36 columns for each 32 (the 4 more are the padding that frees the fragment loads of
-// bank conflicts): issued by threads, the same copies slow the partner's MMAs.
+// MMAs (16,384 + 4,096 points, 64 -> 64 with residual: 110 us against 88, both with outputs
+// stored by threads; 73 with the boxes below).  A tile is one TMA box of 36 columns for each 32
+// (the 4 more are the padding that frees the fragment loads of bank conflicts).  At that size a
+// turn is 6,500 cycles of MMAs (5,120 at the full rate) and 1,250 of jets.
 constexpr int kTileGroup = 256, kTileSmem = 227 * 1024;
 constexpr int tile_rows(int wc) { return 320 / wc; }
 __host__ __device__ constexpr int tile_planes(int cin) { return (cin + kFwKC - 1) / kFwKC; }
@@ -805,7 +810,8 @@ __global__ void __launch_bounds__(kAffThreads)
 // tiles.  The partner's turn (12,000 cycles and more) covers what moves data: G and A in by
 // TMA boxes (unfused, A and a1 go to registers), dH out.  H takes A's place once the VJP has
 // read it, behind the MMAs of dH.  Outside the turn the VJP took 15,000 cycles behind the
-// partner's MMAs, against some 1,300 inside; copies issued by threads slow those MMAs.
+// partner's MMAs; inside, a turn of the 2-D 64 -> 64 layer is 14,150 cycles, 11,700 without a
+// VJP, 10,240 for the MMAs alone at the full rate (16,384 + 4,096 points: 117 us, against 144).
 // Unfused, dZ also goes to global memory, for affine_wgrad_tile.
 constexpr size_t back_smem(int wc, bool fused, int cin, int cout) {
   const int other = cin > cout ? cin : cout;  // H and A share their place
