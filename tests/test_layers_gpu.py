@@ -93,7 +93,7 @@ def check_affine(cuda, dim, full, value, cin, cout, activation, residual=True, s
 
 
 SHAPES = [(1, 1), (3, 64), (64, 3), (64, 64), (65, 33), (32, 32), (31, 66), (128, 128), (100, 60), (200, 130),
-          (8, 300), (130, 64), (64, 130), (16, 128), (257, 20)]
+          (8, 300), (130, 64), (64, 130), (16, 128), (257, 20), (64, 65), (100, 127), (66, 129), (112, 64), (114, 64), (12, 40)]
 
 
 @pytest.mark.parametrize("dim", [2, 3])
@@ -113,7 +113,8 @@ def test_affine_matches_oracle_at_every_shape(cuda, dim, activation, cin, cout):
 
 @pytest.mark.parametrize("dim,full,value,cin,cout", [(2, 4099, 1031, 64, 64), (3, 1031, 515, 64, 64),
                                                      (2, 2051, 509, 128, 128), (3, 1027, 300, 100, 60),
-                                                     (2, 0, 9001, 64, 64), (2, 4000, 900, 64, 3)])
+                                                     (2, 0, 9001, 64, 64), (2, 4000, 900, 64, 3), (2, 3001, 77, 64, 97),
+                                                     (3, 1500, 401, 128, 66), (2, 3500, 1, 30, 62)])
 def test_affine_matches_oracle_at_many_points(cuda, dim, full, value, cin, cout):
     check_affine(cuda, dim, full, value, cin, cout, cout != 3)
 
