@@ -46,6 +46,7 @@ SIGNATURES = {
     "flashns_b200_layer_norm": [_c_int] + [_c_ptr] * 5 + [_c_dbl, _c_i64, _c_i64, _c_int, _c_ptr],
     "flashns_b200_layer_norm_vjp_scratch": [_c_int, _c_i64, _c_i64, _c_int, ctypes.POINTER(_c_size)],
     "flashns_b200_layer_norm_vjp": [_c_int] + [_c_ptr] * 9 + [_c_size, _c_i64, _c_i64, _c_int, _c_ptr],
+    "flashns_b200_layer_wait_polls": [ctypes.c_uint, ctypes.c_uint],
     "flashns_b200_affine": [_c_int, _c_int] + [_c_ptr] * 7 + [_c_i64, _c_i64, _c_int, _c_int, _c_ptr],
     "flashns_b200_affine_vjp_scratch": [_c_int, _c_int, _c_i64, _c_i64, _c_int, _c_int, ctypes.POINTER(_c_size)],
     "flashns_b200_affine_vjp": [_c_int, _c_int] + [_c_ptr] * 9 + [_c_size, _c_i64, _c_i64, _c_int, _c_int, _c_ptr],

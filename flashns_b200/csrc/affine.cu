@@ -25,6 +25,25 @@ namespace {
 
 constexpr int kAffThreads = 256;
 
+// Polls after which a wait on a copy gives up: on a tile, and on what a tile's outputs need
+// besides.  Fewer than kMbarSpins only where a test makes the waits give up.
+struct Polls {
+  unsigned tile, late;
+};
+thread_local Polls t_polls{kMbarSpins, kMbarSpins};
+
+// A wait that gives up sets the fault word and then, bounded too, lets the copy land: a late one
+// would write into the place's next use, or into another block's memory.  False in the whole
+// warp if any of its lanes gave up (call it with the whole warp).
+__device__ __forceinline__ bool wait_copy(uint64_t* bar, unsigned phase, unsigned polls) {
+  const bool ok = mbar_wait(bar, phase, polls);
+  if (__all_sync(0xffffffffu, ok)) return true;
+  if (!ok) atomicExch(&g_affine_fault, 1);
+  mbar_wait(bar, phase);
+  __syncwarp();
+  return false;
+}
+
 template <int DIM>
 __device__ __forceinline__ void tanh_forward(const double* z, double* h, double& a1) {
   if constexpr (DIM == 2) jet_fwd_2d3(z, h, a1); else jet_fwd_3d3(z, h, a1);
@@ -507,7 +526,7 @@ __global__ void __launch_bounds__(2 * kTileGroup, 1)
     affine_forward_tile(const __grid_constant__ TileMaps maps, const double* __restrict__ weight,
                         const double* __restrict__ bias, const double* __restrict__ residual, double* __restrict__ out,
                         double* __restrict__ activated, double* __restrict__ aux, Packed rows, int cin, int cout,
-                        bool vec_w, bool vec_out, Leave leave) {
+                        bool vec_w, bool vec_out, Leave leave, Polls polls) {
   constexpr int Q = Jet<DIM>::Q, NT = 5, RT = tile_rows(WC), CB = 16 * WC, LD = kFwLD, PLANE = RT * LD;
   extern __shared__ __align__(128) double smem[];
   const int tid = threadIdx.x, group = tid / kTileGroup, gt = tid % kTileGroup, warp = gt >> 5, wc = warp % WC, wr = warp / WC;
@@ -549,7 +568,8 @@ __global__ void __launch_bounds__(2 * kTileGroup, 1)
   const double *ap = sw + ch * ldw + t, *bp = tile_at + brow * LD + t;
   const Turns<2, kTileGroup> turns(group);
   unsigned phase = 0;
-  bool dead = false;  // a copy's bounded wait gave up: the group keeps the turns and does no work
+  // a copy's wait gave up: in this warp; in this group, which keeps the turns and does no more work
+  bool late = false, dead = false;
   for (int64_t tile = first; tile < tiles; tile += 2 * per) {
     double acc[NT][4];
 #pragma unroll
@@ -557,7 +577,8 @@ __global__ void __launch_bounds__(2 * kTileGroup, 1)
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[j][e] = 0.0;
     const int x = c0 + wc * 16, y = int(tile * RT) + wr * 40;  // this warp's box
-    if (residual && leave == kOwnBoxes && x < cout) fetch_box(&maps.residual, box, x, y, bar_box, lane);
+    const bool fetched = residual && leave == kOwnBoxes && x < cout && !late && !dead;
+    if (fetched) fetch_box(&maps.residual, box, x, y, bar_box, lane);
     if (residual && leave != kOwnBoxes) {  // towards L2, for this tile's epilogue
       const int64_t r0 = tile * RT, left = total - r0;
       if (vec_out && blocks == 1) {
@@ -569,8 +590,9 @@ __global__ void __launch_bounds__(2 * kTileGroup, 1)
       }
     }
     if (!dead) {
-      dead = named_sync_or(1 + group, kTileGroup, !mbar_wait(bars + group, phase));
-      if (dead && gt == 0) atomicExch(&g_affine_fault, 1);
+      const bool ok = wait_copy(bars + group, phase, polls.tile);
+      dead = named_sync_or(1 + group, kTileGroup, late || !ok);
+      if (dead && fetched) mbar_wait(bar_box, phase);  // no box is under way when the block ends
     }
     turns.take();
     if (!dead && c0 + wc * 16 < cout) {
@@ -595,14 +617,16 @@ __global__ void __launch_bounds__(2 * kTileGroup, 1)
       if (leave == kByThreads) {
         if (live) forward_store<DIM>(h0, h1, u, c, rows, cout, residual, out, activated, vec_out, c + 1 < cout);
       } else {
-        if (x < cout) {
+        if (x < cout && !dead) {
           if (residual) {
             if (leave == kInTile) fetch_box(&maps.residual, box, x, y, bar_box, lane);
-            if (!mbar_wait(bar_box, phase)) atomicExch(&g_affine_fault, 1);
+            late = !wait_copy(bar_box, phase, polls.late);
           }
-          box_pairs(box, h0, h1, t * 10, g, residual != nullptr);
-          send_box(&maps.out, box, x, y, lane);
-          if (activated) {
+          if (!late) {
+            box_pairs(box, h0, h1, t * 10, g, residual != nullptr);
+            send_box(&maps.out, box, x, y, lane);
+          }
+          if (!late && activated) {
             box_pairs(box, h0, h1, t * 10, g, false);
             send_box(&maps.activated, box, x, y, lane);
           }
@@ -663,15 +687,17 @@ __global__ void __launch_bounds__(2 * kTileGroup, 1)
           for (int s = 0; s < Q; ++s, to += step)
             if (s < n) *to = z[s];
         }
-      } else if (x < cout) {
+      } else if (x < cout && !dead) {
         const int r0 = (t >> 1) * 20, channel = 2 * g + (t & 1);
         if (residual) {
           if (leave == kInTile) fetch_box(&maps.residual, box, x, y, bar_box, lane);
-          if (!mbar_wait(bar_box, phase)) atomicExch(&g_affine_fault, 1);
+          late = !wait_copy(bar_box, phase, polls.late);
         }
-        box_single(box, z, r0, channel, residual != nullptr);
-        send_box(&maps.out, box, x, y, lane);
-        if (activated) {
+        if (!late) {
+          box_single(box, z, r0, channel, residual != nullptr);
+          send_box(&maps.out, box, x, y, lane);
+        }
+        if (!late && activated) {
           box_single(box, z, r0, channel, false);
           send_box(&maps.activated, box, x, y, lane);
         }
@@ -680,8 +706,8 @@ __global__ void __launch_bounds__(2 * kTileGroup, 1)
     phase ^= 1;
     __syncwarp();
     if (leave == kInTile) {
-      named_sync(1 + group, kTileGroup);  // every box has left the tile's place
-      if (gt == 0 && more) load(tile + 2 * per);
+      dead = named_sync_or(1 + group, kTileGroup, late) || dead;  // every box has left the tile's place
+      if (gt == 0 && more && !dead) load(tile + 2 * per);
     }
   }
   if (lane == 0) bulk_wait();
@@ -742,7 +768,7 @@ cudaError_t launch_forward_tile(const double* hidden, const double* weight, cons
   if (e != cudaSuccess) return e;
   const int64_t most = sms / blocks > 0 ? sms / blocks : 1, per = tiles < most ? tiles : most;
   kernel<<<unsigned(per * blocks), 2 * kTileGroup, smem, stream>>>(maps, weight, bias, residual, out, activated, aux, rows,
-                                                                  cin, cout, aligned16(weight), vec_out, leave);
+                                                                  cin, cout, aligned16(weight), vec_out, leave, t_polls);
   return cudaGetLastError();
 }
 
@@ -1437,6 +1463,12 @@ cudaError_t backward(const double* hidden, const double* weight, const double* a
 using namespace flashns_b200;
 
 extern "C" {
+
+int flashns_b200_layer_wait_polls(unsigned tile, unsigned late) {
+  if (tile > kMbarSpins || late > kMbarSpins) return int(cudaErrorInvalidValue);
+  t_polls = {tile, late};
+  return int(cudaSuccess);
+}
 
 int flashns_b200_affine(int dim, int activation, const double* hidden, const double* weight, const double* bias,
                         const double* residual, double* out, double* activated, double* aux, int64_t full_points,

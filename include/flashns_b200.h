@@ -232,6 +232,13 @@ int flashns_b200_affine_vjp(int dim, int activation, const double* hidden, const
                             double* d_weight, double* d_bias, double* scratch, size_t scratch_bytes,
                             int64_t full_points, int64_t value_points, int cin, int cout, cudaStream_t stream);
 
+/* Polls (0..131072, the default, each suspending at most 10 us) after which the affine kernels
+ * launched by this host thread from now on give up a wait: `tile` on a tile's copies, `late` on
+ * what comes after its products.  0 gives up at once, so callers can check that a stuck copy
+ * ends with the fault word set and nothing written from it; a wait that gave up waits once more,
+ * at the default bound, before its memory is used again or its block ends. */
+int flashns_b200_layer_wait_polls(unsigned tile, unsigned late);
+
 /* Vector kernels of the device-resident L-BFGS (no reference counterpart: the reference
  * uses torch.optim.LBFGS, experiments/pinn_solver/solve.py:150-167).
  *   row_dots:      out[r] = rows[r] . v for r < k (rows [k][stride]); fixed-order reductions */
