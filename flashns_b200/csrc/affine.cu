@@ -859,7 +859,7 @@ __global__ void __launch_bounds__(2 * kTileGroup, 1)
                          const double* __restrict__ weight, const double* __restrict__ activated,
                          const double* __restrict__ aux, const double* __restrict__ seed, double* __restrict__ dz,
                          double* __restrict__ dh, double* __restrict__ dw_parts, double* __restrict__ db_parts, Packed rows,
-                         int cin, int cout, bool boxes, bool vec_out, bool vec_w, Leave leave) {
+                         int cin, int cout, bool boxes, bool vec_out, bool vec_w, Leave leave, Polls polls) {
   constexpr int Q = Jet<DIM>::Q, RT = tile_rows(WC), CB = 16 * WC, LD = kFwLD, PLANE = RT * LD, LDW = CB + 4;
   constexpr int NT = RT * WC / 64, UT = RT / Q, PAIRS = UT * CB / kTileGroup;  // n8 tiles a warp; jets a thread
   constexpr bool SWAP = FUSED && ACT;  // A first, then H in its place
@@ -1027,7 +1027,8 @@ __global__ void __launch_bounds__(2 * kTileGroup, 1)
   const Turns<2, kTileGroup> turns(group);
   const int early = c8 / 8 > kEarlySteps ? c8 / 8 - kEarlySteps : 0;
   unsigned phase = 0;
-  bool dead = false, late = false;  // a copy's bounded wait gave up: the group keeps the turns and does no work
+  // a copy's wait gave up: in this warp (H's); in this group, which keeps the turns and does no more work
+  bool late = false, dead = false;
   for (int64_t tile = first; tile < tiles; tile += 2 * per) {
     double acc[NT][4];
 #pragma unroll
@@ -1035,12 +1036,9 @@ __global__ void __launch_bounds__(2 * kTileGroup, 1)
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[j][e] = 0.0;
     cp_async_wait<0>();
-    if (!dead) {
-      dead = named_sync_or(1 + group, kTileGroup, late || (boxes && !mbar_wait(bar, phase)));
-      if (dead && gt == 0) atomicExch(&g_affine_fault, 1);
-    }
+    if (!dead) dead = named_sync_or(1 + group, kTileGroup, boxes && !wait_copy(bar, phase, polls.tile));
     turns.take();
-    form(tile);
+    if (!dead) form(tile);
     if constexpr (ACT) {
       named_sync(1 + group, kTileGroup);  // dZ is there, A has been read
       if (SWAP && !dead && (!boxes || gt == 0)) {
@@ -1073,8 +1071,7 @@ __global__ void __launch_bounds__(2 * kTileGroup, 1)
         cp_async_wait<0>();
         named_sync(1 + group, kTileGroup);
       } else if (!dead) {
-        late = !mbar_wait(bar_h, phase);
-        if (late) atomicExch(&g_affine_fault, 1);
+        late = !wait_copy(bar_h, phase, polls.late);
       }
     }
     if (!FUSED && !(!dead && has_h)) turns.pass();
@@ -1089,10 +1086,12 @@ __global__ void __launch_bounds__(2 * kTileGroup, 1)
       }
     }
     phase ^= 1;
-    named_sync(1 + group, kTileGroup);  // every warp has read dZ and H
+    // every warp has read dZ and H
+    if constexpr (SWAP) dead = named_sync_or(1 + group, kTileGroup, late) || dead;
+    else named_sync(1 + group, kTileGroup);
     const int64_t next = tile + 2 * per;
     if (leave == kByThreads) {
-      store_dz(tile);
+      if (!dead) store_dz(tile);
       if (ACT && !FUSED) named_sync(1 + group, kTileGroup);  // dZ has been read for global memory
       if (next < tiles && !dead) request(next);
       if (!dead && ci < cin) {
@@ -1114,7 +1113,7 @@ __global__ void __launch_bounds__(2 * kTileGroup, 1)
       }
     } else {
       const int y = int(tile * RT) + wr * 40;
-      store_dz(tile);
+      if (!dead) store_dz(tile);
       if (ACT && !FUSED) named_sync(1 + group, kTileGroup);  // dZ has been read for global memory
       if (leave == kOwnBoxes && next < tiles && !dead) request(next);
       if (!dead && i0 + wc * 16 < cin) {
@@ -1397,7 +1396,7 @@ cudaError_t launch_backward_tile(const double* hidden, const double* weight, con
   if (e != cudaSuccess) return e;
   kernel<<<unsigned(per * blocks), 2 * kTileGroup, smem, stream>>>(maps, hidden, weight, activated, aux, seed, dz, dh,
                                                                   dw_parts, db_parts, rows, cin, cout, boxes, vec_out,
-                                                                  cin % 2 == 0 && aligned16(weight), leave);
+                                                                  cin % 2 == 0 && aligned16(weight), leave, t_polls);
   return cudaGetLastError();
 }
 

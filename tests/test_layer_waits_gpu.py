@@ -10,7 +10,7 @@ import torch
 
 from oracle import jets as J
 from tests.layers_cases import affine_case
-from tests.test_layers_gpu import T, guarded
+from tests.test_layers_gpu import T, guarded, parts
 
 pytestmark = pytest.mark.gpu
 POLLS = 1 << 17
@@ -71,6 +71,21 @@ def forward(lib, cuda, dim, full, value, cin, cout, residual, activation=True):
     return Call(lib, cuda, [rows * cout] * 2 + [(full + value) * cout] if activation else [rows * cout], launch)
 
 
+def adjoint(lib, cuda, dim, full, value, cin, cout, activation=True):
+    """Outputs d_hidden, d_weight, d_bias, then the scratch."""
+    k = affine_case(dim, full, value, cin, cout)
+    h, w, b, g = (T(k[n], cuda) for n in ("h", "w", "b", "seed"))
+    _, act, aux = parts(dim, full, value)[0].affine_activation(parts(dim, full, value)[1], h, w, b)
+    size = ctypes.c_size_t()
+    assert lib.flashns_b200_affine_vjp_scratch(dim, int(activation), full, value, cin, cout, ctypes.byref(size)) == 0
+
+    def launch(views, stream):
+        kept = (act, aux) if activation else (None, None)
+        return lib.flashns_b200_affine_vjp(dim, int(activation), *map(ptr, (h, w, *kept, g, *views)), size.value, full,
+                                           value, cin, cout, stream)
+    return Call(lib, cuda, [h.numel(), w.numel(), cout, size.value // 8], launch)
+
+
 def recovers(call, lib, expected):
     assert fault(lib, clear=True) == 1
     assert fault(lib) == 0
@@ -105,6 +120,34 @@ def test_forward_gives_up_on_a_residual(cuda, lib, dim, full, value, cin, cout):
     else:
         assert untouched(got[0]) and untouched(got[1])
         recovers(call, lib, expected)
+
+
+# dH through boxes of its own, boxes in the tile's place, by threads; one kernel (to 64 wide), then two
+ADJOINT = [(2, 3000, 100, 64, 64), (2, 9, 5, 64, 64), (2, 3000, 100, 30, 62), (2, 3000, 100, 64, 3), (3, 1300, 90, 64, 64),
+           (2, 2500, 77, 128, 128), (2, 2500, 77, 100, 80), (3, 900, 50, 128, 66), (2, 2500, 77, 65, 66)]
+
+
+@pytest.mark.parametrize("dim,full,value,cin,cout", ADJOINT)
+@pytest.mark.parametrize("activation", [False, True])
+def test_adjoint_gives_up_on_a_tile(cuda, lib, dim, full, value, cin, cout, activation):
+    call = adjoint(lib, cuda, dim, full, value, cin, cout, activation)
+    expected = call.run()[:3]
+    assert fault(lib) == 0
+    got = call.run(tile=0)
+    if cout % 2 or (max(cin, cout) <= 64 and cin % 2):  # no tile comes by TMA: nothing waits
+        assert fault(lib) == 0 and all(map(torch.equal, got, expected))
+    else:
+        assert untouched(got[0])
+        recovers(call, lib, expected)
+
+
+@pytest.mark.parametrize("dim,full,value,cin,cout", [c for c in ADJOINT if max(c[3:]) <= 64 and c[4] % 2 == 0])
+def test_adjoint_gives_up_on_its_input(cuda, lib, dim, full, value, cin, cout):
+    """H, which takes A's place behind the products of dH."""
+    call = adjoint(lib, cuda, dim, full, value, cin, cout)
+    expected = call.run()[:3]
+    assert untouched(call.run(late=0)[0])
+    recovers(call, lib, expected)
 
 
 def test_polls_are_bounded(lib):
