@@ -1184,7 +1184,7 @@ __global__ void __launch_bounds__(kWgThreads, 1)
     affine_wgrad_tile(const __grid_constant__ CUtensorMap dz_map, const __grid_constant__ CUtensorMap hidden_map,
                       const double* __restrict__ dz, const double* __restrict__ hidden,
                       double* __restrict__ dw_parts, double* __restrict__ db_parts,
-                      int64_t total, int64_t full_rows, int q, int cin, int cout, bool boxes) {
+                      int64_t total, int64_t full_rows, int q, int cin, int cout, bool boxes, Polls polls) {
   constexpr int CZ = wg_cout(MT, WI), CI = 32 * WI, PZ = CZ / kFwKC, P = PZ + WI, LD = kFwLD, PLANE = kWgRows * LD;
   extern __shared__ __align__(128) double smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -1246,13 +1246,20 @@ __global__ void __launch_bounds__(kWgThreads, 1)
     const int ahead = stage == 0 ? 2 : stage - 1;  // tile k - 1's stage, tile k + 2's next
     if (boxes) {
       // the warps meet only at the stages: a warp that is done with one starts on the next
-      bool ok = mbar_wait(bars + stage, phase);
+      bool ok = mbar_wait(bars + stage, phase, polls.tile);
       if (tid == 0 && k + 2 < mine) {
-        ok = ok && (k == 0 || mbar_wait(empty + ahead, unsigned((k - 1) / kWgStages) & 1));
+        ok = ok && (k == 0 || mbar_wait(empty + ahead, unsigned((k - 1) / kWgStages) & 1, polls.late));
         if (ok) load(k + 2, ahead);
       }
-      if (!__all_sync(0xffffffffu, ok)) {  // a bounded wait gave up; the other warps' will too
+      if (!__all_sync(0xffffffffu, ok)) {  // a wait gave up; the other warps' will too
         if (lane == 0) atomicExch(&g_affine_fault, 1);
+        // The first warp, whose lane 0 asks for the tiles, stays (waits bounded too) until those
+        // under way have landed: the block's memory is another's when it has ended.
+        if (warp == 0) {
+          const bool asked = __shfl_sync(0xffffffffu, ok, 0);  // for tile k + 2 as well
+          const int64_t end = mine < k + 2 + asked ? mine : k + 2 + asked;
+          for (int64_t n = k; n < end; ++n) mbar_wait(bars + n % kWgStages, unsigned(n / kWgStages) & 1);
+        }
         return;
       }
     } else {
@@ -1413,7 +1420,7 @@ cudaError_t launch_wgrad(const double* dz, const double* hidden, double* dw_part
   if (e == cudaSuccess && boxes) e = matrix_map(&hidden_map, hidden, total, cin, kFwLD, kWgRows);
   if (e != cudaSuccess) return e;
   kernel<<<unsigned(parts * blocks), kWgThreads, smem, stream>>>(dz_map, hidden_map, dz, hidden, dw_parts, db_parts, total,
-                                                                full_rows, q, cin, cout, boxes);
+                                                                full_rows, q, cin, cout, boxes, t_polls);
   return cudaGetLastError();
 }
 

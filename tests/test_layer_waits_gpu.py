@@ -150,5 +150,23 @@ def test_adjoint_gives_up_on_its_input(cuda, lib, dim, full, value, cin, cout):
     recovers(call, lib, expected)
 
 
+# several stages a block; one stage; blocks with fewer stages than others; 64 to 256 wide blocks
+WGRAD = [(2, 3000, 100, 64, 130), (2, 3, 1, 64, 130), (2, 1500, 93, 130, 140), (3, 1300, 90, 200, 192), (2, 9000, 41, 66, 320)]
+
+
+@pytest.mark.parametrize("dim,full,value,cin,cout", WGRAD)
+@pytest.mark.parametrize("tile,late", [(0, POLLS), (2000, 0)])
+def test_weight_gradient_gives_up(cuda, lib, dim, full, value, cin, cout, tile, late):
+    """Above 128 outputs only the weight gradient waits: on its stages, and (`late`) for a free one."""
+    call = adjoint(lib, cuda, dim, full, value, cin, cout, activation=False)
+    expected = call.run()[:3]
+    got = call.run(tile=tile, late=late)
+    assert torch.equal(got[0], expected[0])
+    if tile and full == 3:  # one stage: there is none to free
+        assert fault(lib) == 0 and all(map(torch.equal, got, expected))
+    else:
+        recovers(call, lib, expected)
+
+
 def test_polls_are_bounded(lib):
     assert lib.flashns_b200_layer_wait_polls(POLLS + 1, 1) == 1 and lib.flashns_b200_layer_wait_polls(1, POLLS + 1) == 1
