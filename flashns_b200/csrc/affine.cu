@@ -1487,9 +1487,9 @@ int flashns_b200_affine(int dim, int activation, const double* hidden, const dou
   if (count == 0) return int(cudaSuccess);
   if (!hidden || !weight || !bias || !out) return int(cudaErrorInvalidValue);
   const size_t in = size_t(count) * cin * sizeof(double), bytes = size_t(count) * cout * sizeof(double);
-  if (ranges_overlap(out, bytes, hidden, in) || ranges_overlap(out, bytes, residual, bytes) ||
-      ranges_overlap(activated, bytes, hidden, in) || ranges_overlap(activated, bytes, residual, bytes) ||
-      ranges_overlap(out, bytes, activated, bytes))
+  const size_t weights = size_t(cin) * cout * sizeof(double), small = size_t(cout) * sizeof(double);
+  if (outputs_overlap({{out, bytes}, {activated, bytes}, {aux, size_t(full_points + value_points) * small}},
+                      {{hidden, in}, {weight, weights}, {bias, small}, {residual, bytes}}))
     return int(cudaErrorInvalidValue);
   // TMA boxes: rows on 16-byte boundaries, row numbers that fit their 32-bit coordinate
   const bool boxes = cin % 2 == 0 && aligned16(hidden) && count < INT_MAX - 1024;
@@ -1531,11 +1531,13 @@ int flashns_b200_affine_vjp(int dim, int activation, const double* hidden, const
   if (!hidden || !weight || !seed || !d_hidden || !scratch || !aligned16(scratch) || (activation && (!activated || !aux)))
     return int(cudaErrorInvalidValue);
   const size_t in = size_t(count) * cin * sizeof(double), bytes = size_t(count) * cout * sizeof(double);
-  if (ranges_overlap(d_hidden, in, hidden, in) || ranges_overlap(d_hidden, in, seed, bytes) ||
-      ranges_overlap(d_hidden, in, activated, bytes) || ranges_overlap(d_hidden, in, scratch, scratch_bytes))
+  const size_t weights = size_t(cin) * cout * sizeof(double), small = size_t(cout) * sizeof(double);
+  if (outputs_overlap({{d_hidden, in}, {d_weight, weights}, {d_bias, small}, {scratch, scratch_bytes}},
+                      {{hidden, in}, {weight, weights}, {seed, bytes}, {activation ? activated : nullptr, bytes},
+                       {activation ? aux : nullptr, size_t(full_points + value_points) * small}}))
     return int(cudaErrorInvalidValue);
   // at least one share of dW and db, whatever the device
-  if (scratch_bytes < (size_t(cin) + 1) * cout * sizeof(double)) return int(cudaErrorInvalidValue);
+  if (scratch_bytes < weights + small) return int(cudaErrorInvalidValue);
   int sms = 0;
   const cudaError_t e = sm_count(&sms);
   if (e != cudaSuccess) return int(e);

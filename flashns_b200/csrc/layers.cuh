@@ -6,6 +6,7 @@
 #include <climits>
 #include <cstddef>
 #include <cstdint>
+#include <initializer_list>
 #include <mutex>
 
 #include "common.cuh"
@@ -107,6 +108,21 @@ inline bool layer_sizes_ok(int dim, int64_t full, int64_t value, int widest) {
 inline bool ranges_overlap(const void* a, size_t na, const void* b, size_t nb) {
   const auto pa = reinterpret_cast<uintptr_t>(a), pb = reinterpret_cast<uintptr_t>(b);
   return a && b && na && nb && (pa <= pb ? pb - pa < na : pa - pb < nb);
+}
+
+struct Span {
+  const void* at;  // null: no such tensor
+  size_t bytes;
+};
+// whether an output (or the scratch) lies over an input or another output
+inline bool outputs_overlap(std::initializer_list<Span> outputs, std::initializer_list<Span> inputs) {
+  for (const Span* o = outputs.begin(); o != outputs.end(); ++o) {
+    for (const Span& i : inputs)
+      if (ranges_overlap(o->at, o->bytes, i.at, i.bytes)) return true;
+    for (const Span* other = outputs.begin(); other != o; ++other)
+      if (ranges_overlap(o->at, o->bytes, other->at, other->bytes)) return true;
+  }
+  return false;
 }
 
 inline cudaError_t sm_count(int* sms) {

@@ -701,9 +701,7 @@ int flashns_b200_layer_norm(int dim, const double* value, const double* gain, co
   if (!value || !gain || !bias || !out || !stats) return int(cudaErrorInvalidValue);
   const size_t bytes = size_t(count) * channels * sizeof(double), small = size_t(channels) * sizeof(double);
   const size_t stat = size_t(count) * 2 * sizeof(double);
-  if (ranges_overlap(out, bytes, value, bytes) || ranges_overlap(stats, stat, value, bytes) ||
-      ranges_overlap(out, bytes, stats, stat) || ranges_overlap(out, bytes, gain, small) ||
-      ranges_overlap(out, bytes, bias, small))
+  if (outputs_overlap({{out, bytes}, {stats, stat}}, {{value, bytes}, {gain, small}, {bias, small}}))
     return int(cudaErrorInvalidValue);
   int sms = 0;
   cudaError_t e = sm_count(&sms);
@@ -740,9 +738,8 @@ int flashns_b200_layer_norm_vjp(int dim, const double* value, const double* gain
   }
   if (!value || !gain || !stats || !seed || !d_value || !scratch) return int(cudaErrorInvalidValue);
   const size_t bytes = size_t(count) * channels * sizeof(double), stat = size_t(count) * 2 * sizeof(double);
-  if (ranges_overlap(d_value, bytes, value, bytes) || ranges_overlap(d_value, bytes, seed, bytes) ||
-      ranges_overlap(d_value, bytes, skip, bytes) || ranges_overlap(d_value, bytes, stats, stat) ||
-      ranges_overlap(d_value, bytes, scratch, scratch_bytes))
+  if (outputs_overlap({{d_value, bytes}, {d_gain, small}, {d_bias, small}, {scratch, scratch_bytes}},
+                      {{value, bytes}, {gain, small}, {stats, stat}, {seed, bytes}, {skip, bytes}}))
     return int(cudaErrorInvalidValue);
   int sms = 0;
   cudaError_t e = sm_count(&sms);

@@ -198,3 +198,37 @@ def test_layer_hooks_refuse_host_and_narrow_tensors():
                  lambda: nat.affine_activation_vjp(layout, x, w, x, aux, x)):
         with pytest.raises(ValueError, match="CUDA FP64"):
             call()
+
+
+def test_layer_entry_points_refuse_every_overlap_of_an_output():
+    """An output or the scratch over any input or any other output, from the same address to the
+    last byte: cudaErrorInvalidValue (1) before any device call; the pointers are never dereferenced."""
+    from flashns_b200 import _lib, build
+    build.build()
+    lib = _lib.library()
+    full, value, cin, cout, scratch = 3, 2, 8, 4, 1 << 20
+    rows, points = full * 10 + value, full + value
+    # (argument, doubles, is written), in the order of the call
+    norm = [("value", rows * cin, 0), ("gain", cin, 0), ("bias", cin, 0), ("out", rows * cin, 1), ("stats", rows * 2, 1)]
+    norm_vjp = [("value", rows * cin, 0), ("gain", cin, 0), ("stats", rows * 2, 0), ("seed", rows * cin, 0),
+                ("skip", rows * cin, 0), ("d_value", rows * cin, 1), ("d_gain", cin, 1), ("d_bias", cin, 1),
+                ("scratch", scratch // 8, 1)]
+    affine = [("hidden", rows * cin, 0), ("weight", cout * cin, 0), ("bias", cout, 0), ("residual", rows * cout, 0),
+              ("out", rows * cout, 1), ("activated", rows * cout, 1), ("aux", points * cout, 1)]
+    affine_vjp = [("hidden", rows * cin, 0), ("weight", cout * cin, 0), ("activated", rows * cout, 0),
+                  ("aux", points * cout, 0), ("seed", rows * cout, 0), ("d_hidden", rows * cin, 1),
+                  ("d_weight", cout * cin, 1), ("d_bias", cout, 1), ("scratch", scratch // 8, 1)]
+    calls = [(norm, lambda p: lib.flashns_b200_layer_norm(2, *p, 1e-5, full, value, cin, None)),
+             (norm_vjp, lambda p: lib.flashns_b200_layer_norm_vjp(2, *p, scratch, full, value, cin, None)),
+             (affine, lambda p: lib.flashns_b200_affine(2, 1, *p, full, value, cin, cout, None)),
+             (affine_vjp, lambda p: lib.flashns_b200_affine_vjp(2, 1, *p, scratch, full, value, cin, cout, None))]
+    for arguments, call in calls:
+        for i, (name, size, written) in enumerate(arguments):
+            for j, (other, length, also) in enumerate(arguments):
+                if i == j or not written or (also and j > i):
+                    continue
+                # the scratch stays on a 16-byte boundary
+                for at in {0, 8 * (length - 1) // 16 * 16, -(8 * (size - 1) // 16 * 16)}:
+                    p = [(k + 1) << 24 for k in range(len(arguments))]
+                    p[i] = p[j] + at
+                    assert call(p) == 1, (name, other, at)
