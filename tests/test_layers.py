@@ -232,3 +232,22 @@ def test_layer_entry_points_refuse_every_overlap_of_an_output():
                     p = [(k + 1) << 24 for k in range(len(arguments))]
                     p[i] = p[j] + at
                     assert call(p) == 1, (name, other, at)
+
+
+@pytest.mark.parametrize("groups", [2, 3, 4])
+def test_affine_turns_end_for_every_tile_count(groups):
+    """The forward kernels' groups take turns by the protocol of the evaluation's: group g of block b
+    has the tiles b + (g + groups k) per, which are the block's tiles g, g + groups, ..., so every
+    order of the groups ends with no arrival pending."""
+    import itertools
+    from tests.test_turn_protocol import count, run
+    for blocks, tiles in itertools.product((1, 3), range(0, 40)):
+        per = min(max(tiles, 1), blocks)
+        for b in range(per):
+            mine = len(range(b, tiles, per))
+            for g in range(groups):
+                first, step = b + g * per, per * groups
+                assert ((tiles - 1 - first) // step + 1 if first < tiles else 0) == count(mine, g, groups)
+    for order in itertools.permutations(range(groups)):
+        for m in range(0, 40):
+            run(m, order, groups)

@@ -497,3 +497,93 @@ def test_residual_net_on_the_hooks_matches_nested_differentiation(cuda, width, i
     assert set(grads) == set(expected)
     for k in expected:
         assert rel_norm(grads[k].cpu(), expected[k]) <= 1e-10, k
+
+
+# Odd or wide inputs (four, three or two groups of warps by turns) with several tiles for every group
+# and one more for some, both ways round; dW with several stages a block, asked for by TMA or not.
+@pytest.mark.parametrize("dim,full,value,cin,cout", [(2, 5003, 41, 33, 17), (2, 4800, 0, 33, 64), (2, 4000, 900, 130, 64),
+                                                     (2, 3001, 77, 96, 190), (2, 3001, 77, 300, 40), (2, 5001, 13, 65, 191),
+                                                     (3, 4001, 37, 33, 17), (3, 1500, 401, 190, 150), (3, 2600, 77, 258, 40),
+                                                     (3, 2003, 9, 161, 131)])
+@pytest.mark.parametrize("activation", [False, True])
+def test_affine_by_small_groups_matches_oracle_at_many_points(cuda, dim, full, value, cin, cout, activation):
+    check_affine(cuda, dim, full, value, cin, cout, activation)
+
+
+# a stream function's two outputs and two inputs; outputs below a box's 16 columns; widths whose boxes
+# find no room (82 to 112 inputs forward, 74 to 96 outputs backward, above 64 outputs)
+@pytest.mark.parametrize("dim", [2, 3])
+@pytest.mark.parametrize("full,value", [(41, 29), (2101, 333)])
+@pytest.mark.parametrize("cin,cout", [(2, 64), (64, 2), (2, 2), (64, 4), (64, 10), (96, 96), (82, 74), (112, 80), (64, 96),
+                                      (90, 66), (8, 90)])
+def test_affine_at_narrow_widths_and_without_boxes(cuda, dim, full, value, cin, cout):
+    for activation in (False, True):
+        check_affine(cuda, dim, full, value, cin, cout, activation, residual=activation)
+    check_affine(cuda, dim, full, value, cin, cout, True, residual=False)
+
+
+def past_32_bits(cuda, full, value, widths, dim=2):
+    """Random packed rows of these widths, and the trailing points as a small layout of their own:
+    their row count and (full, value).  90 GB are needed."""
+    if torch.cuda.mem_get_info()[0] < 90 << 30:
+        torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 90 << 30:
+        pytest.skip("90 GB of free device memory needed")
+    end = (64, value) if value < 4096 else (0, 4096)
+    rows = full * J.q(dim) + value
+    assert rows * max(widths) > 1 << 31
+    x = torch.empty(rows, widths[0], dtype=torch.float64, device=cuda).uniform_(-1, 1)
+    return x, end[0] * J.q(dim) + end[1], end
+
+
+@pytest.mark.parametrize("full,value,cin,cout", [(3_400_003, 5, 8, 64), (1_003, 33_600_000, 8, 64), (3_400_003, 5, 64, 8),
+                                                 (3_300_003, 7, 8, 66), (1_700_003, 3, 8, 130)])
+def test_full_points_and_kept_values_past_32_bits(cuda, full, value, cin, cout):
+    """More than 2^31 values with full points, `activated` and `aux` kept, through the adjoint: the
+    last points match the oracle.  The seed is zero but there, so that the weight and bias gradients
+    are sums over them alone and their bound is as tight as at that size."""
+    x, tail, (e_full, e_value) = past_32_bits(cuda, full, value, (cin, cout))
+    f64 = dict(dtype=torch.float64, device=cuda)
+    nat, layout = parts(2, full, value)
+    points = e_full + e_value
+    w, b = torch.randn(cout, cin, **f64) / cin ** 0.5, torch.rand(cout, **f64)
+    h, n_w, n_b = (t.cpu().numpy() for t in (x[-tail:], w, b))
+    _, act, aux = nat.affine_activation(layout, x, w, b)
+    exp, mag = (L.affine(h, n_w, n_b, None, 2, e_full, True, magnitude=v) for v in (False, True))
+    for got, e, m in zip((act[-tail:], act[-tail:], aux[-points:]), exp, mag):
+        assert worst(got.cpu(), e, m, affine_roundings(cin)) <= 1
+    seed = torch.zeros(layout.rows, cout, **f64)
+    seed[-tail:].uniform_(-1, 1)
+    n_act, n_aux, n_seed = (t.cpu().numpy() for t in (act[-tail:], aux[-points:], seed[-tail:]))
+    back = nat.affine_activation_vjp(layout, x, w, act, aux, seed)
+    assert not back[0][:-tail].any()
+    exp, mag = (L.affine_vjp(h, n_w, n_act, n_aux, n_seed, 2, e_full, magnitude=v) for v in (False, True))
+    for got, e, m, n in zip((back[0][-tail:], *back[1:]), exp, mag, (cout, tail, tail)):
+        assert worst(got.cpu(), e, m, affine_vjp_roundings(n)) <= 1
+    del x, act, aux, seed, back, got
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("full,value", [(3_400_003, 5), (1_003, 33_600_000)])
+def test_norm_of_full_points_past_32_bits(cuda, full, value):
+    c = 64
+    x, tail, (e_full, _) = past_32_bits(cuda, full, value, (c,))
+    f64 = dict(dtype=torch.float64, device=cuda)
+    nat, layout = parts(2, full, value)
+    gain, bias = torch.rand(c, **f64), torch.rand(c, **f64)
+    end, n_gain, n_bias = (t.cpu().numpy() for t in (x[-tail:], gain, bias))
+    out, stats = nat.layer_norm(layout, x, gain, bias, eps=EPS)
+    exp, mag = (L.layer_norm(end, n_gain, n_bias, EPS, 2, e_full, magnitude=v) for v in (False, True))
+    for got, e, m in zip((out, stats), exp, mag):
+        assert worst(got[-tail:].cpu(), e, m, norm_roundings(c)) <= 1
+    del out, got
+    seed = torch.zeros_like(x)
+    seed[-tail:].uniform_(-1, 1)
+    n_stats, n_seed = stats[-tail:].cpu().numpy(), seed[-tail:].cpu().numpy()
+    back = nat.layer_norm_vjp(layout, x, gain, stats, seed)
+    assert not back[0][:-tail].any()
+    exp, mag = (L.layer_norm_vjp(end, n_gain, n_stats, n_seed, None, 2, e_full, magnitude=v) for v in (False, True))
+    for got, e, m, n in zip((back[0][-tail:], *back[1:]), exp, mag, (0, tail, tail)):
+        assert worst(got.cpu(), e, m, norm_vjp_roundings(c, n)) <= 1
+    del x, stats, seed, back, got
+    torch.cuda.empty_cache()
