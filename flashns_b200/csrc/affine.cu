@@ -408,7 +408,7 @@ __global__ void __launch_bounds__(NG* GW * 32, 1)
 // access, and the partner's turn covers the group's.  The jets stay inside the turn because
 // DMMA and DFMA share one datapath with DMMA first: outside it they crawl behind the partner's
 // MMAs (16,384 + 4,096 points, 64 -> 64 with residual: 110 us against 88, both with outputs
-// stored by threads; 73 with the boxes below).  A tile is one TMA box of 36 columns for each 32
+// stored by threads; 76 with the boxes below).  A tile is one TMA box of 36 columns for each 32
 // (the 4 more are the padding that frees the fragment loads of bank conflicts).  At that size a
 // turn is 6,500 cycles of MMAs (5,120 at the full rate) and 1,250 of jets.
 constexpr int kTileGroup = 256, kTileSmem = 227 * 1024;
@@ -448,7 +448,10 @@ struct TileMaps {
 // keep the load/store unit busy for 1,400 cycles a tile (5,000 with the residual and a second
 // output), in which the partner's fragment loads, and with them its MMAs, hardly advance.  The
 // boxes have room of their own, or lie in the tile that has been read, whose successor (and the
-// residual) then arrives a little later.
+// residual) then arrives a little later.  Where neither has the room for a group's eight boxes,
+// threads load and store: with more than 64 outputs, layers of 82 to 112 inputs (dH: of 74 to
+// 96 outputs); in 3-D with a residual, which never takes the tile's place, layers from 74 inputs on
+// (82 with more than 64 outputs).
 enum Leave { kByThreads, kInTile, kOwnBoxes };
 constexpr int kBoxDoubles = 40 * 16, kBoxesBytes = 8 * kBoxDoubles * 8;  // a warp's; a group's
 
@@ -776,7 +779,7 @@ cudaError_t launch_forward_tile(const double* hidden, const double* weight, cons
 template <int DIM, bool ACT, typename... Args>
 cudaError_t forward(int cin, int cout, bool values, bool boxes, Args... args) {
   // tanhs of value rows alone (a point a row: the dimension does not matter) go with the small
-  // groups, without turns: 40,401 rows 64 -> 64 take 27 us, in whole tiles 35
+  // groups, without turns: 40,401 rows 64 -> 64 take 29 us, in whole tiles 35
   if constexpr (ACT) {
     if (values) {
       if (cin <= 160) return launch_forward<2, true, 4, 4, 3, false, true, false>(args...);

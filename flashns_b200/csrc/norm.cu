@@ -220,8 +220,9 @@ __global__ void __launch_bounds__(kNormThreads)
 //
 // Measured: 16,384 + 4,096 points, 64 wide: 35 us (0.75 of the copy bandwidth; launch and first
 // loads are 4), the adjoint with a skip 61 (0.87); 3-D 32,768 + 8,192 points, 128 wide: 259
-// (0.81); the 3-D adjoint at 4,099 + 1,031 points, 100 wide: 66 (0.46), bound by the issue of
-// its 8 warps, each of which forms r * r * r and w for its point.
+// (0.81); the 3-D adjoint at 4,099 + 1,031 points, 100 wide: 66 (0.46): its 8 warps, for which
+// there are registers, wait for one another's sums and on latency (0.44 instructions a cycle
+// and scheduler), and each forms r * r * r and w for its point.
 constexpr int kUnitMostLanes = 256;  // lanes of the widest group
 constexpr size_t kUnitSmem = 226 * 1024;
 template <int DIM, bool BACKWARD>

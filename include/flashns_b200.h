@@ -199,8 +199,9 @@ int flashns_b200_residuals(int head, int dim, const double* jets, double nu, dou
 /* ---- layers of a pre-norm residual network on packed jets (norm.cu, affine.cu) ----
  * No reference counterpart.  Rows are packed as in PackedLayout: full_points x Q, then
  * value_points; FP64, contiguous, any channel counts >= 1.  Outputs and scratch may overlap
- * neither an input nor one another (cudaErrorInvalidValue).  Sums run in a fixed order: equal
- * inputs give equal bits.
+ * neither an input nor one another (cudaErrorInvalidValue).  Sums run in an order fixed by the
+ * sizes, the device's multiprocessors and whether tensors start on 16-byte boundaries: with
+ * these equal, equal inputs give equal bits.
  *
  * Layer norm over the channels, exact through the jets: D = X - mean, r = (mean D * D +
  * eps)^(-1/2) with the truncated product *, out = gain (r * D) + bias (order-0 rows); a value
